@@ -19,6 +19,9 @@
  *   fa_block_tables_from_lists <- BlockMask fields      src/pallas_flexattn/block_mask.py:16-51
  *   fa_lse_merge         <- (no counterpart; combine step of the context-parallel ring)
  *   fa_decode            <- (no counterpart; split-KV decode against a K/V cache)
+ *   fa_rotary            <- (no counterpart; rotary positions of q and k, and their gradient)
+ *   fa_paged_append      <- (no counterpart; new keys and values into a paged K/V cache)
+ *   fa_paged_attn        <- (no counterpart; attention against a paged, possibly 8-bit cache)
  */
 #ifndef FLEXATTN_H_
 #define FLEXATTN_H_
@@ -47,7 +50,8 @@ enum {
   FA_ERR_TIMEOUT = 4,     /* a device-side bounded wait gave up */
 };
 
-enum { FA_DTYPE_F32 = 0, FA_DTYPE_BF16 = 1 };
+enum { FA_DTYPE_F32 = 0, FA_DTYPE_BF16 = 1,
+       FA_DTYPE_E4M3 = 2 /* paged caches only: 8-bit, 4 exponent and 3 fraction bits */ };
 
 /* Which kernel family runs the attention tiles. */
 enum {
@@ -289,6 +293,100 @@ typedef struct {
 /* Bytes of device workspace fa_decode needs (the chunks' partial o and lse). */
 FA_API int fa_decode_workspace_size(const FaDecodeParams* p, size_t* bytes);
 FA_API int fa_decode(const FaDecodeParams* p, void* workspace, size_t workspace_bytes, fa_stream_t stream);
+
+/* ------------------------------------------------------------------ rotary positions
+ * Pair i of the first rotary_dim elements of a head row at position p is turned by the angle
+ * 2 pi p turns[i] / 2^64 and scaled by `magnitude`:
+ *     (a, b) -> magnitude (a cos - b sin, b cos + a sin)
+ * The pairs are (x[i], x[i + rotary_dim / 2]) or, interleaved, (x[2i], x[2i + 1]); elements
+ * from rotary_dim on are copied.  turns[] holds the fraction of a turn per position as 64-bit
+ * fixed point, so p * turns[i] mod 2^64 is the exact phase at any 32-bit position. */
+enum { FA_ROTARY_HALF = 0, FA_ROTARY_INTERLEAVED = 1 };
+
+typedef struct {
+  int32_t rotary_dim;    /* even, <= D; 0 = no rotation (a copy) */
+  int32_t layout;        /* FA_ROTARY_* */
+  const uint64_t* turns; /* [rotary_dim / 2] device */
+  float magnitude;
+} FaRotarySpec;
+
+typedef struct {
+  int32_t dtype;            /* FA_DTYPE_BF16 or FA_DTYPE_F32, of all four tensors */
+  int32_t B, H, H_kv, T, D; /* H or H_kv may be 0: that tensor is not touched */
+  FaTensor q, k;            /* [B, H, T, D], [B, H_kv, T, D] */
+  FaTensor q_out, k_out;    /* may be q and k themselves */
+  const int32_t* positions; /* [B, T] device int32 (any sign), or NULL: pos_offset + t */
+  int64_t pos_stride_b;     /* elements between batches; 0 = shared */
+  int32_t pos_offset;
+  int32_t inverse;          /* 1 = the transposed rotation (the gradient's) */
+  FaRotarySpec rotary;
+} FaRotaryParams;
+
+FA_API int fa_rotary(const FaRotaryParams* p, fa_stream_t stream);
+
+/* ------------------------------------------------------------------ paged K/V cache
+ * k, v: [num_pages, H_kv, page_size, D] (FaTensor strides: page, head, row).  Cached position
+ * j of sequence b is row j % page_size of page block_table[b][j / page_size].  An e4m3 cache
+ * holds codes with one scale per page and K/V head: value = code * scale.  fa_paged_append
+ * makes the scales powers of two, so that rescaling a page only loses what falls below the
+ * 8-bit type's smallest step. */
+typedef struct {
+  int32_t dtype;             /* FA_DTYPE_BF16 or FA_DTYPE_E4M3 */
+  int32_t num_pages, H_kv, page_size, D; /* page_size in {16, 32, 64, 128}; D in {64, 128, 256} */
+  FaTensor k, v;
+  float* k_scale;            /* [num_pages, H_kv] contiguous; e4m3 only */
+  float* v_scale;
+  const int32_t* block_table; /* [B, table_cols] device page numbers */
+  int32_t table_cols;
+  int64_t table_stride;       /* elements between sequences */
+} FaPagedCache;
+
+/* Append: token i < new_lens[b] of sequence b goes to position kv_lens[b] - new_lens[b] + i;
+ * kv_lens counts the sequence with its new tokens.  k is rotated on the way when
+ * rotary.rotary_dim > 0, and so is q into q_out (rows i >= new_lens[b] of q_out become 0) when
+ * q.ptr is given.  e4m3: a page's scale becomes the larger of its scale (if the page already
+ * holds rows of the sequence) and the least power of two >= (largest finite new magnitude) / 448;
+ * when it grows, the rows held are requantised.  Magnitudes above 448 * scale (infinities) are
+ * stored as +-448, NaN as NaN.  Rows behind the new tokens are left as they were.
+ * A page that is written must belong to one sequence of the call only.
+ * Lengths or page numbers out of range write nothing (that sequence, that page) and set
+ * *status to FA_ERR_INVALID. */
+typedef struct {
+  int32_t dtype;            /* of q, k, v, q_out: FA_DTYPE_BF16 or FA_DTYPE_F32 */
+  int32_t B, H, T;          /* H may be 0 (no q) */
+  FaTensor q, k, v, q_out;  /* [B, H, T, D], [B, H_kv, T, D] */
+  const int32_t* kv_lens;   /* [B] device */
+  const int32_t* new_lens;  /* [B] device, or NULL: T */
+  FaRotarySpec rotary;      /* rotary_dim a multiple of 16 */
+  FaPagedCache cache;
+  int32_t* status;
+} FaPagedAppendParams;
+
+FA_API int fa_paged_append(const FaPagedAppendParams* p, fa_stream_t stream);
+
+/* Attention of Tq query rows per sequence against the cache.  Row i < q_lens[b] sits at position
+ * kv_lens[b] - q_lens[b] + i; rows from q_lens[b] on are padding and get o = 0, lse = -inf, as
+ * do rows that see no key.  Any Tq (a decode step, drafted tokens, a chunk of a prompt).
+ * bf16 q and o; mask flags CAUSAL / WINDOW; score flags ALIBI / SOFTCAP.  The cached positions
+ * of all sequences are dealt out evenly over the SMs, whatever their lengths; parts of one
+ * sequence on several SMs meet in the workspace and are joined by a second kernel.  A page
+ * number out of range hides its positions and sets *status to FA_ERR_INVALID, as does a length
+ * beyond table_cols * page_size (which is cut). */
+typedef struct {
+  int32_t B, H, Tq;
+  FaTensor q, o;           /* [B, H, Tq, D] bf16 */
+  float* lse;              /* [B, H, Tq] fp32 natural-log logsumexp, contiguous */
+  const int32_t* kv_lens;  /* [B] device */
+  const int32_t* q_lens;   /* [B] device, or NULL: Tq */
+  float scale;
+  FaMaskSpec mask;         /* q_offset / kv_offset must be 0 */
+  FaScoreSpec score;
+  FaPagedCache cache;
+  int32_t* status;
+} FaPagedAttnParams;
+
+FA_API int fa_paged_attn_workspace_size(const FaPagedAttnParams* p, size_t* bytes);
+FA_API int fa_paged_attn(const FaPagedAttnParams* p, void* workspace, size_t workspace_bytes, fa_stream_t stream);
 
 #ifdef __cplusplus
 }

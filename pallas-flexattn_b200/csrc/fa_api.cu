@@ -166,6 +166,22 @@ int make_row_tile_map(CUtensorMap* map, const FaTensor& t, int dtype, int B, int
   return FA_OK;
 }
 
+int make_page_map(CUtensorMap* map, const FaPagedCache& c, const FaTensor& t, const char* name) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(FA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int es = c.dtype == FA_DTYPE_E4M3 ? 1 : 2, span = c.D * es < 128 ? 64 : 128;
+  cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)c.page_size, (cuuint64_t)c.H_kv, (cuuint64_t)c.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)t.stride_t * es, (cuuint64_t)t.stride_h * es, (cuuint64_t)t.stride_b * es};
+  cuuint32_t box[4] = {(cuuint32_t)(span / es), (cuuint32_t)c.page_size, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.ptr, dims,
+                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FA_ERR_INVALID, "tensor map for %s rejected (CUresult %d)", name, (int)r);
+  return FA_OK;
+}
+
 }  // namespace fa
 
 using namespace fa;

@@ -44,4 +44,10 @@ cudaError_t launch_tables_from_lists(int num_b, int nq, int nkv, const int32_t* 
                                      const int32_t* full_num, const int32_t* full_idx, int kv_cap,
                                      const FaBlockMaskOut& out, cudaStream_t stream);
 
+// 4-D tensor map over a page pool [num_pages, H_kv, page_size, D]: box = one panel (128 bytes of a
+// row, 64 where a row is shorter) x the rows of a page, swizzled over the panel's width.
+int make_page_map(CUtensorMap* map, const FaPagedCache& c, const FaTensor& t, const char* name);
+// Checks of a paged cache shared by fa_paged_append and fa_paged_attn (fa_rotary.cu).
+int check_paged_cache(const FaPagedCache& c, int B, const char* who);
+
 }  // namespace fa

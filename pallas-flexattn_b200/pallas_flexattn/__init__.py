@@ -13,6 +13,15 @@ from .flash_attn import (
     mha_reference,
 )
 from .decode import flash_attention_decode
+from .paged import PagedKVCache, flash_attention_paged, paged_kv_append
+from .rotary import (
+    RotarySpec,
+    by_parts_scaling,
+    linear_scaling,
+    ntk_scaling,
+    rotary_embedding,
+    rotary_spec,
+)
 from .mask_mod import (
     MaskMod,
     and_masks,
@@ -72,4 +81,13 @@ __all__ = [
     "compose_score_mods",
     "autotune",
     "check_device_status",
+    "rotary_embedding",
+    "rotary_spec",
+    "RotarySpec",
+    "linear_scaling",
+    "ntk_scaling",
+    "by_parts_scaling",
+    "PagedKVCache",
+    "paged_kv_append",
+    "flash_attention_paged",
 ]

@@ -12,7 +12,8 @@ import os
 from pathlib import Path
 
 FA_OK, FA_ERR_INVALID, FA_ERR_UNSUPPORTED, FA_ERR_CUDA, FA_ERR_TIMEOUT = 0, 1, 2, 3, 4
-FA_DTYPE_F32, FA_DTYPE_BF16 = 0, 1
+FA_DTYPE_F32, FA_DTYPE_BF16, FA_DTYPE_E4M3 = 0, 1, 2
+FA_ROTARY_HALF, FA_ROTARY_INTERLEAVED = 0, 1
 FA_KERNEL_AUTO, FA_KERNEL_TC, FA_KERNEL_SIMT = 0, 1, 2
 FA_MASK_CAUSAL, FA_MASK_WINDOW, FA_MASK_DOCUMENT, FA_MASK_TILE_TABLE, FA_MASK_DOC_SORTED = 1, 2, 4, 8, 16
 FA_MASK_BITMASK = 32
@@ -181,6 +182,88 @@ class FaBlockMaskOut(C.Structure):
     ]
 
 
+class FaRotarySpec(C.Structure):
+    _fields_ = [
+        ("rotary_dim", C.c_int32),
+        ("layout", C.c_int32),
+        ("turns", C.c_void_p),
+        ("magnitude", C.c_float),
+    ]
+
+
+class FaRotaryParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("B", C.c_int32),
+        ("H", C.c_int32),
+        ("H_kv", C.c_int32),
+        ("T", C.c_int32),
+        ("D", C.c_int32),
+        ("q", FaTensor),
+        ("k", FaTensor),
+        ("q_out", FaTensor),
+        ("k_out", FaTensor),
+        ("positions", C.c_void_p),
+        ("pos_stride_b", C.c_int64),
+        ("pos_offset", C.c_int32),
+        ("inverse", C.c_int32),
+        ("rotary", FaRotarySpec),
+    ]
+
+
+class FaPagedCache(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("H_kv", C.c_int32),
+        ("page_size", C.c_int32),
+        ("D", C.c_int32),
+        ("k", FaTensor),
+        ("v", FaTensor),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("block_table", C.c_void_p),
+        ("table_cols", C.c_int32),
+        ("table_stride", C.c_int64),
+    ]
+
+
+class FaPagedAppendParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("B", C.c_int32),
+        ("H", C.c_int32),
+        ("T", C.c_int32),
+        ("q", FaTensor),
+        ("k", FaTensor),
+        ("v", FaTensor),
+        ("q_out", FaTensor),
+        ("kv_lens", C.c_void_p),
+        ("new_lens", C.c_void_p),
+        ("rotary", FaRotarySpec),
+        ("cache", FaPagedCache),
+        ("status", C.c_void_p),
+    ]
+
+
+class FaPagedAttnParams(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32),
+        ("H", C.c_int32),
+        ("Tq", C.c_int32),
+        ("q", FaTensor),
+        ("o", FaTensor),
+        ("lse", C.c_void_p),
+        ("kv_lens", C.c_void_p),
+        ("q_lens", C.c_void_p),
+        ("scale", C.c_float),
+        ("mask", FaMaskSpec),
+        ("score", FaScoreSpec),
+        ("cache", FaPagedCache),
+        ("status", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); the exported surface of include/flexattn.h
 EXPORTS = {
     "fa_version": (C.c_char_p, []),
@@ -202,6 +285,10 @@ EXPORTS = {
     ),
     "fa_decode_workspace_size": (C.c_int, [C.POINTER(FaDecodeParams), C.POINTER(C.c_size_t)]),
     "fa_decode": (C.c_int, [C.POINTER(FaDecodeParams), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fa_rotary": (C.c_int, [C.POINTER(FaRotaryParams), C.c_void_p]),
+    "fa_paged_append": (C.c_int, [C.POINTER(FaPagedAppendParams), C.c_void_p]),
+    "fa_paged_attn_workspace_size": (C.c_int, [C.POINTER(FaPagedAttnParams), C.POINTER(C.c_size_t)]),
+    "fa_paged_attn": (C.c_int, [C.POINTER(FaPagedAttnParams), C.c_void_p, C.c_size_t, C.c_void_p]),
     "fa_lse_merge": (
         C.c_int,
         [C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p],

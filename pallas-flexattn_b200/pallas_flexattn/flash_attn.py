@@ -60,7 +60,8 @@ _STATUS: dict = {}
 
 
 def device_status(device) -> torch.Tensor:
-    """Per-device int32 the kernels set when a bounded device-side wait gives up."""
+    """Per-device int32 that kernels set: FA_ERR_TIMEOUT when a bounded device-side wait gives up,
+    FA_ERR_INVALID when a length or page number on the device is out of range."""
     device = torch.device(device)
     k = str(device)
     if k not in _STATUS:
@@ -69,12 +70,14 @@ def device_status(device) -> torch.Tensor:
 
 
 def check_device_status(device=None) -> None:
-    """Synchronise and raise if any kernel on `device` reported a timeout."""
+    """Synchronise and raise if any kernel on `device` reported a timeout or an invalid length or page."""
     device = torch.device(device if device is not None else "cuda")
     st = device_status(device)
     v = int(st.item())
     if v:
         st.zero_()
+        if v == L.FA_ERR_INVALID:
+            raise L.FlexAttnError(v, "a length or page number read on the device was out of range (it was skipped)")
         raise L.FlexAttnError(v, "a device-side wait timed out (kernel aborted its tile)")
 
 
