@@ -6,24 +6,27 @@
 // chunk is bound by the tensor cores and the exponentials.
 //
 // Orientation.  The 128 cached positions of a tile are the MMA's M, the query rows its N:
-//     S^T [128 positions x N] = K Q^T       A = K as stored (K-major), B = Q
-//     O^T [D x N]            += V^T P^T     A = V as stored (M-major), B = P from shared memory
-// so the exponentials are spent on real query rows only (N is 8 to 64 of them; with the rows as M
+//     S^T [128 positions x R] = K Q^T       A = K as stored (K-major), B = Q
+//     O^T [D x R]            += V^T P^T     A = V as stored (M-major), B = P from shared memory
+// so the exponentials are spent on real query rows only (R is 8 to 64 of them; with the rows as M
 // they would be padded to 128), and each thread owns one position: its page's scales are two
 // registers.
 //
 // 8-bit codes go to the tensor cores as they are (kind::f8f6f4): converting a tile in shared memory
 // would cost as many instructions as everything else here.  The other operand is split into two e4m3
-// parts side by side in N, z = hi + lo / 16: q is scaled by a power of two per row so that its largest
-// magnitude lies in [128, 256); a bf16 has 8 significant bits, each part 4, so the split is exact
-// down to 2^-20 of the row's largest element.  Probabilities lie in [0, 256] and keep a relative
-// error of 2^-9 (the bf16 path rounds them to 2^-9 too); what is lost below 2^-14 of the largest
-// is below the sums' own rounding.  Both products accumulate in fp32.
+// parts, z = hi + lo, that meet in the fp32 accumulator: both parts' MMAs add to the same columns
+// (R >= 16), or for R = 8 the parts lie side by side in the MMA's smallest N of 16, with lo held
+// times 16, and are added when read.  q is scaled by a power of two per row so that its largest
+// magnitude lies in [128, 256): a bf16 has 8 significant bits, each part 4, so the split is exact
+// down to 2^-17 of the row's largest element.  Probabilities lie in [0, 431] with a largest one
+// of at least 128 / 431 of that: the split is off by 2^-8 relative (as a bf16 P is), or 2^-17 of the
+// largest below that.
 //
-// Scales.  ks multiplies the thread's logits.  vs goes into the probabilities: P = 2^(x + log2 vs -
-// my + 4) with a reference my of its own per row, so that a row whose weight sits on pages of small
-// values keeps its precision.  The softmax sum uses x - mx.  Both references move only when a tile
-// exceeds them by more than 4 (log2 units), one barrier vote per tile.
+// Scales.  ks multiplies the thread's logits.  vs goes into the exponent: with z = x + log2 vs and
+// a reference m >= max z - 1.75 per row, P = 2^(z - m + 7) weighs the codes, and the softmax sum
+// adds P / vs; o = sum P code / sum (P / vs).  So a row whose weight sits on pages of small values
+// keeps its precision.  The reference moves only when a tile exceeds it by more than 1.75: one
+// barrier vote per tile.
 //
 // Work.  The tiles of all (sequence, row group, K/V head) units, in that order, are cut into equal
 // contiguous ranges, one per CTA (one CTA per SM): ragged batches balance themselves, and nothing
@@ -31,8 +34,12 @@
 // that crosses CTAs leaves at most one partial (o, lse) at each end of a CTA's range in the
 // workspace, joined by paged_merge_kernel in CTA order.
 //
-// Warps: 0-3 softmax (thread = position of the tile; later = element of D), 4 TMA producer (lane =
-// page of the tile), 5 MMA issue, 6-7 build the next unit's Q operand and row constants.
+// Warps: softmax groups of four (thread = position of a tile; at the end = element of D), then one
+// that produces (lane = page of a tile), one that issues S, one that issues P V, and one that builds
+// the next unit's Q operand and row constants.  Up to 16 rows there are two groups that take the tiles
+// in turn, each with its own O, references and sums, joined when the unit ends: a tile's chain
+// (wait, TMEM read, vote, exponentials, store, fence) takes longer than its bytes take to arrive, so
+// two tiles have to be in work at once.  With more rows each group takes 16 of them.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -50,12 +57,12 @@ namespace fa {
 namespace {
 
 constexpr int kTile = 128;         // cached positions of a tile: the MMA's M
-constexpr int kPThreads = 256;
 constexpr int kSms = 148;
 constexpr int kMaxSlots = 24;      // K or V tiles in the shared-memory ring
-constexpr int kScaleRing = kMaxSlots / 2 + 4;  // tiles whose scales may be live at once
-constexpr float kSlack = 4.f;      // a reference moves when exceeded by this much (log2 units)
-constexpr float kLift = 4.f;       // 8-bit P is 2^(x - reference + kLift) <= 2^(kSlack + kLift)
+constexpr int kScaleRing = 16;     // tiles whose scales may be live at once (> kMaxSlots / 2 + 1)
+constexpr float kSlack = 1.75f;    // a reference moves when exceeded by more than this (log2 units)
+constexpr float kLift = 7.f;       // P = 2^(z - reference + kLift) <= 2^8.75 = 431: below e4m3's 448
+constexpr float kUnset = -1e30f;   // reference of a row that has seen nothing yet
 
 struct PagedArgs {
   int B, H, Hkv, Tq, G, M;         // M = G * Tq query rows per sequence and K/V head
@@ -79,22 +86,30 @@ struct PagedArgs {
 
 template <int D, int ES, int R>
 struct Shape {
-  static constexpr int N = ES == 1 ? 2 * R : R;     // columns of S and O: hi and lo parts, or rows
+  static constexpr bool SIDE = ES == 1 && R == 8;   // hi and lo parts side by side in N
+  static constexpr bool TURNS = R <= 16;            // the softmax groups take tiles in turn, else 16 rows each
+  static constexpr int NG = TURNS ? 2 : R / 16;     // softmax groups
+  static constexpr int NSM = 128 * NG;              // softmax threads
+  static constexpr int NT = NSM + 128;
+  static constexpr int N = SIDE ? 16 : R;           // columns of S and O
+  static constexpr int C = R < 16 ? R : 16;         // rows per softmax thread
+  static constexpr int PARTS = ES == 1 && !SIDE ? 2 : 1;  // operands of Q and P (hi, lo)
   static constexpr int ROWB = D * ES;               // bytes of one cached position
   static constexpr int SW = ROWB < 128 ? 64 : 128;  // swizzle span
   static constexpr int PANEL = kTile * SW;
   static constexpr int SLOT = kTile * ROWB;
   static constexpr int QPANEL = N * SW;
-  static constexpr int QBUF = N * ROWB;
-  static constexpr int PBUF = N * kTile * ES;
+  static constexpr int QPART = N * ROWB, QBUF = PARTS * QPART;
+  static constexpr int PPART = N * kTile * ES, PBUF = PARTS * PPART;
   static constexpr int NO = D <= 128 ? 1 : D / 128; // blocks of 128 elements of O
-  static constexpr uint32_t TM_O = 2 * N;           // TMEM: two S buffers, then O
-  static constexpr int USED = (2 + NO) * N;
+  static constexpr int ON = NO * N;                 // TMEM columns of one O
+  static constexpr uint32_t TM_O = 2 * N;           // TMEM: two S buffers, then one O or one per group
+  static constexpr int USED = 2 * N + (TURNS ? 2 : 1) * ON;
   static constexpr uint32_t TM_COLS = USED <= 32 ? 32 : USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
-  static_assert(USED <= 512 && N % 16 == 0 && N <= 256, "operand shape");
+  static_assert(USED <= 512 && N % 16 == 0 && N <= 256 && (ES == 1 || R >= 16), "operand shape");
 };
 
-// Row constants of one unit, built by warps 6-7 (double-buffered with Q).
+// Row constants of one unit (double-buffered with Q).
 template <int R> struct RowConst {
   float xs[R];      // logit = dot * (ks * xs): scale, the row's power of two, and log2(e) unless softcapped
   float slope[R];   // ALiBi slope in the same domain
@@ -103,21 +118,20 @@ template <int R> struct RowConst {
   int64_t orow[R];  // element offset of the row in o, -1: no such row
   int64_t lrow[R];  // index of the row in lse
 };
-// Running state of the unit in work, and scratch of the softmax warps.
-template <int R> struct RowState {
-  float mx[R], my[R];          // references of the sum and of O (log2 units), -inf at first
-  float mref[R], thx[R], thy[R], w[R];  // mx or 0; mx + slack; my + slack; 2^(mref - my + lift)
-  float al[R], ao[R];          // factors of the last move
-  float fin[R];                // factor of O at the end
-  float red[4][2][R];
+// Running state of one softmax group: its rows, or its share of the tiles.
+struct RowState {
+  float m[16], bias[16];  // reference; kLift - reference
+  float move[16];         // factor of the last move
+  float red[4][16];
+  float fin[16];          // factor of O at the end
 };
 template <int R> struct Smem {
   RowConst<R> rc[2];
-  RowState<R> rs;
+  RowState rs[R <= 16 ? 2 : R / 16];
   float2 scales[kScaleRing][8];  // (ks, vs) of a tile's pages; ks = -inf hides the page
-  int odd[kScaleRing];           // the tile has a hidden page
-  uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], fin_bar;
-  int scan[8];
+  int odd[kScaleRing];           // the tile has a hidden page, or one of a scale below 2^-100
+  uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], fin_bar[2];
+  int scan[24];
   int total, per_cta, first_entry, first_off;
   uint32_t tmem;
   int abort_flag, never;
@@ -191,15 +205,18 @@ struct Walker {
       off = entry_off - hk * e.nt;
     }
   }
-  __device__ __forceinline__ bool next(const PagedArgs& a, Seg* s) {
-    if (left <= 0) return false;
-    while (off >= e.nt) {  // the unit is done: the next head, or the next entry that has tiles
-      off = 0;
-      if (e.nt > 0 && ++hk < a.Hkv) break;
+  // Moves tiles beyond a unit's end on into the next head, or the next entry that has tiles.
+  __device__ __forceinline__ void settle(const PagedArgs& a) {
+    while (off >= e.nt) {
+      off -= e.nt;
+      if (e.nt > 0 && ++hk < a.Hkv) continue;
       hk = 0;
       e = entry_of<R>(a, ++idx);
-      if (e.nt > 0) break;
     }
+  }
+  __device__ __forceinline__ bool next(const PagedArgs& a, Seg* s) {
+    if (left <= 0) return false;
+    settle(a);
     s->hk = hk;
     s->t0 = e.t0 + off;
     s->nt = min(e.nt - off, left);
@@ -210,6 +227,25 @@ struct Walker {
     return true;
   }
 };
+
+// mbar_wait that looks at the clock only now and then: most waits here are short.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 15u) == 0u) {
+      if (*abort_flag) return false;
+      const uint64_t t = globaltimer_ns();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > FA_WAIT_TIMEOUT_NS) return false;
+    }
+  }
+}
+__device__ __forceinline__ bool wait_for_w(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const int ok = wait_for(bar, parity, abort_flag) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
 
 __device__ __forceinline__ bool vote_or(int id, int nthreads, bool pred) {
   uint32_t r;
@@ -224,21 +260,25 @@ __device__ __forceinline__ bool vote_or(int id, int nthreads, bool pred) {
   return r != 0;
 }
 
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+__device__ __forceinline__ uint32_t e4m3x2(__half2 v) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
   return r;
 }
-__device__ __forceinline__ float2 e4m3x2_value(uint32_t v) {
+__device__ __forceinline__ __half2 e4m3x2_value(uint32_t v) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return *reinterpret_cast<const __half2*>(&h);
 }
-// Two values as hi + lo / 16: the packed hi parts, and the lo parts through *lo2.
+// Two values of magnitude up to 448 as hi + lo (lo held times 16 if X16): packed hi parts, lo parts
+// through *lo2.  Between the two e4m3 parts the value passes through fp16: 11 bits, finer than both.
+template <bool X16>
 __device__ __forceinline__ uint32_t split_e4m3x2(float a, float b, uint32_t* lo2) {
-  const uint32_t h = e4m3x2(a, b);
-  const float2 v = e4m3x2_value(h);
-  *lo2 = e4m3x2((a - v.x) * 16.f, (b - v.y) * 16.f);
+  const __half2 v = __floats2half2_rn(a, b);
+  const uint32_t h = e4m3x2(v);
+  __half2 r = __hsub2(v, e4m3x2_value(h));
+  if (X16) r = __hmul2(r, __float2half2_rn(16.f));
+  *lo2 = e4m3x2(r);
   return h;
 }
 
@@ -248,24 +288,153 @@ __device__ __forceinline__ uint32_t panel_off(int r, int c) {
   return (uint32_t)(r * SW + ((SW == 128 ? (c ^ (r & 7)) : (c ^ ((r >> 1) & 3))) << 4));
 }
 
-// Columns [c, c + W) of a TMEM row (W 16 or 32) as floats, without waiting.
-template <int W>
-__device__ __forceinline__ void tmem_cols(uint32_t addr, uint32_t (&r)[W]) {
-  if constexpr (W == 16) tmem_ld16(addr, r);
-  else tmem_ld32(addr, r);
+// Sums of C values over a warp: lane l ends with the sum of column l * C / 32 (lanes of the same
+// column hold the same).  Each step exchanges the half of the columns that the partner keeps.
+template <int C>
+__device__ __forceinline__ float warp_col_sums(float (&v)[C], int lane) {
+  int o = 16;
+#pragma unroll
+  for (int h = C / 2; h >= 1; h /= 2, o /= 2) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int k = 0; k < h; ++k) {
+      const float give = up ? v[k] : v[k + h], keep = up ? v[k + h] : v[k];
+      v[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  float r = v[0];
+#pragma unroll
+  for (; o; o /= 2) r += __shfl_xor_sync(0xffffffffu, r, o);
+  return r;
 }
-template <int W>
-__device__ __forceinline__ void tmem_put(uint32_t addr, const uint32_t (&r)[W]) {
-  if constexpr (W == 16) tmem_st16(addr, r);
-  else tmem_st32(addr, r);
+
+// Rows from n0 on of a Q operand: zeros that see nothing.
+template <int D, int ES, int R, int NT>
+__device__ __forceinline__ void zero_rows(unsigned char* q, RowConst<R>& rc, int n0, int t) {
+  using S = Shape<D, ES, R>;
+  constexpr int CH = S::SW / 16;  // 16-byte chunks of a row in a panel
+#pragma unroll 1
+  for (int k = t; k < (R - n0) * (S::ROWB / 16) * (ES == 1 ? 2 : 1); k += NT) {
+    const int part = k / ((R - n0) * (S::ROWB / 16)), in = k % ((R - n0) * (S::ROWB / 16));
+    const int n = n0 + in / (S::ROWB / 16), c = in % (S::ROWB / 16);
+    *reinterpret_cast<uint4*>(q + part * (S::SIDE ? R * S::SW : S::QPART) + (c / CH) * S::QPANEL + n * S::SW + (c % CH) * 16) =
+        make_uint4(0u, 0u, 0u, 0u);
+  }
+  for (int n = n0 + t; n < R; n += NT) {
+    rc.xs[n] = rc.slope[n] = 0.f;
+    rc.lo[n] = 1;
+    rc.hi[n] = rc.qpos[n] = 0;
+    rc.orow[n] = -1;
+  }
+}
+
+// The Q operand and the row constants of a unit's row group and K/V head, by NT threads.
+template <int D, int ES, int R, int NT>
+__device__ __forceinline__ void build_q(const PagedArgs& a, const Entry& e, int hk, unsigned char* q, RowConst<R>& rc,
+                                        int t) {
+  using S = Shape<D, ES, R>;
+  constexpr int SW = S::SW;
+  constexpr int TPR = D / 8;      // threads per row, 8 elements each
+  constexpr int ROWS = NT / TPR;  // rows at once
+  constexpr int PASSES = (R + ROWS - 1) / ROWS;
+  constexpr int UN = PASSES < 2 ? 1 : 2;  // rows in flight per thread (unrolling more costs instruction fetches)
+  const int d0 = (t % TPR) * 8;
+  const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0;
+  const float dom = capped ? 1.f : kLog2e;
+#pragma unroll 1
+  for (int p0 = 0; p0 < PASSES; p0 += UN) {
+    if (p0 > 0 && e.rg * R + p0 * ROWS >= a.M) {  // rows that do not exist: an operand of zeros
+      zero_rows<D, ES, R, NT>(q, rc, p0 * ROWS, t);
+      break;
+    }
+    uint4 raws[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int n = (p0 + u) * ROWS + t / TPR, m = e.rg * R + n, i = m / a.G;
+      raws[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (n < R && m < a.M && i < e.ql) {
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.ptr) + (int64_t)e.b * a.q.stride_b +
+                             (int64_t)(hk * a.G + (m - i * a.G)) * a.q.stride_h + (int64_t)i * a.q.stride_t + d0;
+        if (a.q_vec) {
+          raws[u] = __ldg(reinterpret_cast<const uint4*>(qp));
+        } else {
+          raws[u].x = (uint32_t)qp[0] | ((uint32_t)qp[1] << 16);
+          raws[u].y = (uint32_t)qp[2] | ((uint32_t)qp[3] << 16);
+          raws[u].z = (uint32_t)qp[4] | ((uint32_t)qp[5] << 16);
+          raws[u].w = (uint32_t)qp[6] | ((uint32_t)qp[7] << 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int n = (p0 + u) * ROWS + t / TPR, m = e.rg * R + n, i = m / a.G, h = hk * a.G + (m - i * a.G);
+      const uint4 raw = raws[u];
+      float fix = 1.f;  // undoes the row's power of two
+      if constexpr (ES == 2) {
+        if (n < R) *reinterpret_cast<uint4*>(q + (d0 * 2 / SW) * S::QPANEL + panel_off<SW>(n, (d0 * 2 % SW) >> 4)) = raw;
+      } else {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        float f[8], top = 0.f;
+        bool odd = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f[2 * k] = __uint_as_float(w[k] << 16);
+          f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          top = fmaxf(top, fabsf(f[k]));
+          odd = odd | !(fabsf(f[k]) < INFINITY);
+        }
+        if (odd) top = INFINITY;
+#pragma unroll
+        for (int o = TPR / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // 2^sh brings the largest magnitude into [128, 256) (at most 2^100: tinier rows stay small)
+        const int ex = (int)(__float_as_uint(top) >> 23) - 127;
+        const int sh = top > 0.f && top < INFINITY ? min(7 - ex, 100) : 0;
+        const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
+        fix = __uint_as_float((uint32_t)(127 - sh) << 23);
+        if (top == INFINITY) fix = __uint_as_float(0x7fc00000u);  // NaN or infinity in q: the row is NaN
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) hi[k] = split_e4m3x2<S::SIDE>(f[2 * k] * up, f[2 * k + 1] * up, &lo[k]);
+        if (n < R) {
+          unsigned char* at = q + (d0 / SW) * S::QPANEL + (d0 & 8);
+          const int c = (d0 % SW) >> 4;
+          *reinterpret_cast<uint2*>(at + panel_off<SW>(n, c)) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
+          *reinterpret_cast<uint2*>(at + (S::SIDE ? panel_off<SW>(R + n, c) : S::QPART + panel_off<SW>(n, c))) =
+              make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+        }
+      }
+      if (d0 == 0 && n < R) {
+        const bool real = m < a.M, live = real && i < e.ql;
+        const int qpos = e.len - e.ql + i;
+        int lo = 0, hi = e.len - 1;
+        if (a.mask.flags & FA_MASK_CAUSAL) hi = min(hi, qpos);
+        if (a.mask.flags & FA_MASK_WINDOW) {
+          if (a.mask.window_left >= 0) lo = max(lo, qpos - a.mask.window_left);
+          if (a.mask.window_right >= 0) hi = (int)min((int64_t)hi, (int64_t)qpos + a.mask.window_right);
+        }
+        rc.xs[n] = a.scale * fix * dom;
+        rc.slope[n] = live && (a.score.flags & FA_SCORE_ALIBI) ? __ldg(a.score.alibi_slopes + h) * dom : 0.f;
+        rc.lo[n] = live ? lo : 1;
+        rc.hi[n] = live ? hi : 0;
+        rc.qpos[n] = qpos;
+        rc.orow[n] = real ? (int64_t)e.b * a.o.stride_b + (int64_t)h * a.o.stride_h + (int64_t)i * a.o.stride_t : -1;
+        rc.lrow[n] = ((int64_t)e.b * a.H + h) * a.Tq + i;
+      }
+    }
+  }
 }
 
 template <int D, int ES, int R>
-__global__ void __launch_bounds__(kPThreads, 1)
+__global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                       const PagedArgs a) {
   using S = Shape<D, ES, R>;
-  constexpr int N = S::N, SW = S::SW;
+  constexpr int N = S::N, SW = S::SW, C = S::C, NG = S::NG, NSM = S::NSM, NT = S::NT;
+  constexpr int W_LOAD = 4 * NG, W_S = W_LOAD + 1, W_PV = W_LOAD + 2, W_Q = W_LOAD + 3;  // warps behind the softmax
+  constexpr bool TURNS = S::TURNS;
   constexpr uint32_t LAYOUT = SW == 128 ? SMEM_SWIZZLE_128B : SMEM_SWIZZLE_64B;
   constexpr int KPOS = 32 / ES;  // positions per PV MMA
   constexpr uint32_t IDESC_S = ES == 1 ? make_idesc_e4m3(128, N, 0, 0) : make_idesc_bf16(128, N, 0, 0);
@@ -285,32 +454,32 @@ __global__ void __launch_bounds__(kPThreads, 1)
   griddep_launch();
 
   // ---------------------------------------------------------------- setup: barriers, TMEM, range
-  if (tid == 0) {
+  if (tid == NT - 1) {  // (the first warps have entries to count)
     for (int i = 0; i < NS; ++i) {
       mbar_init(sm.full + i, 1);
       mbar_init(sm.empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(sm.s_full + i, 1);
-      mbar_init(sm.p_full + i, 4);
+      mbar_init(sm.p_full + i, TURNS ? 4 : 4 * NG);
       mbar_init(sm.o_full + i, 1);
-      mbar_init(sm.q_full + i, 2);
-      mbar_init(sm.q_empty + i, 5);  // the MMA issuer's commit and four softmax warps
+      mbar_init(sm.q_full + i, 1);
+      mbar_init(sm.q_empty + i, 1 + 4 * NG);  // the S issuer's commit and the softmax warps
+      mbar_init(sm.fin_bar + i, 1);
     }
-    mbar_init(&sm.fin_bar, 1);
     sm.abort_flag = 0;
     sm.never = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
-  if (warp == 5) {
+  if (warp == W_S) {
     tmem_alloc(&sm.tmem, S::TM_COLS);
     tmem_relinquish();
   }
   {
     // Exclusive prefix of the entries' tiles over the threads, each with a run of entries.
-    const int run = (a.entries + kPThreads - 1) / kPThreads, e0 = min(tid * run, a.entries),
+    const int run = (a.entries + NT - 1) / NT, e0 = min(tid * run, a.entries),
               e1 = min(e0 + run, a.entries);
     int mine = 0;
     bool bad = false;
@@ -333,7 +502,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     __syncthreads();
     int before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < NT / 32; ++w) {
       if (w < warp) before += sm.scan[w];
       total += sm.scan[w];
     }
@@ -366,96 +535,139 @@ __global__ void __launch_bounds__(kPThreads, 1)
   wk.begin(a, sm.first_entry, sm.first_off, my_tiles);
   Seg sg;
 
-  if (warp == 4) {
+  if (warp == W_LOAD) {
     // ---------------------------------------------------------------- producer
-    // Lane l serves page l of a tile.  Page numbers are fetched two tiles ahead and scales one, so
-    // neither latency holds up the ring.
-    const int ppt = kTile / a.ps;
-    struct Ahead {
-      int page, col, hk, tile, active, lo, hi;
+    // A batch of 32 pages (32 / pages-per-tile tiles): each lane holds the number and the scales of one
+    // page, and fetches the next batch's while this one's loads go out.
+    const int ppt = kTile / a.ps, batch = 32 / ppt, sub = lane / ppt, pg = lane - sub * ppt;
+    struct Page {
+      int page, hk, active;
       float ks, vs;
     };
-    Ahead x0, x1, x2;  // the tile to issue, the next, the one after
-    int left_in_seg = 0, tile = 0;
-    auto fetch = [&](Ahead& x) {  // page number of the next tile of the walk
-      x.tile = -1;
-      if (left_in_seg == 0) {
-        if (!wk.next(a, &sg)) return;
-        left_in_seg = sg.nt;
-        tile = sg.t0;
+    int at = sub;  // this lane's tile in the CTA's range
+    auto fetch = [&](Page& x) {
+      x.active = 0;
+      x.page = 0;
+      x.hk = 0;
+      if (at < my_tiles) {
+        wk.settle(a);
+        const int pos = (wk.e.t0 + wk.off) * kTile + pg * a.ps;
+        x.hk = wk.hk;
+        x.active = pos <= wk.e.hi && pos + a.ps > wk.e.lo;
+        if (x.active) x.page = __ldg(a.table + (int64_t)wk.e.b * a.table_stride + pos / a.ps);
       }
-      x.tile = tile++;
-      --left_in_seg;
-      x.hk = sg.hk;
-      const int pos = x.tile * kTile + lane * a.ps;
-      x.active = lane < ppt && pos <= wk.e.hi && pos + a.ps > wk.e.lo;
-      x.page = x.active ? __ldg(a.table + (int64_t)wk.e.b * a.table_stride + pos / a.ps) : 0;
+      at += batch;
+      wk.off += batch;
     };
-    auto fetch_scales = [&](Ahead& x) {
-      const bool good = x.tile >= 0 && x.active && (unsigned)x.page < (unsigned)a.num_pages;
+    auto fetch_scales = [&](Page& x) {
       x.ks = -INFINITY;
-      x.vs = 0.f;
-      if (good) {
+      x.vs = 1.f;
+      if (x.active && (unsigned)x.page < (unsigned)a.num_pages) {
         if constexpr (ES == 1) {
           x.ks = __ldg(a.k_scale + (int64_t)x.page * a.Hkv + x.hk);
           x.vs = __ldg(a.v_scale + (int64_t)x.page * a.Hkv + x.hk);
         } else {
           x.ks = 1.f;
-          x.vs = 1.f;
         }
       }
     };
-    int issued = 0;  // slots filled so far (K and V of a tile take one each)
-    fetch(x0);
-    fetch(x1);
-    fetch_scales(x0);
-    for (int j = 0; x0.tile >= 0; ++j) {
-      fetch(x2);
-      fetch_scales(x1);
-      const bool hidden = x0.active && (unsigned)x0.page >= (unsigned)a.num_pages;
-      const unsigned act = __ballot_sync(0xffffffffu, x0.active);
-      const bool any_hidden = __any_sync(0xffffffffu, hidden);
-      if (any_hidden && lane == 0) report_status(a.status, FA_ERR_INVALID);
-      const uint32_t bytes = (uint32_t)__popc(act) * a.ps * S::ROWB;
-      bool ok = true;
+    int issued = 0, slot = 0;  // slots filled so far (K and V of a tile take one each); the next one
+    uint32_t phase = 1;        // parity of the empty barriers' phase that frees it (the first is free)
+    Page x, y;
+    wk.off += sub;
+    fetch(x);
+    fetch_scales(x);
+    bool ok = true;
+    for (int j0 = 0; ok && j0 < my_tiles; j0 += batch) {
+      fetch(y);
+      const bool hidden = x.active && (unsigned)x.page >= (unsigned)a.num_pages;
+      const unsigned act = __ballot_sync(0xffffffffu, x.active), hid = __ballot_sync(0xffffffffu, hidden);
+      if (hid && lane == 0) report_status(a.status, FA_ERR_INVALID);
+      const int page = hidden ? a.num_pages : x.page;  // reads as zeros: the map's bounds check
+      const int n = min(batch, my_tiles - j0);
+      const unsigned pages = ppt == 32 ? 0xffffffffu : (1u << ppt) - 1u;
+      unsigned small = 0;
+      for (int k = 0; ok && k < n; ++k) {
+        const int ring = (j0 + k) % kScaleRing;
+        const uint32_t bytes = (uint32_t)__popc((act >> (k * ppt)) & pages) * a.ps * S::ROWB;
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int ld = 2 * j + kv, slot = ld % NS;
-        if (ld >= NS) ok = mbar_wait_w(sm.empty + slot, (uint32_t)((ld / NS - 1) & 1), abort_flag);
-        if (!ok) break;
-        if (kv == 0) {  // the K slot's release says that the tile whose scales lay here is done
-          if (lane < 8) sm.scales[j % kScaleRing][lane] = make_float2(x0.ks, x0.vs);
-          if (lane == 0) sm.odd[j % kScaleRing] = any_hidden;
+        for (int kv = 0; kv < 2; ++kv) {
+          ok = wait_for_w(sm.empty + slot, phase, abort_flag);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(sm.full + slot, bytes);
           __syncwarp();
-        }
-        if (lane == 0) mbar_arrive_expect_tx(sm.full + slot, bytes);
-        __syncwarp();
-        if (x0.active) {  // a page number out of range reads as zeros: the map's bounds check
-          unsigned char* dst = base + (size_t)slot * S::SLOT + (size_t)lane * a.ps * SW;
-          const int page = hidden ? a.num_pages : x0.page;
+          if (sub == k && x.active) {
+            unsigned char* dst = base + (size_t)slot * S::SLOT + (size_t)pg * a.ps * SW;
 #pragma unroll
-          for (int p = 0; p < S::ROWB / SW; ++p)
-            tma_load_4d(dst + p * S::PANEL, kv ? &tv : &tk, sm.full + slot, p * (SW / ES), 0, x0.hk, page);
+            for (int p = 0; p < S::ROWB / SW; ++p)
+              tma_load_4d(dst + p * S::PANEL, kv ? &tv : &tk, sm.full + slot, p * (SW / ES), 0, x.hk, page);
+          }
+          if (kv == 0) {
+            // This slot being free says that the tile whose scales lay here is done.  The scales are
+            // there before the slot's barrier can complete.
+            if (ES == 1 && k == 0) small = __ballot_sync(0xffffffffu, x.active && !(x.vs >= 0x1p-100f));
+            if (sub == k) sm.scales[ring][pg] = make_float2(x.ks, x.vs);
+            if (lane == 0) sm.odd[ring] = (((hid | small) >> (k * ppt)) & pages) != 0;
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(sm.full + slot);
+          ++issued;
+          if (++slot == NS) {
+            slot = 0;
+            phase ^= 1u;
+          }
         }
-        issued = ld + 1;
+        if (k == 0) fetch_scales(y);
       }
-      if (!ok) {
-        if (lane == 0) *abort_flag = 1;
-        break;
-      }
-      x0 = x1;
-      x1 = x2;
+      x = y;
     }
+    if (!ok && lane == 0) *abort_flag = 1;
     // every slot's latest load lands before the CTA may exit
     for (int ld = max(0, issued - NS); ld < issued; ++ld)
-      mbar_wait_w(sm.full + ld % NS, (uint32_t)((ld / NS) & 1), never);
-  } else if (warp == 5) {
-    // ---------------------------------------------------------------- MMA issue
-    // S(0), S(1), then per tile PV(j) once P(j) is written, and S(j + 2) into the buffer that
-    // the softmax of j has read.
+      wait_for_w(sm.full + ld % NS, (uint32_t)((ld / NS) & 1), never);
+  } else if (warp == W_S) {
+    // ---------------------------------------------------------------- S issue
+    // S(j) goes into buffer j & 1 once the softmax of j - 2 has read it (it has written P(j - 2)).
     const uint32_t slot_k = (uint32_t)make_smem_desc(smem_u32(base), 16, 8 * SW, LAYOUT);
     const uint32_t q_lo = (uint32_t)make_smem_desc(smem_u32(sQ), 16, 8 * SW, LAYOUT);
     const uint32_t hi_k = (uint32_t)(make_smem_desc(0, 16, 8 * SW, LAYOUT) >> 32);
+    int slot = 0, j = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int seg = 0; ok && wk.next(a, &sg); ++seg) {
+      ok = wait_for_w(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag);
+      const uint32_t qb = q_lo + (uint32_t)(((seg & 1) * S::QBUF) >> 4);
+      for (int it = 0; ok && it < sg.nt; ++it, ++j) {
+        if (j >= 2) ok = wait_for_w(sm.p_full + (j & 1), (uint32_t)(((j >> 1) - 1) & 1), abort_flag);
+        ok = ok && wait_for_w(sm.full + slot, phase, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ka = slot_k + (uint32_t)((slot * S::SLOT) >> 4);
+#pragma unroll
+        for (int pt = 0; pt < S::PARTS; ++pt)
+#pragma unroll
+          for (int kk = 0; kk < S::ROWB / 32; ++kk) {
+            const uint32_t p = kk * 32 / SW, in = (kk * 32 % SW) >> 4;
+            const uint32_t ad = ka + p * (S::PANEL >> 4) + in,
+                           bd = qb + pt * (S::QPART >> 4) + p * (S::QPANEL >> 4) + in;
+            if constexpr (ES == 1) mma_f8_ss_w(tmem + (j & 1) * N, ad, hi_k, bd, hi_k, IDESC_S, pt + kk > 0);
+            else mma_ss_w(tmem + (j & 1) * N, ad, hi_k, bd, hi_k, IDESC_S, kk > 0);
+          }
+        tc_commit_w(sm.s_full + (j & 1));
+        tc_commit_w(sm.empty + slot);
+        slot += 2;
+        if (slot >= NS) {
+          slot -= NS;
+          phase ^= 1u;
+        }
+      }
+      tc_commit_w(sm.q_empty + (seg & 1));
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+    tc_commit_w(sm.fin_bar);
+    wait_for_w(sm.fin_bar, 0, never);  // every MMA has retired before TMEM is freed
+  } else if (warp == W_PV) {
+    // ---------------------------------------------------------------- P V issue
     // V as the M-major operand: panels of SW bytes of D are LBO apart (a head dim of 64 has one
     // panel, read twice: rows 64-127 of O repeat rows 0-63 and are not used)
     constexpr uint32_t V_LBO = D * ES > SW && ES == 2 ? S::PANEL : 0;
@@ -465,345 +677,241 @@ __global__ void __launch_bounds__(kPThreads, 1)
     // next 16 bytes of N 2048
     const uint32_t p_lo = (uint32_t)make_smem_desc(smem_u32(sP), 128, 2048, SMEM_SWIZZLE_NONE);
     const uint32_t hi_p = (uint32_t)(make_smem_desc(0, 128, 2048, SMEM_SWIZZLE_NONE) >> 32);
-    int seg = -1, left_in_seg = 0;
-    unsigned starts = 0;  // bit k: the tile k before the one whose S was issued last begins a unit's part
+    int slot = 1 % NS, j = 0;
+    uint32_t phase = 0;
     bool ok = true;
-    auto issue_s = [&](int j) -> bool {
-      starts <<= 1;
-      if (left_in_seg == 0) {
-        wk.next(a, &sg);
-        left_in_seg = sg.nt;
-        ++seg;
-        starts |= 1u;
-        if (!mbar_wait_w(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag)) return false;
-      }
-      const int ld = 2 * j, slot = ld % NS;
-      if (!mbar_wait_w(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) return false;
-      tc_fence_after();
-      const uint32_t ka = slot_k + (uint32_t)((slot * S::SLOT) >> 4), qb = q_lo + (uint32_t)(((seg & 1) * S::QBUF) >> 4);
+    while (ok && wk.next(a, &sg)) {
+      for (int it = 0; ok && it < sg.nt; ++it, ++j) {
+        ok = wait_for_w(sm.full + slot, phase, abort_flag) &&
+             wait_for_w(sm.p_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc0 = it >= (TURNS ? 2 : 1) ? 1u : 0u;  // the first tile that this O takes overwrites it
+        const uint32_t o = tmem + S::TM_O + (TURNS ? (j & 1) * S::ON : 0);
+        const uint32_t pb = p_lo + (uint32_t)(((j & 1) * S::PBUF) >> 4);
 #pragma unroll
-      for (int kk = 0; kk < S::ROWB / 32; ++kk) {
-        const uint32_t p = kk * 32 / SW, in = (kk * 32 % SW) >> 4;
-        if constexpr (ES == 1)
-          mma_f8_ss_w(tmem + (j & 1) * N, ka + p * (S::PANEL >> 4) + in, hi_k, qb + p * (S::QPANEL >> 4) + in, hi_k,
-                      IDESC_S, kk > 0);
-        else
-          mma_ss_w(tmem + (j & 1) * N, ka + p * (S::PANEL >> 4) + in, hi_k, qb + p * (S::QPANEL >> 4) + in, hi_k,
-                   IDESC_S, kk > 0);
-      }
-      tc_commit_w(sm.s_full + (j & 1));
-      tc_commit_w(sm.empty + slot);
-      if (--left_in_seg == 0) tc_commit_w(sm.q_empty + (seg & 1));
-      return true;
-    };
-    for (int j = 0; j < 2 && ok; ++j) {
-      if (j < my_tiles) ok = issue_s(j);
-      else starts <<= 1;
-    }
-    for (int j = 0; j < my_tiles && ok; ++j) {
-      const int ld = 2 * j + 1, slot = ld % NS;
-      ok = mbar_wait_w(sm.p_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag) &&
-           mbar_wait_w(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      const bool fresh = (starts >> 1) & 1u;  // S has been issued one tile beyond j
-      const uint32_t pb = p_lo + (uint32_t)(((j & 1) * S::PBUF) >> 4);
+        for (int db = 0; db < S::NO; ++db) {
+          const uint32_t va = slot_v + (uint32_t)((slot * S::SLOT + db * (128 * ES / SW) * S::PANEL) >> 4);
 #pragma unroll
-      for (int db = 0; db < S::NO; ++db) {
-        const uint32_t va = slot_v + (uint32_t)((slot * S::SLOT + db * (128 * ES / SW) * S::PANEL) >> 4);
+          for (int pt = 0; pt < S::PARTS; ++pt)
 #pragma unroll
-        for (int kk = 0; kk < kTile / KPOS; ++kk) {
-          const uint32_t acc = (fresh && kk == 0) ? 0u : 1u;
-          if constexpr (ES == 1)
-            mma_f8_ss_w(tmem + S::TM_O + db * N, va + kk * ((KPOS * SW) >> 4), hi_v, pb + kk * ((KPOS * 16) >> 4),
-                        hi_p, IDESC_PV, acc);
-          else
-            mma_ss_w(tmem + S::TM_O + db * N, va + kk * ((KPOS * SW) >> 4), hi_v, pb + kk * ((KPOS * 16) >> 4), hi_p,
-                     IDESC_PV, acc);
+            for (int kk = 0; kk < kTile / KPOS; ++kk) {
+              const uint32_t ad = va + kk * ((KPOS * SW) >> 4),
+                             bd = pb + pt * (S::PPART >> 4) + kk * ((KPOS * 16) >> 4);
+              if constexpr (ES == 1) mma_f8_ss_w(o + db * N, ad, hi_v, bd, hi_p, IDESC_PV, pt + kk > 0 ? 1u : acc0);
+              else mma_ss_w(o + db * N, ad, hi_v, bd, hi_p, IDESC_PV, kk > 0 ? 1u : acc0);
+            }
+        }
+        tc_commit_w(sm.o_full + (j & 1));
+        tc_commit_w(sm.empty + slot);
+        slot += 2;
+        if (slot >= NS) {
+          slot -= NS;
+          phase ^= 1u;
         }
       }
-      tc_commit_w(sm.empty + slot);
-      tc_commit_w(sm.o_full + (j & 1));
-      if (j + 2 < my_tiles) ok = issue_s(j + 2);
-      else starts <<= 1;
     }
     if (!ok && lane == 0) *abort_flag = 1;
-    tc_commit_w(&sm.fin_bar);
-    mbar_wait_w(&sm.fin_bar, 0, never);  // every MMA has retired before TMEM is freed
-  } else if (warp >= 6) {
+    tc_commit_w(sm.fin_bar + 1);
+    wait_for_w(sm.fin_bar + 1, 0, never);
+  } else if (warp == W_Q) {
     // ---------------------------------------------------------------- Q operand and row constants
-    constexpr int TPR = D / 8;          // threads per row, 8 elements each
-    constexpr int ROWS = 64 / TPR;      // rows at once
-    static_assert(R % ROWS == 0, "whole passes: the shuffles below need full warps");
-    const int t = tid - 192, d0 = (t % TPR) * 8;
+    // The softmax warps build the first unit's (they have nothing else to do yet).
     bool ok = true;
     for (int seg = 0; ok && wk.next(a, &sg); ++seg) {
       const int buf = seg & 1;
-      if (seg >= 2) ok = mbar_wait_w(sm.q_empty + buf, (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
-      if (!ok) break;
-      RowConst<R>& rc = sm.rc[buf];
-      const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0;
-      const float dom = capped ? 1.f : kLog2e;
-#pragma unroll 2
-      for (int n0 = 0; n0 < R; n0 += ROWS) {
-        const int n = n0 + t / TPR;
-        const int m = wk.e.rg * R + n, i = m / a.G, h = sg.hk * a.G + (m - i * a.G);
-        const bool real = m < a.M, live = real && i < wk.e.ql;
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (live) {
-          const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.ptr) + (int64_t)wk.e.b * a.q.stride_b +
-                               (int64_t)h * a.q.stride_h + (int64_t)i * a.q.stride_t + d0;
-          if (a.q_vec) {
-            raw = __ldg(reinterpret_cast<const uint4*>(qp));
-          } else {
-            raw.x = (uint32_t)qp[0] | ((uint32_t)qp[1] << 16);
-            raw.y = (uint32_t)qp[2] | ((uint32_t)qp[3] << 16);
-            raw.z = (uint32_t)qp[4] | ((uint32_t)qp[5] << 16);
-            raw.w = (uint32_t)qp[6] | ((uint32_t)qp[7] << 16);
-          }
-        }
-        float fix = 1.f;  // undoes the row's power of two
-        unsigned char* q = sQ + buf * S::QBUF;
-        if constexpr (ES == 2) {
-          *reinterpret_cast<uint4*>(q + (d0 * 2 / SW) * S::QPANEL + panel_off<SW>(n, (d0 * 2 % SW) >> 4)) = raw;
-        } else {
-          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-          float f[8], top = 0.f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            f[2 * k] = __uint_as_float(w[k] << 16);
-            f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-          }
-          bool odd = false;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            top = fmaxf(top, fabsf(f[k]));
-            odd = odd || !(fabsf(f[k]) < INFINITY);
-          }
-          if (odd) top = INFINITY;
-#pragma unroll
-          for (int o = TPR / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          // 2^sh brings the largest magnitude into [128, 256) (at most 2^100: tinier rows stay small)
-          const int ex = (int)(__float_as_uint(top) >> 23) - 127;
-          const int sh = top > 0.f && top < INFINITY ? min(7 - ex, 100) : 0;
-          const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
-          fix = __uint_as_float((uint32_t)(127 - sh) << 23);
-          if (top == INFINITY) fix = __uint_as_float(0x7fc00000u);  // NaN or infinity in q: the row is NaN
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) hi[k] = split_e4m3x2(f[2 * k] * up, f[2 * k + 1] * up, &lo[k]);
-          unsigned char* at = q + (d0 / SW) * S::QPANEL + (d0 & 8);
-          const int c = (d0 % SW) >> 4;
-          *reinterpret_cast<uint2*>(at + panel_off<SW>(n, c)) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
-          *reinterpret_cast<uint2*>(at + panel_off<SW>(R + n, c)) =
-              make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
-        }
-        if (d0 == 0) {
-          const int qpos = wk.e.len - wk.e.ql + i;
-          int lo = 0, hi = wk.e.len - 1;
-          if (a.mask.flags & FA_MASK_CAUSAL) hi = min(hi, qpos);
-          if (a.mask.flags & FA_MASK_WINDOW) {
-            if (a.mask.window_left >= 0) lo = max(lo, qpos - a.mask.window_left);
-            if (a.mask.window_right >= 0) hi = (int)min((int64_t)hi, (int64_t)qpos + a.mask.window_right);
-          }
-          rc.xs[n] = a.scale * fix * dom;
-          rc.slope[n] = live && (a.score.flags & FA_SCORE_ALIBI) ? __ldg(a.score.alibi_slopes + h) * dom : 0.f;
-          rc.lo[n] = live ? lo : 1;
-          rc.hi[n] = live ? hi : 0;
-          rc.qpos[n] = qpos;
-          rc.orow[n] = real ? (int64_t)wk.e.b * a.o.stride_b + (int64_t)h * a.o.stride_h + (int64_t)i * a.o.stride_t : -1;
-          rc.lrow[n] = ((int64_t)wk.e.b * a.H + h) * a.Tq + i;
-        }
+      if (seg == 0) {
+        named_bar_sync(6, NSM + 32);
+      } else {
+        if (seg >= 2) ok = wait_for_w(sm.q_empty + buf, (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
+        if (!ok) break;
+        build_q<D, ES, R, 32>(a, wk.e, sg.hk, sQ + buf * S::QBUF, sm.rc[buf], lane);
+        fence_proxy_async_smem();
       }
-      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.q_full + buf);
     }
     // Entries without a tile: their rows see nothing.
-    const int t64 = tid - 192;
     for (int e = cta; e < a.entries; e += gridDim.x) {
       const Entry x = entry_of<R>(a, e);
       if (x.nt) continue;
       const int m0 = x.rg * R, rows = min(R, a.M - m0);
-      for (int k = t64; k < a.Hkv * rows * D; k += 64) {
-        const int d = k % D, r = k / D, hk = r / rows, m = m0 + r % rows, i = m / a.G, h = hk * a.G + m % a.G;
-        reinterpret_cast<uint16_t*>(a.o.ptr)[(int64_t)x.b * a.o.stride_b + (int64_t)h * a.o.stride_h +
-                                             (int64_t)i * a.o.stride_t + d] = 0;
-        if (d == 0) a.lse[((int64_t)x.b * a.H + h) * a.Tq + i] = -INFINITY;
+      for (int r = 0; r < a.Hkv * rows; ++r) {
+        const int hk = r / rows, m = m0 + r % rows, i = m / a.G, h = hk * a.G + m % a.G;
+        uint16_t* o = reinterpret_cast<uint16_t*>(a.o.ptr) + (int64_t)x.b * a.o.stride_b + (int64_t)h * a.o.stride_h +
+                      (int64_t)i * a.o.stride_t;
+#pragma unroll
+        for (int d = 0; d < D; d += 32) o[d + lane] = 0;
+        if (lane == 0) a.lse[((int64_t)x.b * a.H + h) * a.Tq + i] = -INFINITY;
       }
     }
   } else {
     // ---------------------------------------------------------------- softmax (thread = position)
-    RowState<R>& rs = sm.rs;
-    const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    const int grp = warp >> 2, t = tid & 127, bar = 1 + grp;
+    RowState& rs = sm.rs[grp];
+    const int c0 = TURNS ? 0 : grp * C;  // this thread's rows are [c0, c0 + C)
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_o = t_lane + S::TM_O + (TURNS ? grp * S::ON : c0);
     const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0, alibi = (a.score.flags & FA_SCORE_ALIBI) != 0;
     const float cap2 = capped ? a.score.softcap * kLog2e : 0.f, cap_k = capped ? 2.f * kLog2e / a.score.softcap : 0.f;
-    constexpr int RC = R < 32 ? R : 32;        // rows per TMEM read (x2 parts for 8-bit codes)
-    constexpr int PW = 16 / ES;                // columns per 16-byte store of P
+    const int my_page = t / a.ps;
+    constexpr int PW = 16 / ES;  // rows per 16-byte store of P
+    constexpr int CH = 4;        // rows worked on together; the ones behind the last real row are left out
     int unit0 = -1, unit1 = -1, j = 0;
     for (int seg = 0; wk.next(a, &sg); ++seg) {
       const RowConst<R>& rc = sm.rc[seg & 1];
-      if (tid < R) {
-        rs.mx[tid] = rs.my[tid] = rs.thx[tid] = rs.thy[tid] = -INFINITY;
-        rs.mref[tid] = 0.f;
-        rs.w[tid] = 1.f;
+      if (seg == 0) {
+        build_q<D, ES, R, NSM>(a, wk.e, sg.hk, sQ, sm.rc[0], tid);
+        fence_proxy_async_smem();
+        named_bar_sync(6, NSM + 32);
       }
-      if (!mbar_wait(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag)) *abort_flag = 1;
-      named_bar_sync(1, 128);
-      float l[R];
+      const int rr = min(a.M - wk.e.rg * R - c0, C);  // this thread's real rows
+      if (t < C) {
+        rs.m[t] = kUnset;
+        rs.bias[t] = kLift - kUnset;
+      }
+      // No wait leaves the loops: after a time-out every later wait returns at once and nothing is
+      // written at the end.
+      if (!wait_for(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag)) *abort_flag = 1;
+      named_bar_sync(bar, 128);
+      float l[C];
 #pragma unroll
-      for (int n = 0; n < R; ++n) l[n] = 0.f;
+      for (int n = 0; n < C; ++n) l[n] = 0.f;
+      bool filled = false;  // this group's O holds something of this unit
+      const int j0 = j;     // the unit's first tile
       for (int it = 0; it < sg.nt; ++it, ++j) {
-        const int pos = (sg.t0 + it) * kTile + tid;
-        // No wait leaves the loop: after a time-out every later wait returns at once and nothing
-        // is written at the end.
-        if (!mbar_wait(sm.s_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag)) *abort_flag = 1;
+        if (TURNS && (j & 1) != grp) continue;
+        const int p0 = (sg.t0 + it) * kTile, pos = p0 + t;
+        if (!wait_for(sm.s_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag)) *abort_flag = 1;
         tc_fence_after();
-        const float2 sc = sm.scales[j % kScaleRing][tid / a.ps];
+        uint32_t r[16];
+        tmem_ld16(t_lane + (j & 1) * N + c0, r);
+        const float2 sc = sm.scales[j % kScaleRing][my_page];
+        const int odd = sm.odd[j % kScaleRing];
         const bool shown = sc.x != -INFINITY;
-        const float ks = shown ? sc.x : 0.f, vs = sc.y;
-        const int p0 = (sg.t0 + it) * kTile;
-        const bool inside = p0 >= wk.e.in_lo && p0 + kTile - 1 <= wk.e.in_hi && !sm.odd[j % kScaleRing];
-        // a scale below 2^-100 (none that an append makes) counts as 2^-100 here: w stays finite
-        const float lv = ES == 1 ? fmaxf(lg2_approx(vs), -100.f) : 0.f;
-        float x[R];
-        bool over = false;
+        const float ks = ES == 1 ? (shown ? sc.x : 0.f) : 1.f;
+        // a value scale below 2^-100 counts as zero: its codes are cleared below
+        const float lv = ES == 1 ? fmaxf(lg2_approx(sc.y), -100.f) : 0.f;
+        const float inv_vs = ES == 1 ? ex2_approx(-lv) : 1.f;
+        const bool inside = p0 >= wk.e.in_lo && p0 + kTile - 1 <= wk.e.in_hi && !odd;
+        tmem_ld_wait();
+        reg_pin(r);
+        float z[C], top = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < R; c += RC) {
-          if constexpr (ES == 1) {
-            constexpr int W = R == 8 ? 16 : RC;  // R = 8: hi and lo parts in one read
-            uint32_t h[W], lo[W];
-            tmem_cols<W>(t_lane + (j & 1) * N + c, h);
-            if constexpr (R > 8) tmem_cols<W>(t_lane + (j & 1) * N + R + c, lo);
-            tmem_ld_wait();
-            reg_pin(h);
-            if constexpr (R > 8) reg_pin(lo);
+        for (int c = 0; c < C; c += CH) {
+          if (c >= rr) {
 #pragma unroll
-            for (int n = 0; n < RC; ++n)
-              x[c + n] = fmaf(__uint_as_float(R == 8 ? h[(8 + n) % W] : lo[n]), 0.0625f, __uint_as_float(h[n]));
-          } else {
-            uint32_t h[RC];
-            tmem_cols<RC>(t_lane + (j & 1) * N + c, h);
-            tmem_ld_wait();
-            reg_pin(h);
-#pragma unroll
-            for (int n = 0; n < RC; ++n) x[c + n] = __uint_as_float(h[n]);
+            for (int n = c; n < c + CH; ++n) z[n] = -INFINITY;
+            continue;
           }
-        }
+          const float4 k4 = *reinterpret_cast<const float4*>(rc.xs + c0 + c);
+          const float xs[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
-        for (int n = 0; n < R; ++n) x[n] *= ES == 1 ? ks * rc.xs[n] : rc.xs[n];
-        if (alibi) {
+          for (int u = 0; u < CH; ++u) {
+            float x = __uint_as_float(r[c + u]);
+            if constexpr (S::SIDE) x = fmaf(__uint_as_float(r[8 + c + u]), 0.0625f, x);
+            const float k = ES == 1 ? ks * xs[u] : xs[u];
+            z[c + u] = (alibi | capped) ? x * k : fmaf(x, k, lv);
+          }
+          if (alibi | capped) {
 #pragma unroll
-          for (int n = 0; n < R; ++n) x[n] = fmaf(rc.slope[n], (float)(pos - rc.qpos[n]), x[n]);
-        }
-        if (capped) {  // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))), in log2 units
-#pragma unroll
-          for (int n = 0; n < R; ++n) x[n] = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + ex2_approx(x[n] * cap_k)), cap2);
-        }
-        if (!inside) {
-#pragma unroll
-          for (int n = 0; n < R; ++n)
-            if (!shown || pos < rc.lo[n] || pos > rc.hi[n]) x[n] = -INFINITY;
-        }
-#pragma unroll
-        for (int n = 0; n < R; ++n) over = over || x[n] > (ES == 1 ? fminf(rs.thx[n], rs.thy[n] - lv) : rs.thx[n]);
-        if (vote_or(1, 128, over)) {
-          // ---- a reference has to move: the tile's largest x (and x + lv) per row
-#pragma unroll
-          for (int n = 0; n < R; ++n) {
-            const float mx = warp_max(x[n]), my = ES == 1 ? warp_max(x[n] + lv) : 0.f;
-            if (lane == (n & 31)) {
-              rs.red[warp][0][n] = mx;
-              if (ES == 1) rs.red[warp][1][n] = my;
+            for (int u = 0; u < CH; ++u) {
+              float x = z[c + u];
+              if (alibi) x = fmaf(rc.slope[c0 + c + u], (float)(pos - rc.qpos[c0 + c + u]), x);
+              // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))), in log2 units
+              if (capped) x = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + ex2_approx(x * cap_k)), cap2);
+              z[c + u] = x + lv;
             }
           }
-          named_bar_sync(1, 128);
-          if (tid < R) {
-            const int n = tid;
-            const float ox = rs.mx[n], oy = rs.my[n];
-            const float nx = fmaxf(fmaxf(rs.red[0][0][n], rs.red[1][0][n]), fmaxf(rs.red[2][0][n], rs.red[3][0][n]));
-            const float mx = nx > ox + kSlack ? nx : ox;
-            float my = mx;
-            if constexpr (ES == 1) {
-              const float ny = fmaxf(fmaxf(rs.red[0][1][n], rs.red[1][1][n]), fmaxf(rs.red[2][1][n], rs.red[3][1][n]));
-              my = ny > oy + kSlack ? ny : oy;
-            }
-            rs.al[n] = mx != ox ? ex2_approx(ox - mx) : 1.f;
-            rs.ao[n] = my != oy ? ex2_approx(oy - my) : 1.f;
-            const float mref = mx == -INFINITY ? 0.f : mx;
-            rs.mx[n] = mx;
-            rs.my[n] = my;
-            rs.mref[n] = mref;
-            rs.thx[n] = mx + kSlack;
-            rs.thy[n] = my + kSlack;
-            rs.w[n] = ES == 1 && my != -INFINITY ? ex2_approx(mref - my + kLift) : 1.f;
-          }
-          named_bar_sync(1, 128);
+          if (!inside) {
 #pragma unroll
-          for (int n = 0; n < R; ++n) l[n] *= rs.al[n];
-          if (it > 0) {  // O holds earlier tiles' sums: PV(j - 1) must have retired
-            if (!mbar_wait(sm.o_full + ((j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag)) *abort_flag = 1;
+            for (int u = 0; u < CH; ++u)
+              if (!shown | (pos < rc.lo[c0 + c + u]) | (pos > rc.hi[c0 + c + u])) z[c + u] = -INFINITY;
+          }
+          const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
+          top = fmax3f(top, fmax3f(z[c] + b4.x, z[c + 1] + b4.y, z[c + 2] + b4.z), z[c + 3] + b4.w);
+        }
+        if (vote_or(bar, 128, top > kLift + kSlack)) {
+          // ---- a reference has to move to the tile's largest z of its row
+#pragma unroll
+          for (int n = 0; n < C; ++n) {
+            const float m = warp_max(z[n]);
+            if (lane == n) rs.red[warp & 3][n] = m;
+          }
+          named_bar_sync(bar, 128);
+          if (t < C) {
+            const float old = rs.m[t];
+            const float nm = fmaxf(fmaxf(rs.red[0][t], rs.red[1][t]), fmaxf(rs.red[2][t], rs.red[3][t]));
+            const float m = nm > old + kSlack ? nm : old;
+            rs.move[t] = m != old ? ex2_approx(old - m) : 1.f;
+            rs.m[t] = m;
+            rs.bias[t] = kLift - m;
+          }
+          named_bar_sync(bar, 128);
+#pragma unroll
+          for (int n = 0; n < C; ++n) l[n] *= rs.move[n];
+          if (filled) {  // this O's last P V must have retired
+            const int jo = j - (TURNS ? 2 : 1);
+            if (!wait_for(sm.o_full + (jo & 1), (uint32_t)((jo >> 1) & 1), abort_flag)) *abort_flag = 1;
             tc_fence_after();
-            constexpr int W = N < 32 ? N : 32;
 #pragma unroll 1
-            for (int c = 0; c < S::NO * N; c += W) {
-              uint32_t o[W];
-              tmem_cols<W>(t_lane + S::TM_O + c, o);
+            for (int db = 0; db < S::NO; ++db) {
+              uint32_t o[16];
+              tmem_ld16(t_o + db * N, o);
               tmem_ld_wait();
               reg_pin(o);
 #pragma unroll
-              for (int k = 0; k < W; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * rs.ao[(c + k) % R]);
-              tmem_put<W>(t_lane + S::TM_O + c, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * rs.move[k % C]);
+              tmem_st16(t_o + db * N, o);
             }
             tmem_st_wait();
           }
         }
+        filled = true;
+        // P(j - 2), which lies where P(j) goes, has been read
+        if (j >= 2 && !wait_for(sm.o_full + (j & 1), (uint32_t)(((j >> 1) - 1) & 1), abort_flag)) *abort_flag = 1;
         // ---- probabilities: the sum in fp32, P into shared memory as the B operand
-        if (j >= 2 && !mbar_wait(sm.o_full + (j & 1), (uint32_t)(((j >> 1) - 1) & 1), abort_flag)) *abort_flag = 1;
-        unsigned char* pw = sP + (j & 1) * S::PBUF + (tid >> 3) * 128 + (tid & 7) * 16;
+        unsigned char* pw = sP + (j & 1) * S::PBUF + (c0 / PW) * 2048 + (t >> 3) * 128 + (t & 7) * 16;
+        uint32_t hi[C / 4 * ES], lo[C / 4];  // packed P (bf16: hi alone)
 #pragma unroll
-        for (int n = 0; n < R; ++n) {
-          const float p = ex2_approx(x[n] - rs.mref[n]);
-          l[n] += p;
-          x[n] = ES == 1 ? p * (rs.w[n] * vs) : p;
-        }
-        if constexpr (ES == 2) {
+        for (int c = 0; c < C; c += CH) {
 #pragma unroll
-          for (int g = 0; g < R / PW; ++g) {
-            uint32_t w[4];
+          for (int k = 0; k < ES; ++k) hi[c / 4 * ES + k] = 0u;
+          lo[c / 4] = 0u;
+          if (c >= rr) continue;
+          const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
+          const float p[4] = {ex2_approx(z[c] + b4.x), ex2_approx(z[c + 1] + b4.y), ex2_approx(z[c + 2] + b4.z),
+                              ex2_approx(z[c + 3] + b4.w)};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2(x[g * PW + 2 * k], x[g * PW + 2 * k + 1]);
-            *reinterpret_cast<uint4*>(pw + g * 2048) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        } else {
-          uint32_t hi[R / 4], lo[R / 4];
-#pragma unroll
-          for (int k = 0; k < R / 4; ++k) {
-            uint32_t l0, l1;
-            const uint32_t h0 = split_e4m3x2(x[4 * k], x[4 * k + 1], &l0);
-            const uint32_t h1 = split_e4m3x2(x[4 * k + 2], x[4 * k + 3], &l1);
-            hi[k] = h0 | (h1 << 16);
-            lo[k] = l0 | (l1 << 16);
-          }
-          if constexpr (R == 8) {
-            *reinterpret_cast<uint4*>(pw) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+          for (int u = 0; u < CH; ++u) l[c + u] = ES == 1 ? fmaf(p[u], inv_vs, l[c + u]) : l[c + u] + p[u];
+          if constexpr (ES == 2) {
+            hi[c / 2] = pack_bf16x2(p[0], p[1]);
+            hi[c / 2 + 1] = pack_bf16x2(p[2], p[3]);
           } else {
-#pragma unroll
-            for (int g = 0; g < R / 16; ++g) {
-              *reinterpret_cast<uint4*>(pw + g * 2048) = make_uint4(hi[4 * g], hi[4 * g + 1], hi[4 * g + 2], hi[4 * g + 3]);
-              *reinterpret_cast<uint4*>(pw + (R / 16 + g) * 2048) =
-                  make_uint4(lo[4 * g], lo[4 * g + 1], lo[4 * g + 2], lo[4 * g + 3]);
-            }
+            uint32_t l0, l1;
+            const uint32_t h0 = split_e4m3x2<S::SIDE>(p[0], p[1], &l0);
+            const uint32_t h1 = split_e4m3x2<S::SIDE>(p[2], p[3], &l1);
+            hi[c / 4] = h0 | (h1 << 16);
+            lo[c / 4] = l0 | (l1 << 16);
           }
         }
-        if (p0 < wk.e.lo || p0 + kTile - 1 > wk.e.hi) {
-          // Positions that no row sees may hold anything (a zero probability times NaN is NaN):
-          // their rows of V become zero once the tile has landed.
+        if constexpr (S::SIDE) {
+          *reinterpret_cast<uint4*>(pw) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+        } else {
+          *reinterpret_cast<uint4*>(pw) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if constexpr (ES == 1) *reinterpret_cast<uint4*>(pw + S::PPART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          else *reinterpret_cast<uint4*>(pw + 2048) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+        }
+        if (p0 < wk.e.lo || p0 + kTile - 1 > wk.e.hi || odd) {
+          // Positions that no row sees may hold anything (a zero probability times NaN is NaN), and
+          // value scales of zero make no contribution: these rows of V become zero when the tile
+          // has landed.
           const int ld = 2 * j + 1, slot = ld % NS;
-          if (!mbar_wait(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
-          if (pos < wk.e.lo || pos > wk.e.hi) {
-            unsigned char* v = base + (size_t)slot * S::SLOT + tid * SW;
-#pragma unroll
+          if (!wait_for(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
+          const bool mine = TURNS || grp == 0;  // one group clears
+          if (mine && (pos < wk.e.lo || pos > wk.e.hi || (ES == 1 && !(sc.y >= 0x1p-100f)))) {
+            unsigned char* v = base + (size_t)slot * S::SLOT + t * SW;
+#pragma unroll 1
             for (int p = 0; p < S::ROWB / SW; ++p)
 #pragma unroll
               for (int c = 0; c < SW / 16; ++c)
@@ -815,67 +923,87 @@ __global__ void __launch_bounds__(kPThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(sm.p_full + (j & 1));
       }
-      // ---- end of the unit's part: join the threads' sums, scale O and write it
-#pragma unroll
-      for (int n = 0; n < R; ++n) {
-        float v = l[n];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == (n & 31)) rs.red[warp][0][n] = v;
-      }
-      named_bar_sync(1, 128);
-      if (!mbar_wait(sm.o_full + ((j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag)) *abort_flag = 1;
-      tc_fence_after();
+      // ---- end of the unit's part: join the threads' sums (and the groups', where they took turns),
+      //      scale O and write it
+      const float ls = warp_col_sums<C>(l, lane);
+      if (lane % (32 / C) == 0) rs.red[warp & 3][lane / (32 / C)] = ls;
+      if (TURNS) named_bar_sync(5, NSM);
+      else named_bar_sync(bar, 128);
       const bool whole = sg.first && sg.last;
       const int part = 2 * cta + (seg == 0 ? 0 : 1);
       const int unit = 2 * (wk.idx * a.Hkv + sg.hk) + (sg.first ? 1 : 0);
-      const bool good = !*abort_flag;
       if (!whole) (seg == 0 ? unit0 : unit1) = unit;
-      if (tid < R) {
-        const int n = tid;
-        const float sum = (rs.red[0][0][n] + rs.red[1][0][n]) + (rs.red[2][0][n] + rs.red[3][0][n]);
+      if (t < C) {
+        float m = rs.m[t], sum = (rs.red[0][t] + rs.red[1][t]) + (rs.red[2][t] + rs.red[3][t]), f = 1.f;
+        if (TURNS) {  // the other group's partial sums, reference and O
+          const RowState& ro = sm.rs[grp ^ 1];
+          const float so = (ro.red[0][t] + ro.red[1][t]) + (ro.red[2][t] + ro.red[3][t]);
+          const float top = fmaxf(m, ro.m[t]);
+          f = ex2_approx(m - top);
+          // the same order in both groups: they have to agree on the sum
+          const float mine = sum * f, other = so * ex2_approx(ro.m[t] - top);
+          sum = grp == 0 ? mine + other : other + mine;
+          m = top;
+        }
         // a NaN stays one; a row that may see nothing took part in the tiles that needed no mask
-        const bool some = !(sum == 0.f) && rc.lo[n] <= rc.hi[n];
-        rs.fin[n] = some ? 1.f / (rs.w[n] * sum) : 0.f;
-        const float lse = some ? (rs.mref[n] + log2f(sum)) * kLn2 : -INFINITY;
-        if (good) {
-          if (!whole) a.part_lse[(int64_t)part * R + n] = lse;
-          else if (rc.orow[n] >= 0) a.lse[rc.lrow[n]] = lse;
+        const bool some = !(sum == 0.f) && rc.lo[c0 + t] <= rc.hi[c0 + t];
+        rs.fin[t] = some ? f / sum : 0.f;
+        const float lse = some ? (m - kLift + log2f(sum)) * kLn2 : -INFINITY;
+        if (!*abort_flag && (!TURNS || grp == 0)) {
+          if (!whole) a.part_lse[(int64_t)part * R + c0 + t] = lse;
+          else if (rc.orow[c0 + t] >= 0) a.lse[rc.lrow[c0 + t]] = lse;
         }
       }
-      named_bar_sync(1, 128);
-      if (D >= 128 || warp < 2) {
-        constexpr int W = R < 16 ? 16 : (R < 32 ? 16 : 32);  // columns per read
+      // the last P V of each O
+      for (int k = max(j0, j - 2); k < j; ++k)
+        if (!wait_for(sm.o_full + (k & 1), (uint32_t)((k >> 1) & 1), abort_flag)) *abort_flag = 1;
+      tc_fence_after();
+      if (TURNS) named_bar_sync(5, NSM);
+      else named_bar_sync(bar, 128);
+      const bool good = !*abort_flag;
+      // which of the two O hold something
+      const bool has0 = !TURNS || j - j0 >= 2 || (j0 & 1) == 0, has1 = TURNS && (j - j0 >= 2 || (j0 & 1) == 1);
+      if (D >= 128 || (warp & 3) < 2) {
+        // rows [w0, w1) of this thread's c0.. are written by it; four at a time
+        const int w0 = TURNS ? grp * (C / 2) : 0, w1 = min(TURNS ? w0 + C / 2 : C, rr);
+        const RowState &r0 = sm.rs[TURNS ? 0 : grp], &r1 = sm.rs[1];
 #pragma unroll 1
-        for (int db = 0; db < S::NO; ++db) {
-          const int d = db * 128 + tid;
-#pragma unroll 1
-          for (int c = 0; c < R; c += W) {
-            const uint32_t at = t_lane + S::TM_O + db * N + c;
-            uint32_t h[W], lo[W];
-            tmem_cols<W>(at, h);
-            if constexpr (ES == 1 && R > 8) tmem_cols<W>(at + R, lo);
-            tmem_ld_wait();
-            reg_pin(h);
-            if constexpr (ES == 1 && R > 8) reg_pin(lo);
+        for (int k = 0; k < S::NO * C / 4; ++k) {
+          const int db = k / (C / 4), n0 = (k % (C / 4)) * 4, d = db * 128 + t;
+          if (n0 < w0 || n0 >= w1) continue;
+          const uint32_t at = t_lane + S::TM_O + db * N + c0 + n0;
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < (R < W ? R : W); ++k) {
-              float v = __uint_as_float(h[k]);
-              if constexpr (ES == 1) v = fmaf(__uint_as_float(R == 8 ? h[(8 + k) % W] : lo[k]), 0.0625f, v);
-              v *= rs.fin[c + k];
-              if (!good) continue;
-              if (!whole) {
-                a.part_o[((int64_t)part * R + c + k) * D + d] = v;
-              } else if (rc.orow[c + k] >= 0) {
-                reinterpret_cast<__nv_bfloat16*>(a.o.ptr)[rc.orow[c + k] + d] = __float2bfloat16_rn(v);
-              }
+          for (int g = 0; g < (TURNS ? 2 : 1); ++g) {
+            if (!(g ? has1 : has0)) continue;
+            uint32_t x[4], y[4];
+            tmem_ld4(at + g * S::ON, x);
+            if constexpr (S::SIDE) tmem_ld4(at + g * S::ON + 8, y);
+            tmem_ld_wait();
+            reg_pin(x);
+            if constexpr (S::SIDE) reg_pin(y);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              float o = __uint_as_float(x[u]);
+              if constexpr (S::SIDE) o = fmaf(__uint_as_float(y[u]), 0.0625f, o);
+              v[u] = fmaf(o, (g ? r1 : r0).fin[n0 + u], v[u]);
             }
+          }
+          if (!good) continue;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int n = c0 + n0 + u;
+            if (!whole) a.part_o[((int64_t)part * R + n) * D + d] = v[u];
+            else if (rc.orow[n] >= 0) reinterpret_cast<__nv_bfloat16*>(a.o.ptr)[rc.orow[n] + d] = __float2bfloat16_rn(v[u]);
           }
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.q_empty + (seg & 1));
+      // O may be overwritten, and the sums and references set anew, when all of its readers are here
+      if (TURNS) named_bar_sync(5, NSM);
+      else named_bar_sync(bar, 128);
     }
     if (tid == 0) {
       a.part_unit[2 * cta] = unit0;
@@ -885,7 +1013,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == W_S) {
     tc_fence_after();
     tmem_dealloc(tmem, S::TM_COLS);
   }
@@ -896,7 +1024,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
 // resident when the last CTA of the attention kernel ends.
 template <int D, int R>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a, const int ctas) {
-  __shared__ float w_sh[8][2 * kSms + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, n = blockIdx.y * 8 + warp;
   griddep_wait();
   const int u0 = a.part_unit[2 * c], u1 = a.part_unit[2 * c + 1];
@@ -910,39 +1037,39 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a, con
   } else {
     return;
   }
-  int parts = 1;  // the unit's parts: `first`, then slot 2 (c + k) of the CTAs that follow
-  for (int k = c + 1; k < ctas; k += 32) {
-    const bool same = k + lane < ctas && a.part_unit[2 * (k + lane)] == 2 * key;
-    const unsigned m = __ballot_sync(0xffffffffu, same);
-    const int run = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
-    parts += run;
-    if (run < 32) break;
-  }
   const int e = key / a.Hkv, hk = key % a.Hkv, b = e / a.groups, m = (e % a.groups) * R + n;
   if (n >= R || m >= a.M) return;
-  auto slot = [&](int k) -> int64_t { return k == 0 ? first : 2 * (c + k); };
-  float* w = w_sh[warp];
-  float top = -INFINITY;
-  for (int k = lane; k < parts; k += 32) top = fmaxf(top, a.part_lse[slot(k) * R + n]);
-  top = warp_max(top);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int k = lane; k < parts; k += 32) {
-    const float v = expf(a.part_lse[slot(k) * R + n] - ref);
-    w[k] = v;
-    sum += v;
-  }
+  // The unit's parts: `first`, then slot 2 k of the CTAs k that follow as long as it is this unit's.
+  // 32 parts at a time: lane k weighs part k, then every lane sums its elements of D over the parts,
+  // rescaled when a later batch has a larger lse.
+  float acc[D / 32], top = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncwarp();
-  float acc[D / 32];
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  for (int k0 = 0;; k0 += 32) {
+    const int k = k0 + lane;  // part; CTA c + k
+    const bool same = k == 0 || (c + k < ctas && a.part_unit[2 * (c + k)] == 2 * key);
+    const unsigned m32 = __ballot_sync(0xffffffffu, same);
+    const int run = m32 == 0xffffffffu ? 32 : __ffs(~m32) - 1;
+    if (run == 0) break;
+    const float ls = lane < run ? a.part_lse[(int64_t)(k == 0 ? first : 2 * (c + k)) * R + n] : -INFINITY;
+    const float nt = fmaxf(top, warp_max(ls)), ref = nt == -INFINITY ? 0.f : nt;
+    const float w = lane < run ? expf(ls - ref) : 0.f;
+    float ws = w;
 #pragma unroll
-  for (int k = 0; k < D / 32; ++k) acc[k] = 0.f;
+    for (int o = 16; o; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+    const float back = top == -INFINITY ? 0.f : expf(top - ref);
+    sum = sum * back + ws;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] *= back;
+    top = nt;
 #pragma unroll 4
-  for (int k = 0; k < parts; ++k) {
-    const float* po = a.part_o + (slot(k) * R + n) * D + lane;
+    for (int i = 0; i < run; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      const float* po = a.part_o + ((int64_t)(k0 + i == 0 ? first : 2 * (c + k0 + i)) * R + n) * D + lane;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w[k], po[32 * i], acc[i]);
+      for (int v = 0; v < D / 32; ++v) acc[v] = fmaf(wi, po[32 * v], acc[v]);
+    }
+    if (run < 32) break;
   }
   const int i = m / a.G, h = hk * a.G + m % a.G;
   __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.o.ptr) + (int64_t)b * a.o.stride_b +
@@ -951,7 +1078,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a, con
   const float inv = some ? 1.f / sum : 0.f;
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) o[lane + 32 * k] = __float2bfloat16_rn(acc[k] * inv);
-  if (lane == 0) a.lse[((int64_t)b * a.H + h) * a.Tq + i] = some ? ref + logf(sum) : -INFINITY;
+  if (lane == 0) a.lse[((int64_t)b * a.H + h) * a.Tq + i] = some ? (top == -INFINITY ? 0.f : top) + logf(sum) : -INFINITY;
 }
 
 struct PagedPlan {
@@ -1005,13 +1132,13 @@ int check_paged(const FaPagedAttnParams* p) {
 template <int D, int ES, int R>
 cudaError_t launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedArgs& a, const PagedPlan& pl,
                          cudaStream_t stream) {
-  const size_t fixed = paged_smem_bytes<D, ES, R>(0), limit = 232448;
+  const size_t fixed = paged_smem_bytes<D, ES, R>(0), limit = 232448 - 2048;  // room for a block of the merge kernel
   a.slots = (int)std::min<size_t>(kMaxSlots, (limit - fixed) / Shape<D, ES, R>::SLOT);
   const size_t smem = paged_smem_bytes<D, ES, R>(a.slots);
   cudaError_t e =
       cudaFuncSetAttribute(paged_attn_kernel<D, ES, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  paged_attn_kernel<D, ES, R><<<pl.ctas, kPThreads, smem, stream>>>(tk, tv, a);
+  paged_attn_kernel<D, ES, R><<<pl.ctas, Shape<D, ES, R>::NT, smem, stream>>>(tk, tv, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (a.cols * a.ps <= kTile) return cudaSuccess;  // one tile per unit: no unit crosses CTAs
   cudaLaunchConfig_t cfg = {};

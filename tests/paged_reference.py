@@ -111,11 +111,11 @@ def attend64(q, cache, table, lens, qlens, kind, window, slopes, cap, scale, hid
             see = see & ~gone[None]
             s = torch.einsum("gtd,nd->gtn", qq, kk) * scale
             # S: D exact products summed in fp32 (each addition off by 2^-23 of the terms' sum at most), an
-            # 8-bit q split exact down to 2^-20 of its largest element, three fp32 products after it
+            # 8-bit q split exact down to 2^-17 of its largest element, three fp32 products after it
             mag = torch.einsum("gtd,nd->gtn", qq.abs(), kk.abs()) * scale
             err = mag * (D + 16) * 2.0 ** -23 + s.abs() * 4 * U_F32
             if f8:
-                err = err + 2.0 ** -20 * qq.abs().amax(-1, keepdim=True) * kk.abs().sum(-1) * scale
+                err = err + 2.0 ** -17 * qq.abs().amax(-1, keepdim=True) * kk.abs().sum(-1) * scale
             if slopes is not None:
                 al = slopes[hk * G:(hk + 1) * G].double()[:, None, None] * (pos[None] - qpos[:, None]).double()
                 s = s + al
@@ -123,7 +123,8 @@ def attend64(q, cache, table, lens, qlens, kind, window, slopes, cap, scale, hid
             if cap:
                 s = cap * torch.tanh(s / cap)
                 err = err + cap * 2.0 ** -21  # 1 - 2 / (1 + e^z): exponential, quotient and sum, 2^-23 each at most
-            err = err + s.abs() * 2 * U_F32 + 2.0 ** -22  # into log2 units and back, the exponential itself
+            # into log2 units and back, the exponential itself, and the sum with log2 vs
+            err = err + s.abs() * 2 * U_F32 + 2.0 ** -22 + vs.clamp(min=2.0 ** -100).log2().abs() * 2 * U_F32
             s = s.masked_fill(~see, -math.inf)
             top = s.amax(-1, keepdim=True)
             top = torch.where(top == -math.inf, torch.zeros_like(top), top)
@@ -141,9 +142,9 @@ def attend64(q, cache, table, lens, qlens, kind, window, slopes, cap, scale, hid
             rel = U_BF16 + 2.1 * dx[..., None] + (n + 64) * 2.0 ** -23
             tol = pv * rel + oo.abs() * U_BF16
             if f8:
-                # parts below e4m3's smallest step: 2^-14 of P, where the largest p vs is at least 2^4
+                # parts below e4m3's smallest step: 2^-10 of P, where the largest p vs is at least 2^7
                 big = (p * vs).amax(-1, keepdim=True)
-                tol = tol + 2.0 ** -18 * big * v0.div(vs.clamp(min=2.0 ** -100)[:, None]).abs().sum(0)
+                tol = tol + 2.0 ** -17 * big * v0.div(vs.clamp(min=2.0 ** -100)[:, None]).abs().sum(0)
             sl = slice(hk * G, (hk + 1) * G)
             o[b, sl, :t] = oo
             lse[b, sl, :t] = torch.where(some, top[..., 0] + torch.log(z), torch.full_like(z, -math.inf))
