@@ -15,12 +15,12 @@
 // 8-bit codes go to the tensor cores as they are (kind::f8f6f4): converting a tile in shared memory
 // would cost as many instructions as everything else here.  The other operand is split into two e4m3
 // parts, z = hi + lo, that meet in the fp32 accumulator: both parts' MMAs add to the same columns
-// (R >= 16), or for R = 8 the parts lie side by side in the MMA's smallest N of 16, with lo held
-// times 16, and are added when read.  q is scaled by a power of two per row so that its largest
-// magnitude lies in [128, 256): a bf16 has 8 significant bits, each part 4, so the split is exact
-// down to 2^-17 of the row's largest element.  Probabilities lie in [0, 431] with a largest one
-// of at least 128 / 431 of that: the split is off by 2^-8 relative (as a bf16 P is), or 2^-17 of the
-// largest below that.
+// (R >= 16), or for R = 8 the parts lie side by side in the MMA's smallest N of 16 and are added
+// when read.  q is scaled by a power of two per row so that its largest magnitude lies in [128, 256):
+// a bf16 has 8 significant bits, each part 4, so the split is exact down to 2^-17 of the row's largest
+// element.  Probabilities lie in [0, 431], the largest of a tile that moved the reference at 128: hi
+// is P cut to 4 bits, lo the rest rounded to 4, off by 2^-8 relative (as a bf16 P is) or by 2^-17 of
+// the largest below that.
 //
 // Scales.  ks multiplies the thread's logits.  vs goes into the exponent: with z = x + log2 vs and
 // a reference m >= max z - 1.75 per row, P = 2^(z - m + 7) weighs the codes, and the softmax sum
@@ -60,13 +60,16 @@ constexpr int kTile = 128;         // cached positions of a tile: the MMA's M
 constexpr int kSms = 148;
 constexpr int kMaxSlots = 24;      // K or V tiles in the shared-memory ring
 constexpr int kScaleRing = 16;     // tiles whose scales may be live at once (> kMaxSlots / 2 + 1)
-constexpr float kSlack = 1.75f;    // a reference moves when exceeded by more than this (log2 units)
-constexpr float kLift = 7.f;       // P = 2^(z - reference + kLift) <= 2^8.75 = 431: below e4m3's 448
+// A reference moves when exceeded by more than slack (log2 units), and P = 2^(z - reference + lift).
+// 8-bit: P in units of 2^-8, so that fp16's exponents line up with e4m3's (split_e4m3x4); at most
+// 2^(7 + 1.75) = 431, below e4m3's 448.  bf16: any size fits.
+__host__ __device__ constexpr float slack_of(int ES) { return ES == 1 ? 1.75f : 8.f; }
+__host__ __device__ constexpr float lift_of(int ES) { return ES == 1 ? 7.f - 8.f : 0.f; }
 constexpr float kUnset = -1e30f;   // reference of a row that has seen nothing yet
 
 struct PagedArgs {
   int B, H, Hkv, Tq, G, M;         // M = G * Tq query rows per sequence and K/V head
-  int ps, cols, num_pages, groups; // groups of R query rows per (sequence, K/V head)
+  int ps_log, cols, num_pages, groups; // groups of R query rows per (sequence, K/V head)
   int entries;                     // B * groups
   int slots;                       // ring depth
   int q_vec;
@@ -120,48 +123,35 @@ template <int R> struct RowConst {
 };
 // Running state of one softmax group: its rows, or its share of the tiles.
 struct RowState {
-  float m[16], bias[16];  // reference; kLift - reference
+  float m[16], bias[16];  // reference; lift - reference
   float move[16];         // factor of the last move
   float red[4][16];
   float fin[16];          // factor of O at the end
 };
-template <int R> struct Smem {
-  RowConst<R> rc[2];
-  RowState rs[R <= 16 ? 2 : R / 16];
-  float2 scales[kScaleRing][8];  // (ks, vs) of a tile's pages; ks = -inf hides the page
-  int odd[kScaleRing];           // the tile has a hidden page, or one of a scale below 2^-100
-  uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], fin_bar[2];
-  int scan[24];
-  int total, per_cta, first_entry, first_off;
-  uint32_t tmem;
-  int abort_flag, never;
-};
-
-template <int D, int ES, int R>
-size_t paged_smem_bytes(int slots) {
-  using S = Shape<D, ES, R>;
-  return 1024 + (size_t)slots * S::SLOT + 2 * S::QBUF + 2 * S::PBUF + sizeof(Smem<R>);
-}
-
 // What one (sequence, row group) has to visit.
 struct Entry {
-  int b, rg, len, ql, i0, i1;  // tokens i0..i1 (clipped to the valid ones)
-  int lo, hi;                  // positions that some row of the group may see
-  int in_lo, in_hi;            // positions that every valid row of the group may see
-  int t0, nt;                  // tiles
+  int b, rg, len, ql;
+  int lo, hi;        // positions that some row of the group may see
+  int in_lo, in_hi;  // positions that every valid row of the group may see
+  int t0, nt;        // tiles
 };
 
 template <int R>
 __device__ __forceinline__ Entry entry_of(const PagedArgs& a, int e) {
   Entry x;
-  x.b = e / a.groups;
+  x.b = a.groups == 1 ? e : e / a.groups;
   x.rg = e - x.b * a.groups;
-  const int cap = a.cols * a.ps;
-  x.len = min(max(__ldg(a.kv_lens + x.b), 0), cap);
-  x.ql = a.q_lens ? min(max(__ldg(a.q_lens + x.b), 0), a.Tq) : a.Tq;
-  x.i0 = x.rg * R / a.G;
-  x.i1 = min((min(x.rg * R + R, a.M) - 1) / a.G, x.ql - 1);
-  const int p0 = x.len - x.ql + x.i0, p1 = x.len - x.ql + x.i1;  // positions of the group's rows
+  const int cap = a.cols << a.ps_log;
+  const int len = __ldg(a.kv_lens + x.b), ql = a.q_lens ? __ldg(a.q_lens + x.b) : a.Tq;
+  x.len = min(max(len, 0), cap);
+  x.ql = min(max(ql, 0), a.Tq);
+  int i0 = 0, i1 = a.Tq - 1;  // tokens of the group's rows
+  if (a.groups > 1) {
+    i0 = x.rg * R / a.G;
+    i1 = (min(x.rg * R + R, a.M) - 1) / a.G;
+  }
+  i1 = min(i1, x.ql - 1);
+  const int p0 = x.len - x.ql + i0, p1 = x.len - x.ql + i1;  // positions of the group's rows
   x.lo = 0;
   x.hi = x.len - 1;
   x.in_lo = 0;
@@ -181,7 +171,7 @@ __device__ __forceinline__ Entry entry_of(const PagedArgs& a, int e) {
     }
   }
   x.t0 = x.lo / kTile;
-  x.nt = (x.i1 < x.i0 || x.hi < x.lo) ? 0 : x.hi / kTile - x.t0 + 1;
+  x.nt = (i1 < i0 || x.hi < x.lo) ? 0 : x.hi / kTile - x.t0 + 1;
   return x;
 }
 
@@ -190,19 +180,22 @@ struct Seg {
   int hk, t0, nt;   // K/V head, first tile (absolute), tiles
   bool first, last; // holds the unit's first / last tile
 };
+struct Start {  // where a CTA's range begins
+  Entry e;
+  int idx, hk, off;
+};
 template <int R>
 struct Walker {
   Entry e;
   int idx, hk, off, left;
-  __device__ __forceinline__ void begin(const PagedArgs& a, int entry, int entry_off, int tiles) {
+  __device__ __forceinline__ void begin(const Start& s, int tiles) {
     left = tiles;
-    idx = entry;
-    hk = off = 0;
     e.nt = 0;
     if (tiles > 0) {
-      e = entry_of<R>(a, entry);
-      hk = entry_off / e.nt;
-      off = entry_off - hk * e.nt;
+      e = s.e;
+      idx = s.idx;
+      hk = s.hk;
+      off = s.off;
     }
   }
   // Moves tiles beyond a unit's end on into the next head, or the next entry that has tiles.
@@ -227,6 +220,24 @@ struct Walker {
     return true;
   }
 };
+
+template <int R> struct Smem {
+  RowConst<R> rc[2];
+  RowState rs[R <= 16 ? 2 : R / 16];
+  float2 scales[kScaleRing][8];  // (ks, vs) of a tile's pages; ks = -inf hides the page
+  int odd[kScaleRing];           // the tile has a hidden page, or one of a scale below 2^-100
+  uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], fin_bar[2];
+  int scan[24];
+  Start start;
+  uint32_t tmem;
+  int abort_flag, never;
+};
+
+template <int D, int ES, int R>
+size_t paged_smem_bytes(int slots) {
+  using S = Shape<D, ES, R>;
+  return 1024 + (size_t)slots * S::SLOT + 2 * S::QBUF + 2 * S::PBUF + sizeof(Smem<R>);
+}
 
 // mbar_wait that looks at the clock only now and then: most waits here are short.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -270,16 +281,26 @@ __device__ __forceinline__ __half2 e4m3x2_value(uint32_t v) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
   return *reinterpret_cast<const __half2*>(&h);
 }
-// Two values of magnitude up to 448 as hi + lo (lo held times 16 if X16): packed hi parts, lo parts
-// through *lo2.  Between the two e4m3 parts the value passes through fp16: 11 bits, finer than both.
-template <bool X16>
+// Two values of magnitude up to 448 as hi + lo: packed hi parts, lo parts through *lo2.  Between the
+// two parts the value passes through fp16: 11 bits, finer than both.
 __device__ __forceinline__ uint32_t split_e4m3x2(float a, float b, uint32_t* lo2) {
   const __half2 v = __floats2half2_rn(a, b);
   const uint32_t h = e4m3x2(v);
-  __half2 r = __hsub2(v, e4m3x2_value(h));
-  if (X16) r = __hmul2(r, __float2half2_rn(16.f));
-  *lo2 = e4m3x2(r);
+  *lo2 = e4m3x2(__hsub2(v, e4m3x2_value(h)));
   return h;
+}
+// The same for four values >= 0 in units of 2^-8 (so at most 1.75), with integer operations: an fp16
+// in these units is the e4m3 code shifted left by 7 bits, down to the subnormal ones, so cutting an
+// fp16 to its upper 9 bits is a truncation to e4m3.  The conversion instructions (three for two
+// values) run at a fraction of the rate and bounded the kernel at 64 rows.  NaN stays NaN.
+__device__ __forceinline__ uint32_t split_e4m3x4(const float (&p)[4], uint32_t* lo4) {
+  const __half2 a = __floats2half2_rn(p[0], p[2]), b = __floats2half2_rn(p[1], p[3]);
+  uint32_t ha = *reinterpret_cast<const uint32_t*>(&a) & 0x7f807f80u, hb = *reinterpret_cast<const uint32_t*>(&b) & 0x7f807f80u;
+  const __half2 ra = __hsub2(a, *reinterpret_cast<const __half2*>(&ha)), rb = __hsub2(b, *reinterpret_cast<const __half2*>(&hb));
+  const uint32_t la = (*reinterpret_cast<const uint32_t*>(&ra) + 0x00400040u) & 0x7f807f80u,
+                 lb = (*reinterpret_cast<const uint32_t*>(&rb) + 0x00400040u) & 0x7f807f80u;
+  *lo4 = (la >> 7) | (lb << 1);
+  return (ha >> 7) | (hb << 1);
 }
 
 // Byte offset of 16-byte chunk c of row r in a panel of rows of SW bytes, swizzled over SW.
@@ -397,7 +418,7 @@ __device__ __forceinline__ void build_q(const PagedArgs& a, const Entry& e, int 
         if (top == INFINITY) fix = __uint_as_float(0x7fc00000u);  // NaN or infinity in q: the row is NaN
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) hi[k] = split_e4m3x2<S::SIDE>(f[2 * k] * up, f[2 * k + 1] * up, &lo[k]);
+        for (int k = 0; k < 4; ++k) hi[k] = split_e4m3x2(f[2 * k] * up, f[2 * k + 1] * up, &lo[k]);
         if (n < R) {
           unsigned char* at = q + (d0 / SW) * S::QPANEL + (d0 & 8);
           const int c = (d0 % SW) >> 4;
@@ -477,21 +498,20 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     tmem_alloc(&sm.tmem, S::TM_COLS);
     tmem_relinquish();
   }
+  int my_tiles;
   {
     // Exclusive prefix of the entries' tiles over the threads, each with a run of entries.
-    const int run = (a.entries + NT - 1) / NT, e0 = min(tid * run, a.entries),
-              e1 = min(e0 + run, a.entries);
+    const int run = (a.entries + NT - 1) / NT, e0 = min(tid * run, a.entries), e1 = min(e0 + run, a.entries);
     int mine = 0;
-    bool bad = false;
+    Entry x;
     for (int e = e0; e < e1; ++e) {
-      const Entry x = entry_of<R>(a, e);
+      x = entry_of<R>(a, e);
       mine += x.nt * a.Hkv;
-      if (x.rg == 0) {
+      if (x.rg == 0 && cta == 0) {
         const int n = __ldg(a.kv_lens + x.b), t = a.q_lens ? __ldg(a.q_lens + x.b) : 0;
-        bad = bad || n < 0 || n > a.cols * a.ps || t < 0 || t > a.Tq;
+        if (n < 0 || n > a.cols << a.ps_log || t < 0 || t > a.Tq) report_status(a.status, FA_ERR_INVALID);
       }
     }
-    if (bad && cta == 0) report_status(a.status, FA_ERR_INVALID);
     int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -503,43 +523,42 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < NT / 32; ++w) {
-      if (w < warp) before += sm.scan[w];
-      total += sm.scan[w];
+      const int v = sm.scan[w];
+      if (w < warp) before += v;
+      total += v;
     }
     const int per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     const int start = (int)min((int64_t)cta * per, (int64_t)total);
+    my_tiles = min(per, total - start);
     int at = before + inc - mine;
-    if (start < total && at <= start && start < at + mine) {
+    if (start < total && at <= start && start < at + mine) {  // the range begins in one of this thread's entries
       for (int e = e0; e < e1; ++e) {
-        const int n = entry_of<R>(a, e).nt * a.Hkv;
+        if (run > 1) x = entry_of<R>(a, e);
+        const int n = x.nt * a.Hkv;
         if (start < at + n) {
-          sm.first_entry = e;
-          sm.first_off = start - at;
+          sm.start.e = x;
+          sm.start.idx = e;
+          sm.start.hk = (start - at) / x.nt;
+          sm.start.off = start - at - sm.start.hk * x.nt;
           break;
         }
         at += n;
       }
-    }
-    if (tid == 0) {
-      sm.total = total;
-      sm.per_cta = per;
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  const int my_start = (int)min((int64_t)cta * sm.per_cta, (int64_t)sm.total);
-  const int my_tiles = min(sm.per_cta, sm.total - my_start);
   Walker<R> wk;
-  wk.begin(a, sm.first_entry, sm.first_off, my_tiles);
+  wk.begin(sm.start, my_tiles);
   Seg sg;
 
   if (warp == W_LOAD) {
     // ---------------------------------------------------------------- producer
     // A batch of 32 pages (32 / pages-per-tile tiles): each lane holds the number and the scales of one
     // page, and fetches the next batch's while this one's loads go out.
-    const int ppt = kTile / a.ps, batch = 32 / ppt, sub = lane / ppt, pg = lane - sub * ppt;
+    const int ppt_log = 7 - a.ps_log, ppt = 1 << ppt_log, batch = 32 >> ppt_log, sub = lane >> ppt_log, pg = lane & (ppt - 1);
     struct Page {
       int page, hk, active;
       float ks, vs;
@@ -551,10 +570,10 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       x.hk = 0;
       if (at < my_tiles) {
         wk.settle(a);
-        const int pos = (wk.e.t0 + wk.off) * kTile + pg * a.ps;
+        const int pos = (wk.e.t0 + wk.off) * kTile + (pg << a.ps_log);
         x.hk = wk.hk;
-        x.active = pos <= wk.e.hi && pos + a.ps > wk.e.lo;
-        if (x.active) x.page = __ldg(a.table + (int64_t)wk.e.b * a.table_stride + pos / a.ps);
+        x.active = pos <= wk.e.hi && pos + (1 << a.ps_log) > wk.e.lo;
+        if (x.active) x.page = __ldg(a.table + (int64_t)wk.e.b * a.table_stride + (pos >> a.ps_log));
       }
       at += batch;
       wk.off += batch;
@@ -585,11 +604,11 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       if (hid && lane == 0) report_status(a.status, FA_ERR_INVALID);
       const int page = hidden ? a.num_pages : x.page;  // reads as zeros: the map's bounds check
       const int n = min(batch, my_tiles - j0);
-      const unsigned pages = ppt == 32 ? 0xffffffffu : (1u << ppt) - 1u;
+      const unsigned pages = (1u << ppt) - 1u;
       unsigned small = 0;
       for (int k = 0; ok && k < n; ++k) {
         const int ring = (j0 + k) % kScaleRing;
-        const uint32_t bytes = (uint32_t)__popc((act >> (k * ppt)) & pages) * a.ps * S::ROWB;
+        const uint32_t bytes = ((uint32_t)__popc((act >> (k << ppt_log)) & pages) << a.ps_log) * S::ROWB;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           ok = wait_for_w(sm.empty + slot, phase, abort_flag);
@@ -597,7 +616,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           if (lane == 0) mbar_expect_tx(sm.full + slot, bytes);
           __syncwarp();
           if (sub == k && x.active) {
-            unsigned char* dst = base + (size_t)slot * S::SLOT + (size_t)pg * a.ps * SW;
+            unsigned char* dst = base + (size_t)slot * S::SLOT + (size_t)(pg << a.ps_log) * SW;
 #pragma unroll
             for (int p = 0; p < S::ROWB / SW; ++p)
               tma_load_4d(dst + p * S::PANEL, kv ? &tv : &tk, sm.full + slot, p * (SW / ES), 0, x.hk, page);
@@ -607,7 +626,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
             // there before the slot's barrier can complete.
             if (ES == 1 && k == 0) small = __ballot_sync(0xffffffffu, x.active && !(x.vs >= 0x1p-100f));
             if (sub == k) sm.scales[ring][pg] = make_float2(x.ks, x.vs);
-            if (lane == 0) sm.odd[ring] = (((hid | small) >> (k * ppt)) & pages) != 0;
+            if (lane == 0) sm.odd[ring] = (((hid | small) >> (k << ppt_log)) & pages) != 0;
             __syncwarp();
           }
           if (lane == 0) mbar_arrive(sm.full + slot);
@@ -754,8 +773,10 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     const uint32_t t_o = t_lane + S::TM_O + (TURNS ? grp * S::ON : c0);
     const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0, alibi = (a.score.flags & FA_SCORE_ALIBI) != 0;
     const float cap2 = capped ? a.score.softcap * kLog2e : 0.f, cap_k = capped ? 2.f * kLog2e / a.score.softcap : 0.f;
-    const int my_page = t / a.ps;
+    const int my_page = t >> a.ps_log;
+    constexpr float LIFT = lift_of(ES), SLACK = slack_of(ES);
     constexpr int PW = 16 / ES;  // rows per 16-byte store of P
+    constexpr bool KEEP = NG < 4;
     constexpr int CH = 4;        // rows worked on together; the ones behind the last real row are left out
     int unit0 = -1, unit1 = -1, j = 0;
     for (int seg = 0; wk.next(a, &sg); ++seg) {
@@ -768,15 +789,19 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       const int rr = min(a.M - wk.e.rg * R - c0, C);  // this thread's real rows
       if (t < C) {
         rs.m[t] = kUnset;
-        rs.bias[t] = kLift - kUnset;
+        rs.bias[t] = LIFT - kUnset;
       }
       // No wait leaves the loops: after a time-out every later wait returns at once and nothing is
       // written at the end.
       if (!wait_for(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag)) *abort_flag = 1;
       named_bar_sync(bar, 128);
-      float l[C];
+      float l[C], xs[C], bias[C];  // (640 threads have no registers for the constants: read per tile)
 #pragma unroll
-      for (int n = 0; n < C; ++n) l[n] = 0.f;
+      for (int n = 0; n < C; ++n) {
+        l[n] = 0.f;
+        xs[n] = rc.xs[c0 + n];
+        bias[n] = LIFT - kUnset;
+      }
       bool filled = false;  // this group's O holds something of this unit
       const int j0 = j;     // the unit's first tile
       for (int it = 0; it < sg.nt; ++it, ++j) {
@@ -796,6 +821,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         const bool inside = p0 >= wk.e.in_lo && p0 + kTile - 1 <= wk.e.in_hi && !odd;
         tmem_ld_wait();
         reg_pin(r);
+        const bool special = alibi | capped | !inside;
         float z[C], top = -INFINITY;
 #pragma unroll
         for (int c = 0; c < C; c += CH) {
@@ -804,34 +830,35 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
             for (int n = c; n < c + CH; ++n) z[n] = -INFINITY;
             continue;
           }
-          const float4 k4 = *reinterpret_cast<const float4*>(rc.xs + c0 + c);
-          const float xs[4] = {k4.x, k4.y, k4.z, k4.w};
-#pragma unroll
-          for (int u = 0; u < CH; ++u) {
-            float x = __uint_as_float(r[c + u]);
-            if constexpr (S::SIDE) x = fmaf(__uint_as_float(r[8 + c + u]), 0.0625f, x);
-            const float k = ES == 1 ? ks * xs[u] : xs[u];
-            z[c + u] = (alibi | capped) ? x * k : fmaf(x, k, lv);
+          if constexpr (!KEEP) {
+            const float4 k4 = *reinterpret_cast<const float4*>(rc.xs + c0 + c);
+            xs[c] = k4.x, xs[c + 1] = k4.y, xs[c + 2] = k4.z, xs[c + 3] = k4.w;
           }
-          if (alibi | capped) {
 #pragma unroll
-            for (int u = 0; u < CH; ++u) {
-              float x = z[c + u];
-              if (alibi) x = fmaf(rc.slope[c0 + c + u], (float)(pos - rc.qpos[c0 + c + u]), x);
+          for (int n = c; n < c + CH; ++n) {
+            float x = __uint_as_float(r[n]);
+            if constexpr (S::SIDE) x += __uint_as_float(r[8 + n]);
+            z[n] = ES == 1 ? fmaf(x, ks * xs[n], lv) : x * xs[n];
+          }
+          if (special) {
+#pragma unroll
+            for (int n = c; n < c + CH; ++n) {
+              float x = __uint_as_float(r[n]);
+              if constexpr (S::SIDE) x += __uint_as_float(r[8 + n]);
+              x *= ES == 1 ? ks * xs[n] : xs[n];
+              if (alibi) x = fmaf(rc.slope[c0 + n], (float)(pos - rc.qpos[c0 + n]), x);
               // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))), in log2 units
               if (capped) x = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + ex2_approx(x * cap_k)), cap2);
-              z[c + u] = x + lv;
+              z[n] = (!shown | (pos < rc.lo[c0 + n]) | (pos > rc.hi[c0 + n])) ? -INFINITY : x + lv;
             }
           }
-          if (!inside) {
-#pragma unroll
-            for (int u = 0; u < CH; ++u)
-              if (!shown | (pos < rc.lo[c0 + c + u]) | (pos > rc.hi[c0 + c + u])) z[c + u] = -INFINITY;
+          if constexpr (!KEEP) {
+            const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
+            bias[c] = b4.x, bias[c + 1] = b4.y, bias[c + 2] = b4.z, bias[c + 3] = b4.w;
           }
-          const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
-          top = fmax3f(top, fmax3f(z[c] + b4.x, z[c + 1] + b4.y, z[c + 2] + b4.z), z[c + 3] + b4.w);
+          top = fmax3f(top, fmax3f(z[c] + bias[c], z[c + 1] + bias[c + 1], z[c + 2] + bias[c + 2]), z[c + 3] + bias[c + 3]);
         }
-        if (vote_or(bar, 128, top > kLift + kSlack)) {
+        if (vote_or(bar, 128, top > LIFT + SLACK)) {
           // ---- a reference has to move to the tile's largest z of its row
 #pragma unroll
           for (int n = 0; n < C; ++n) {
@@ -842,14 +869,17 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           if (t < C) {
             const float old = rs.m[t];
             const float nm = fmaxf(fmaxf(rs.red[0][t], rs.red[1][t]), fmaxf(rs.red[2][t], rs.red[3][t]));
-            const float m = nm > old + kSlack ? nm : old;
+            const float m = nm > old + SLACK ? nm : old;
             rs.move[t] = m != old ? ex2_approx(old - m) : 1.f;
             rs.m[t] = m;
-            rs.bias[t] = kLift - m;
+            rs.bias[t] = LIFT - m;
           }
           named_bar_sync(bar, 128);
 #pragma unroll
-          for (int n = 0; n < C; ++n) l[n] *= rs.move[n];
+          for (int n = 0; n < C; ++n) {
+            l[n] *= rs.move[n];
+            bias[n] = rs.bias[n];
+          }
           if (filled) {  // this O's last P V must have retired
             const int jo = j - (TURNS ? 2 : 1);
             if (!wait_for(sm.o_full + (jo & 1), (uint32_t)((jo >> 1) & 1), abort_flag)) *abort_flag = 1;
@@ -879,20 +909,20 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           for (int k = 0; k < ES; ++k) hi[c / 4 * ES + k] = 0u;
           lo[c / 4] = 0u;
           if (c >= rr) continue;
-          const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
-          const float p[4] = {ex2_approx(z[c] + b4.x), ex2_approx(z[c + 1] + b4.y), ex2_approx(z[c + 2] + b4.z),
-                              ex2_approx(z[c + 3] + b4.w)};
+          if constexpr (!KEEP) {
+            const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
+            bias[c] = b4.x, bias[c + 1] = b4.y, bias[c + 2] = b4.z, bias[c + 3] = b4.w;
+          }
+          float p[4];
+#pragma unroll
+          for (int u = 0; u < CH; ++u) p[u] = ex2_approx(z[c + u] + bias[c + u]);
 #pragma unroll
           for (int u = 0; u < CH; ++u) l[c + u] = ES == 1 ? fmaf(p[u], inv_vs, l[c + u]) : l[c + u] + p[u];
           if constexpr (ES == 2) {
             hi[c / 2] = pack_bf16x2(p[0], p[1]);
             hi[c / 2 + 1] = pack_bf16x2(p[2], p[3]);
           } else {
-            uint32_t l0, l1;
-            const uint32_t h0 = split_e4m3x2<S::SIDE>(p[0], p[1], &l0);
-            const uint32_t h1 = split_e4m3x2<S::SIDE>(p[2], p[3], &l1);
-            hi[c / 4] = h0 | (h1 << 16);
-            lo[c / 4] = l0 | (l1 << 16);
+            hi[c / 4] = split_e4m3x4(p, &lo[c / 4]);
           }
         }
         if constexpr (S::SIDE) {
@@ -947,8 +977,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         }
         // a NaN stays one; a row that may see nothing took part in the tiles that needed no mask
         const bool some = !(sum == 0.f) && rc.lo[c0 + t] <= rc.hi[c0 + t];
-        rs.fin[t] = some ? f / sum : 0.f;
-        const float lse = some ? (m - kLift + log2f(sum)) * kLn2 : -INFINITY;
+        rs.fin[t] = some ? f / sum * (ES == 1 ? 0x1p-8f : 1.f) : 0.f;  // (8-bit P is 2^8 times what the sum adds)
+        const float lse = some ? (m - LIFT + log2f(sum)) * kLn2 : -INFINITY;
         if (!*abort_flag && (!TURNS || grp == 0)) {
           if (!whole) a.part_lse[(int64_t)part * R + c0 + t] = lse;
           else if (rc.orow[c0 + t] >= 0) a.lse[rc.lrow[c0 + t]] = lse;
@@ -985,7 +1015,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               float o = __uint_as_float(x[u]);
-              if constexpr (S::SIDE) o = fmaf(__uint_as_float(y[u]), 0.0625f, o);
+              if constexpr (S::SIDE) o += __uint_as_float(y[u]);
               v[u] = fmaf(o, (g ? r1 : r0).fin[n0 + u], v[u]);
             }
           }
@@ -1140,7 +1170,7 @@ cudaError_t launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedArgs
   if (e != cudaSuccess) return e;
   paged_attn_kernel<D, ES, R><<<pl.ctas, Shape<D, ES, R>::NT, smem, stream>>>(tk, tv, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if (a.cols * a.ps <= kTile) return cudaSuccess;  // one tile per unit: no unit crosses CTAs
+  if ((a.cols << a.ps_log) <= kTile) return cudaSuccess;  // one tile per unit: no unit crosses CTAs
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)pl.ctas, (unsigned)((R + 7) / 8));
   cfg.blockDim = dim3(256);
@@ -1205,7 +1235,7 @@ int fa_paged_attn(const FaPagedAttnParams* p, void* workspace, size_t workspace_
   a.Tq = p->Tq;
   a.G = p->H / c.H_kv;
   a.M = a.G * p->Tq;
-  a.ps = c.page_size;
+  a.ps_log = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : c.page_size == 64 ? 6 : 7;
   a.cols = c.table_cols;
   a.num_pages = c.num_pages;
   a.groups = pl.groups;
