@@ -369,7 +369,8 @@ FA_API int fa_paged_append(const FaPagedAppendParams* p, fa_stream_t stream);
  * do rows that see no key.  Any Tq (a decode step, drafted tokens, a chunk of a prompt).
  * bf16 q and o; mask flags CAUSAL / WINDOW; score flags ALIBI / SOFTCAP.  The cached positions
  * of all sequences are dealt out evenly over the SMs, whatever their lengths; parts of one
- * sequence on several SMs meet in the workspace and are joined by a second kernel.  A page
+ * sequence on several SMs meet in the workspace and are joined after a grid barrier (a
+ * cooperative launch).  A page
  * number out of range hides its positions and sets *status to FA_ERR_INVALID, as does a length
  * beyond table_cols * page_size (which is cut). */
 typedef struct {

@@ -18,21 +18,24 @@
 // (R >= 16), or for R = 8 the parts lie side by side in the MMA's smallest N of 16 and are added
 // when read.  q is scaled by a power of two per row so that its largest magnitude lies in [128, 256):
 // a bf16 has 8 significant bits, each part 4, so the split is exact down to 2^-17 of the row's largest
-// element.  Probabilities lie in [0, 431], the largest of a tile that moved the reference at 128: hi
-// is P cut to 4 bits, lo the rest rounded to 4, off by 2^-8 relative (as a bf16 P is) or by 2^-17 of
+// element.  Probabilities lie in [0, 431], the largest of a tile that moved the reference at 64: hi
+// is P cut to 4 bits, lo the rest rounded to 4, off by 2^-8 relative (as a bf16 P is) or by 2^-16 of
 // the largest below that.
 //
 // Scales.  ks multiplies the thread's logits.  vs goes into the exponent: with z = x + log2 vs and
 // a reference m >= max z - 1.75 per row, P = 2^(z - m + 7) weighs the codes, and the softmax sum
 // adds P / vs; o = sum P code / sum (P / vs).  So a row whose weight sits on pages of small values
 // keeps its precision.  The reference moves only when a tile exceeds it by more than 1.75: one
-// barrier vote per tile.
+// barrier vote per tile.  A unit's tiles are taken from its end to its start: under ALiBi, and mostly
+// without it, the largest logits come first and the references hardly move.
 //
 // Work.  The tiles of all (sequence, row group, K/V head) units, in that order, are cut into equal
 // contiguous ranges, one per CTA (one CTA per SM): ragged batches balance themselves, and nothing
 // about the lengths is needed on the host.  A unit inside one CTA is written to o directly; one
 // that crosses CTAs leaves at most one partial (o, lse) at each end of a CTA's range in the
-// workspace, joined by paged_merge_kernel in CTA order.
+// workspace; after a grid barrier (the launch is cooperative) the CTA that holds a unit's first part
+// joins its parts in CTA order.  A second kernel for that took 5-6 us more on the device and 6 us
+// on the host; counters or flags in the workspace would have to be zero before the call.
 //
 // Warps: softmax groups of four (thread = position of a tile; at the end = element of D), then one
 // that produces (lane = page of a tile), one that issues S, one that issues P V, and one that builds
@@ -40,6 +43,7 @@
 // in turn, each with its own O, references and sums, joined when the unit ends: a tile's chain
 // (wait, TMEM read, vote, exponentials, store, fence) takes longer than its bytes take to arrive, so
 // two tiles have to be in work at once.  With more rows each group takes 16 of them.
+#include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -57,13 +61,14 @@ namespace fa {
 namespace {
 
 constexpr int kTile = 128;         // cached positions of a tile: the MMA's M
-constexpr int kSms = 148;
 constexpr int kMaxSlots = 24;      // K or V tiles in the shared-memory ring
 constexpr int kScaleRing = 16;     // tiles whose scales may be live at once (> kMaxSlots / 2 + 1)
-// A reference moves when exceeded by more than slack (log2 units), and P = 2^(z - reference + lift).
-// 8-bit: P in units of 2^-8, so that fp16's exponents line up with e4m3's (split_e4m3x4); at most
-// 2^(7 + 1.75) = 431, below e4m3's 448.  bf16: any size fits.
-__host__ __device__ constexpr float slack_of(int ES) { return ES == 1 ? 1.75f : 8.f; }
+// A reference moves when exceeded by more than slack (log2 units), to head above the tile's largest z;
+// P = 2^(z - reference + lift).  8-bit: P in units of 2^-8, so that fp16's exponents line up with
+// e4m3's (split_e4m3x4), at most 2^(7 + 1.75) = 431, below e4m3's 448; the head spares most moves
+// (each costs about half a tile's time) for one bit at the small end.  bf16 holds 2^60 as well as 1.
+__host__ __device__ constexpr float slack_of(int ES) { return ES == 1 ? 1.75f : 60.f; }
+__host__ __device__ constexpr float head_of(int ES) { return ES == 1 ? 1.f : 0.f; }
 __host__ __device__ constexpr float lift_of(int ES) { return ES == 1 ? 7.f - 8.f : 0.f; }
 constexpr float kUnset = -1e30f;   // reference of a row that has seen nothing yet
 
@@ -83,7 +88,7 @@ struct PagedArgs {
   FaScoreSpec score;
   float* part_o;    // [2 * CTAs][R][D]
   float* part_lse;  // [2 * CTAs][R]
-  int32_t* part_unit;  // [2 * CTAs]: 2 * unit + (the part is the unit's first), or -1
+  int joins;        // a unit may cross CTAs: the launch is cooperative
   int* status;
 };
 
@@ -177,8 +182,8 @@ __device__ __forceinline__ Entry entry_of(const PagedArgs& a, int e) {
 
 // One CTA's range of tiles, unit by unit.  Every role walks the same sequence by itself.
 struct Seg {
-  int hk, t0, nt;   // K/V head, first tile (absolute), tiles
-  bool first, last; // holds the unit's first / last tile
+  int hk, t0, nt;   // K/V head, first tile taken (they go down from there), tiles
+  bool first, last; // holds the unit's first / last tile in that order
 };
 struct Start {  // where a CTA's range begins
   Entry e;
@@ -211,7 +216,7 @@ struct Walker {
     if (left <= 0) return false;
     settle(a);
     s->hk = hk;
-    s->t0 = e.t0 + off;
+    s->t0 = e.t0 + e.nt - 1 - off;
     s->nt = min(e.nt - off, left);
     s->first = off == 0;
     off += s->nt;
@@ -229,6 +234,9 @@ template <int R> struct Smem {
   uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], fin_bar[2];
   int scan[24];
   Start start;
+  // the unit whose first part this CTA holds: how many parts it has (0: no such unit), the first one's
+  // slot (the others' is 2 k of the CTAs k that follow), its entry and K/V head
+  int join_parts, join_slot, join_entry, join_hk;
   uint32_t tmem;
   int abort_flag, never;
 };
@@ -358,7 +366,8 @@ __device__ __forceinline__ void build_q(const PagedArgs& a, const Entry& e, int 
   constexpr int TPR = D / 8;      // threads per row, 8 elements each
   constexpr int ROWS = NT / TPR;  // rows at once
   constexpr int PASSES = (R + ROWS - 1) / ROWS;
-  constexpr int UN = PASSES < 2 ? 1 : 2;  // rows in flight per thread (unrolling more costs instruction fetches)
+  // rows in flight per thread: a lone warp waits for memory, many warps for instructions
+  constexpr int UN = PASSES < 2 ? 1 : (NT == 32 && PASSES >= 8 ? 8 : 2);
   const int d0 = (t % TPR) * 8;
   const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0;
   const float dom = capped ? 1.f : kLog2e;
@@ -472,7 +481,6 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
   volatile int* never = &sm.never;  // stays 0: waits on it end by time only
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
-  griddep_launch();
 
   // ---------------------------------------------------------------- setup: barriers, TMEM, range
   if (tid == NT - 1) {  // (the first warps have entries to count)
@@ -490,6 +498,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     }
     sm.abort_flag = 0;
     sm.never = 0;
+    sm.join_parts = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
@@ -498,7 +507,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     tmem_alloc(&sm.tmem, S::TM_COLS);
     tmem_relinquish();
   }
-  int my_tiles;
+  int my_tiles, my_start, per;
   {
     // Exclusive prefix of the entries' tiles over the threads, each with a run of entries.
     const int run = (a.entries + NT - 1) / NT, e0 = min(tid * run, a.entries), e1 = min(e0 + run, a.entries);
@@ -527,8 +536,9 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       if (w < warp) before += v;
       total += v;
     }
-    const int per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     const int start = (int)min((int64_t)cta * per, (int64_t)total);
+    my_start = start;
     my_tiles = min(per, total - start);
     int at = before + inc - mine;
     if (start < total && at <= start && start < at + mine) {  // the range begins in one of this thread's entries
@@ -570,7 +580,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       x.hk = 0;
       if (at < my_tiles) {
         wk.settle(a);
-        const int pos = (wk.e.t0 + wk.off) * kTile + (pg << a.ps_log);
+        const int pos = (wk.e.t0 + wk.e.nt - 1 - wk.off) * kTile + (pg << a.ps_log);
         x.hk = wk.hk;
         x.active = pos <= wk.e.hi && pos + (1 << a.ps_log) > wk.e.lo;
         if (x.active) x.page = __ldg(a.table + (int64_t)wk.e.b * a.table_stride + (pos >> a.ps_log));
@@ -750,20 +760,6 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.q_full + buf);
     }
-    // Entries without a tile: their rows see nothing.
-    for (int e = cta; e < a.entries; e += gridDim.x) {
-      const Entry x = entry_of<R>(a, e);
-      if (x.nt) continue;
-      const int m0 = x.rg * R, rows = min(R, a.M - m0);
-      for (int r = 0; r < a.Hkv * rows; ++r) {
-        const int hk = r / rows, m = m0 + r % rows, i = m / a.G, h = hk * a.G + m % a.G;
-        uint16_t* o = reinterpret_cast<uint16_t*>(a.o.ptr) + (int64_t)x.b * a.o.stride_b + (int64_t)h * a.o.stride_h +
-                      (int64_t)i * a.o.stride_t;
-#pragma unroll
-        for (int d = 0; d < D; d += 32) o[d + lane] = 0;
-        if (lane == 0) a.lse[((int64_t)x.b * a.H + h) * a.Tq + i] = -INFINITY;
-      }
-    }
   } else {
     // ---------------------------------------------------------------- softmax (thread = position)
     const int grp = warp >> 2, t = tid & 127, bar = 1 + grp;
@@ -774,11 +770,11 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0, alibi = (a.score.flags & FA_SCORE_ALIBI) != 0;
     const float cap2 = capped ? a.score.softcap * kLog2e : 0.f, cap_k = capped ? 2.f * kLog2e / a.score.softcap : 0.f;
     const int my_page = t >> a.ps_log;
-    constexpr float LIFT = lift_of(ES), SLACK = slack_of(ES);
+    constexpr float LIFT = lift_of(ES), SLACK = slack_of(ES), HEAD = head_of(ES);
     constexpr int PW = 16 / ES;  // rows per 16-byte store of P
     constexpr bool KEEP = NG < 4;
     constexpr int CH = 4;        // rows worked on together; the ones behind the last real row are left out
-    int unit0 = -1, unit1 = -1, j = 0;
+    int j = 0;
     for (int seg = 0; wk.next(a, &sg); ++seg) {
       const RowConst<R>& rc = sm.rc[seg & 1];
       if (seg == 0) {
@@ -806,7 +802,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       const int j0 = j;     // the unit's first tile
       for (int it = 0; it < sg.nt; ++it, ++j) {
         if (TURNS && (j & 1) != grp) continue;
-        const int p0 = (sg.t0 + it) * kTile, pos = p0 + t;
+        const int p0 = (sg.t0 - it) * kTile, pos = p0 + t;
         if (!wait_for(sm.s_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag)) *abort_flag = 1;
         tc_fence_after();
         uint32_t r[16];
@@ -869,7 +865,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           if (t < C) {
             const float old = rs.m[t];
             const float nm = fmaxf(fmaxf(rs.red[0][t], rs.red[1][t]), fmaxf(rs.red[2][t], rs.red[3][t]));
-            const float m = nm > old + SLACK ? nm : old;
+            const float m = nm > old + SLACK ? nm + HEAD : old;
             rs.move[t] = m != old ? ex2_approx(old - m) : 1.f;
             rs.m[t] = m;
             rs.bias[t] = LIFT - m;
@@ -961,8 +957,13 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       else named_bar_sync(bar, 128);
       const bool whole = sg.first && sg.last;
       const int part = 2 * cta + (seg == 0 ? 0 : 1);
-      const int unit = 2 * (wk.idx * a.Hkv + sg.hk) + (sg.first ? 1 : 0);
-      if (!whole) (seg == 0 ? unit0 : unit1) = unit;
+      if (tid == 0 && sg.first && !sg.last) {  // the CTA's last unit, which goes on in the next CTAs
+        const int end = my_start + my_tiles - sg.nt + wk.e.nt;
+        sm.join_parts = (end - 1) / per - cta + 1;
+        sm.join_slot = part;
+        sm.join_entry = wk.idx;
+        sm.join_hk = sg.hk;
+      }
       if (t < C) {
         float m = rs.m[t], sum = (rs.red[0][t] + rs.red[1][t]) + (rs.red[2][t] + rs.red[3][t]), f = 1.f;
         if (TURNS) {  // the other group's partial sums, reference and O
@@ -1035,11 +1036,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       if (TURNS) named_bar_sync(5, NSM);
       else named_bar_sync(bar, 128);
     }
-    if (tid == 0) {
-      a.part_unit[2 * cta] = unit0;
-      a.part_unit[2 * cta + 1] = unit1;
-      if (*abort_flag) report_status(a.status, FA_ERR_TIMEOUT);
-    }
+    if (tid == 0 && *abort_flag) report_status(a.status, FA_ERR_TIMEOUT);
   }
   tc_fence_before();
   __syncthreads();
@@ -1047,68 +1044,88 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     tc_fence_after();
     tmem_dealloc(tmem, S::TM_COLS);
   }
+  // ---------------------------------------------------------------- entries without a tile: rows that see nothing
+  for (int e = cta; e < a.entries; e += gridDim.x) {
+    const Entry x = entry_of<R>(a, e);
+    if (x.nt) continue;
+    const int m0 = x.rg * R, rows = min(R, a.M - m0);
+    for (int r = warp; r < a.Hkv * rows; r += NT / 32) {
+      const int hk = r / rows, m = m0 + r - hk * rows, i = m / a.G, h = hk * a.G + m - i * a.G;
+      uint16_t* o = reinterpret_cast<uint16_t*>(a.o.ptr) + (int64_t)x.b * a.o.stride_b + (int64_t)h * a.o.stride_h +
+                    (int64_t)i * a.o.stride_t;
+#pragma unroll
+      for (int d = 0; d < D; d += 32) o[d + lane] = 0;
+      if (lane == 0) a.lse[((int64_t)x.b * a.H + h) * a.Tq + i] = -INFINITY;
+    }
+  }
+  if (!a.joins) return;
+  // ---------------------------------------------------------------- units that cross CTAs
+  const auto grid = cooperative_groups::this_grid();
+  auto arrived = grid.barrier_arrive();
+  const int parts = sm.join_parts;
+  if (!parts || *abort_flag) return;
+  const int hk = sm.join_hk, slot0 = sm.join_slot, en = sm.join_entry, b = a.groups == 1 ? en : en / a.groups,
+            m0 = (en - b * a.groups) * R;
+  grid.barrier_wait(static_cast<decltype(arrived)&&>(arrived));
+  // One warp per query row, 32 parts at a time: lane k weighs part k, then every lane sums its
+  // elements of D over the parts, rescaled when a later batch has a larger lse.
+  for (int n = warp; n < R && m0 + n < a.M; n += NT / 32) {
+    float acc[D / 32], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+    float po[8][D / 32];
+    auto fetch = [&](int k, int many) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int v = 0; v < D / 32; ++v)
+          po[i][v] = i < many
+                         ? __ldcg(a.part_o + ((int64_t)(k + i == 0 ? slot0 : 2 * (cta + k + i)) * R + n) * D + lane + 32 * v)
+                         : 0.f;
+    };
+#pragma unroll 1
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      const int k = k0 + lane, run = min(32, parts - k0);
+      fetch(k0, min(8, run));  // together with the lse
+      const float ls = lane < run ? __ldcg(a.part_lse + (int64_t)(k == 0 ? slot0 : 2 * (cta + k)) * R + n) : -INFINITY;
+      const float nt = fmaxf(top, warp_max(ls)), ref = nt == -INFINITY ? 0.f : nt;
+      const float w = lane < run ? expf(ls - ref) : 0.f;
+      float ws = w;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+      const float back = top == -INFINITY ? 0.f : expf(top - ref);
+      sum = sum * back + ws;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] *= back;
+      top = nt;
+#pragma unroll 1
+      for (int i0 = 0; i0 < run; i0 += 8) {
+        if (i0 > 0) fetch(k0 + i0, min(8, run - i0));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float wi = __shfl_sync(0xffffffffu, w, i0 + i);  // (0 behind the last part)
+#pragma unroll
+          for (int v = 0; v < D / 32; ++v) acc[v] = fmaf(wi, po[i][v], acc[v]);
+        }
+      }
+    }
+    const int m = m0 + n, i = m / a.G, h = hk * a.G + m - i * a.G;
+    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.o.ptr) + (int64_t)b * a.o.stride_b +
+                       (int64_t)h * a.o.stride_h + (int64_t)i * a.o.stride_t;
+    const bool some = !(sum == 0.f);
+    const float inv = some ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) o[lane + 32 * k] = __float2bfloat16_rn(acc[k] * inv);
+    if (lane == 0) a.lse[((int64_t)b * a.H + h) * a.Tq + i] = some ? (top == -INFINITY ? 0.f : top) + logf(sum) : -INFINITY;
+  }
 }
 
-// Joins the parts of the unit that begins in CTA blockIdx.x and runs on into the next ones, in CTA
-// order: one warp per query row.  Launched with programmatic serialisation, so that its blocks are
-// resident when the last CTA of the attention kernel ends.
-template <int D, int R>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a, const int ctas) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, n = blockIdx.y * 8 + warp;
-  griddep_wait();
-  const int u0 = a.part_unit[2 * c], u1 = a.part_unit[2 * c + 1];
-  int first, key;
-  if (u1 >= 0) {
-    first = 2 * c + 1;
-    key = u1 >> 1;
-  } else if (u0 >= 0 && (u0 & 1)) {
-    first = 2 * c;
-    key = u0 >> 1;
-  } else {
-    return;
-  }
-  const int e = key / a.Hkv, hk = key % a.Hkv, b = e / a.groups, m = (e % a.groups) * R + n;
-  if (n >= R || m >= a.M) return;
-  // The unit's parts: `first`, then slot 2 k of the CTAs k that follow as long as it is this unit's.
-  // 32 parts at a time: lane k weighs part k, then every lane sums its elements of D over the parts,
-  // rescaled when a later batch has a larger lse.
-  float acc[D / 32], top = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  for (int k0 = 0;; k0 += 32) {
-    const int k = k0 + lane;  // part; CTA c + k
-    const bool same = k == 0 || (c + k < ctas && a.part_unit[2 * (c + k)] == 2 * key);
-    const unsigned m32 = __ballot_sync(0xffffffffu, same);
-    const int run = m32 == 0xffffffffu ? 32 : __ffs(~m32) - 1;
-    if (run == 0) break;
-    const float ls = lane < run ? a.part_lse[(int64_t)(k == 0 ? first : 2 * (c + k)) * R + n] : -INFINITY;
-    const float nt = fmaxf(top, warp_max(ls)), ref = nt == -INFINITY ? 0.f : nt;
-    const float w = lane < run ? expf(ls - ref) : 0.f;
-    float ws = w;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
-    const float back = top == -INFINITY ? 0.f : expf(top - ref);
-    sum = sum * back + ws;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] *= back;
-    top = nt;
-#pragma unroll 4
-    for (int i = 0; i < run; ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      const float* po = a.part_o + ((int64_t)(k0 + i == 0 ? first : 2 * (c + k0 + i)) * R + n) * D + lane;
-#pragma unroll
-      for (int v = 0; v < D / 32; ++v) acc[v] = fmaf(wi, po[32 * v], acc[v]);
-    }
-    if (run < 32) break;
-  }
-  const int i = m / a.G, h = hk * a.G + m % a.G;
-  __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.o.ptr) + (int64_t)b * a.o.stride_b +
-                     (int64_t)h * a.o.stride_h + (int64_t)i * a.o.stride_t;
-  const bool some = !(sum == 0.f);
-  const float inv = some ? 1.f / sum : 0.f;
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) o[lane + 32 * k] = __float2bfloat16_rn(acc[k] * inv);
-  if (lane == 0) a.lse[((int64_t)b * a.H + h) * a.Tq + i] = some ? (top == -INFINITY ? 0.f : top) + logf(sum) : -INFINITY;
+// SMs of the current device, each of which takes one CTA (148 where there is no device to ask).
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    n = 0;
+  return n > 0 ? n : 148;
 }
 
 struct PagedPlan {
@@ -1129,8 +1146,8 @@ PagedPlan plan_paged(const FaPagedAttnParams* p) {
   pl.groups = (int)((M + pl.R - 1) / pl.R);
   const int64_t tiles = (int64_t)p->B * pl.groups * p->cache.H_kv *
                         (((int64_t)p->cache.table_cols * p->cache.page_size + kTile - 1) / kTile);
-  pl.ctas = (int)std::min<int64_t>(kSms, tiles);
-  pl.workspace = (size_t)2 * pl.ctas * ((size_t)pl.R * (p->cache.D + 1) * 4 + 4) + 256;
+  pl.ctas = (int)std::min<int64_t>(sm_count(), tiles);
+  pl.workspace = (size_t)2 * pl.ctas * pl.R * (p->cache.D + 1) * 4 + 256;
   return pl;
 }
 
@@ -1162,25 +1179,24 @@ int check_paged(const FaPagedAttnParams* p) {
 template <int D, int ES, int R>
 cudaError_t launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedArgs& a, const PagedPlan& pl,
                          cudaStream_t stream) {
-  const size_t fixed = paged_smem_bytes<D, ES, R>(0), limit = 232448 - 2048;  // room for a block of the merge kernel
+  const size_t fixed = paged_smem_bytes<D, ES, R>(0), limit = 232448;
   a.slots = (int)std::min<size_t>(kMaxSlots, (limit - fixed) / Shape<D, ES, R>::SLOT);
   const size_t smem = paged_smem_bytes<D, ES, R>(a.slots);
   cudaError_t e =
       cudaFuncSetAttribute(paged_attn_kernel<D, ES, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  paged_attn_kernel<D, ES, R><<<pl.ctas, Shape<D, ES, R>::NT, smem, stream>>>(tk, tv, a);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if ((a.cols << a.ps_log) <= kTile) return cudaSuccess;  // one tile per unit: no unit crosses CTAs
+  a.joins = (a.cols << a.ps_log) > kTile && pl.ctas > 1;  // (a unit of one tile lies in one CTA)
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)pl.ctas, (unsigned)((R + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)pl.ctas);
+  cfg.blockDim = dim3(Shape<D, ES, R>::NT);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
+  at.id = cudaLaunchAttributeCooperative;
+  at.val.cooperative = a.joins;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, R>, (const PagedArgs)a, (int)pl.ctas);
+  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<D, ES, R>, tk, tv, (const PagedArgs)a);
 }
 
 template <int D>
@@ -1259,7 +1275,6 @@ int fa_paged_attn(const FaPagedAttnParams* p, void* workspace, size_t workspace_
   a.score = p->score;
   a.part_o = reinterpret_cast<float*>(workspace);
   a.part_lse = a.part_o + (size_t)2 * pl.ctas * pl.R * c.D;
-  a.part_unit = reinterpret_cast<int32_t*>(a.part_lse + (size_t)2 * pl.ctas * pl.R);
   a.status = p->status;
   const bool f8 = c.dtype == FA_DTYPE_E4M3;
   const cudaStream_t st = (cudaStream_t)stream;

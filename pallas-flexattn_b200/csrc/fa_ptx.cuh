@@ -345,12 +345,6 @@ __device__ __forceinline__ void reg_pin(uint32_t (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-// ---------------------------------------------------------------- dependent launches
-// Lets a kernel launched with programmatic stream serialisation start; what it reads of this
-// grid it reads after griddep_wait, which returns when this grid has completed.
-__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // ---------------------------------------------------------------- register rebalancing
 // Executed by every warp of a warpgroup.  The host checks before launch that the
 // per-warpgroup targets sum to no more than the block's launch allocation.

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 FA_OK, FA_ERR_INVALID, FA_ERR_UNSUPPORTED, FA_ERR_CUDA, FA_ERR_TIMEOUT = 0, 1, 2, 3, 4
@@ -325,6 +326,45 @@ def lib() -> C.CDLL:
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+def _layout(cls, base=0):
+    """(offset, format character) of every scalar of a structure, nested ones flattened."""
+    out = []
+    for name, t in cls._fields_:
+        at = base + getattr(cls, name).offset
+        if issubclass(t, C.Structure):
+            out += _layout(t, at)
+        else:
+            out.append((at, {C.c_int32: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "Q"}[t]))
+    return out
+
+
+def packer(cls) -> struct.Struct:
+    """A struct.Struct that packs the scalars of `cls` in order, nested structures flattened: one call
+    instead of one attribute assignment per field (a parameter block has 40 to 60)."""
+    fmt, at = "=", 0
+    for off, ch in _layout(cls):
+        fmt += "x" * (off - at) + ch
+        at = off + struct.calcsize("=" + ch)
+    return struct.Struct(fmt + "x" * (C.sizeof(cls) - at))
+
+
+_packed = {}
+
+
+def packed_call(name: str, *args) -> None:
+    """Call an entry point whose first argument is a packed parameter block (bytes) and whose further
+    ones are pointers or sizes; raises like `check`."""
+    fn = _packed.get(name)
+    if fn is None:
+        fn = lib()[name]  # a function object of its own, with its own argument types
+        fn.restype = C.c_int
+        fn.argtypes = [C.c_char_p] + [C.c_void_p if t is C.c_void_p else t for t in EXPORTS[name][1][1:]]
+        _packed[name] = fn
+    rc = fn(*args)
+    if rc != FA_OK:
+        check(rc)
 
 
 def check(rc: int) -> None:

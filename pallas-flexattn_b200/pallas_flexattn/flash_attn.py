@@ -63,10 +63,23 @@ def device_status(device) -> torch.Tensor:
     """Per-device int32 that kernels set: FA_ERR_TIMEOUT when a bounded device-side wait gives up,
     FA_ERR_INVALID when a length or page number on the device is out of range."""
     device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     k = str(device)
     if k not in _STATUS:
         _STATUS[k] = torch.zeros(1, dtype=torch.int32, device=device)
     return _STATUS[k]
+
+
+_STATUS_PTR: dict = {}
+
+
+def status_ptr(index: int) -> int:
+    """Address of device_status of CUDA device `index`."""
+    p = _STATUS_PTR.get(index)
+    if p is None:
+        p = _STATUS_PTR[index] = device_status(torch.device("cuda", index)).data_ptr()
+    return p
 
 
 def check_device_status(device=None) -> None:
@@ -100,6 +113,26 @@ def _tables_for(spec: MaskSpec, B: int, Tq: int, Tkv: int, bq: int, bkv: int, de
         return bt
     _TABLE_CACHE.move_to_end(key)
     return hit[1]
+
+
+class on_device:
+    """``with on_device(dev) as stream``: `dev` is the current CUDA device inside, `stream` its current
+    stream's handle.  (torch.cuda.device and current_stream cost 3 us between them, this 0.5.)"""
+
+    __slots__ = ("index", "back")
+
+    def __init__(self, dev: torch.device):
+        self.index = dev.index
+
+    def __enter__(self) -> int:
+        self.back = torch._C._cuda_getDevice()
+        if self.back != self.index:
+            torch._C._cuda_setDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.back != self.index:
+            torch._C._cuda_setDevice(self.back)
 
 
 _DTYPES = {torch.bfloat16: L.FA_DTYPE_BF16, torch.float32: L.FA_DTYPE_F32}

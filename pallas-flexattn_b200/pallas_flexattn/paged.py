@@ -27,7 +27,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib as L
-from .flash_attn import _DTYPES, _fa_tensor, _last_contig, device_status
+from .flash_attn import _DTYPES, on_device, status_ptr
 from .mask_mod import MaskMod
 from .mask_mod import spec_of as mask_spec_of
 from .rotary import RotarySpec
@@ -73,7 +73,11 @@ class PagedKVCache:
                     raise ValueError(f"an 8-bit cache needs contiguous fp32 k_scale and v_scale of shape ({n}, {hkv})")
         elif k_scale is not None or v_scale is not None:
             raise ValueError("scales belong to an 8-bit cache")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
+        self._fields = (_CACHE_DTYPES[k.dtype], n, hkv, ps, d, k.data_ptr(), *k.stride()[:3], v.data_ptr(),
+                        *v.stride()[:3], *((k_scale.data_ptr(), v_scale.data_ptr()) if k_scale is not None else (0, 0)))
+        self._shape, self._device = (n, hkv, ps, d), k.device
+        self._ws: dict = {}  # workspace bytes by the shape of a call
 
     @classmethod
     def empty(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,
@@ -85,9 +89,11 @@ class PagedKVCache:
             pools += [torch.ones(shape[:2], dtype=torch.float32, device=device) for _ in range(2)]
         return cls(*pools)
 
-    @property
-    def page_size(self) -> int:
-        return self.k.shape[2]
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scale = property(lambda self: self._k_scale)
+    v_scale = property(lambda self: self._v_scale)
+    page_size = property(lambda self: self._shape[2])
 
     def gather(self, pages: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """Keys and values of a row of a block table as fp32 (H_kv, positions, D): for looking at a
@@ -100,20 +106,28 @@ class PagedKVCache:
             out.append(x.transpose(0, 1).flatten(1, 2))
         return tuple(out)
 
-    def _to_c(self, table: torch.Tensor) -> L.FaPagedCache:
-        c = L.FaPagedCache()
-        c.dtype = _CACHE_DTYPES[self.k.dtype]
-        c.num_pages, c.H_kv, c.page_size, c.D = self.k.shape
-        c.k, c.v = _fa_tensor(self.k), _fa_tensor(self.v)
-        if self.k_scale is not None:
-            c.k_scale, c.v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
-        c.block_table = table.data_ptr()
-        c.table_cols, c.table_stride = table.shape[1], table.stride(0)
-        return c
+    def _packed(self, table: torch.Tensor) -> tuple:
+        """The fields of an FaPagedCache."""
+        return (*self._fields, table.data_ptr(), table.shape[1], table.stride(0))
+
+
+_PACK_APPEND, _PACK_ATTN = L.packer(L.FaPagedAppendParams), L.packer(L.FaPagedAttnParams)
+_NONE = (0, 0, 0, 0)
+_NO_MASK_TABLES = (0,) * 13  # doc_q .. bit_cols of an FaMaskSpec
+
+
+def _fields(t: torch.Tensor) -> tuple:
+    """The fields of an FaTensor."""
+    st = t.stride()
+    return t.data_ptr(), st[0], st[1], st[2]
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(3) == 1 else t.contiguous()
 
 
 def _lengths(name: str, x: Lengths, B: int, dev: torch.device) -> torch.Tensor:
-    if not (isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.device == dev and x.is_contiguous()):
+    if not (isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.device == dev and x.is_contiguous()):
         x = torch.as_tensor(x)
         if x.is_floating_point() or x.dtype == torch.bool:
             raise ValueError(f"{name} must be integers")
@@ -126,9 +140,9 @@ def _lengths(name: str, x: Lengths, B: int, dev: torch.device) -> torch.Tensor:
 def _table(t: torch.Tensor, B: int, dev: torch.device) -> torch.Tensor:
     if t.dim() != 2 or t.shape[0] != B or t.shape[1] == 0:
         raise ValueError(f"block_table must be ({B}, columns), got {tuple(t.shape)}")
-    if t.is_floating_point() or t.dtype == torch.bool:
+    if t.dtype is not torch.int32 and (t.is_floating_point() or t.dtype == torch.bool):
         raise ValueError("block_table must be integers")
-    if t.dtype != torch.int32 or t.device != dev or t.stride(1) != 1:
+    if t.dtype is not torch.int32 or t.device != dev or t.stride(1) != 1:
         t = t.to(device=dev, dtype=torch.int32).contiguous()
     return t
 
@@ -152,41 +166,37 @@ def paged_kv_append(cache: PagedKVCache, block_table: torch.Tensor, kv_lens: Len
     if k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"k and v must be (B, H_kv, T, D), got {tuple(k.shape)} and {tuple(v.shape)}")
     B, hkv, T, D = k.shape
-    if (hkv, D) != (cache.k.shape[1], cache.k.shape[3]):
-        raise ValueError(f"k{tuple(k.shape)} does not fit pages {tuple(cache.k.shape)}")
-    dev = cache.k.device
-    if any(t.device != dev for t in (k, v)) or (q is not None and q.device != dev):
+    if (hkv, D) != cache._shape[1::2]:
+        raise ValueError(f"k{tuple(k.shape)} does not fit pages {cache._shape}")
+    dev = cache._device
+    if k.device != dev or v.device != dev or (q is not None and q.device != dev):
         raise ValueError("k, v, q and the cache must be on one CUDA device")
-    if k.dtype not in _DTYPES or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    dtype = k.dtype
+    if dtype not in _DTYPES or v.dtype != dtype or (q is not None and q.dtype != dtype):
         raise ValueError("q, k, v must share dtype bf16 or fp32")
     if q is not None and (q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, T, D)):
         raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)}")
     if rotary is not None and rotary.head_dim != D:
         raise ValueError(f"head dim {D}, but the rotary_spec is for {rotary.head_dim}")
-    if any(t is not None and t.requires_grad for t in (q, k, v)) and torch.is_grad_enabled():
+    if (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)) and torch.is_grad_enabled():
         raise ValueError("paged_kv_append has no gradient: call it under torch.no_grad()")
-    out = None
+    out, heads, fq, fo = None, 0, _NONE, _NONE
     if q is not None:
-        q = _last_contig(q)
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty(q.shape, dtype=dtype, device=dev)
     if B == 0 or T == 0:
         return out
-    k, v = _last_contig(k), _last_contig(v)
+    if q is not None and q.shape[1]:
+        q = _rows(q)
+        heads, fq, fo = q.shape[1], _fields(q), _fields(out)
+    k, v = _rows(k), _rows(v)
     table, lens = _table(block_table, B, dev), _lengths("kv_lens", kv_lens, B, dev)
     new = None if new_lens is None else _lengths("new_lens", new_lens, B, dev)
-    p = L.FaPagedAppendParams()
-    p.dtype, p.B, p.T = _DTYPES[k.dtype], B, T
-    p.k, p.v = _fa_tensor(k), _fa_tensor(v)
-    if q is not None and q.shape[1]:
-        p.H, p.q, p.q_out = q.shape[1], _fa_tensor(q), _fa_tensor(out)
-    p.kv_lens = lens.data_ptr()
-    p.new_lens = None if new is None else new.data_ptr()
-    if rotary is not None:
-        p.rotary = rotary.to_c(dev)
-    p.cache = cache._to_c(table)
-    p.status = device_status(dev).data_ptr()
-    with torch.cuda.device(dev):
-        L.check(L.lib().fa_paged_append(C.byref(p), torch.cuda.current_stream(dev).cuda_stream))
+    block = _PACK_APPEND.pack(_DTYPES[dtype], B, heads, T, *fq, *_fields(k), *_fields(v), *fo, lens.data_ptr(),
+                              0 if new is None else new.data_ptr(),
+                              *(rotary.packed(dev) if rotary is not None else (0, 0, 0, 1.0)), *cache._packed(table),
+                              status_ptr(dev.index))
+    with on_device(dev) as stream:
+        L.packed_call("fa_paged_append", block, stream)
     return out
 
 
@@ -210,15 +220,15 @@ def flash_attention_paged(q: torch.Tensor, cache: PagedKVCache, block_table: tor
     """
     if q.dim() != 4:
         raise ValueError("q must be (B, H, Tq, D)")
-    dev = cache.k.device
+    dev = cache._device
     if q.device != dev:
         raise ValueError("q and the cache must be on one CUDA device")
     if q.dtype != torch.bfloat16:
         raise ValueError(f"q must be bf16, got {q.dtype}")
     B, H, Tq, D = q.shape
-    hkv = cache.k.shape[1]
-    if D != cache.k.shape[3]:
-        raise ValueError(f"q{tuple(q.shape)} does not fit pages {tuple(cache.k.shape)}")
+    hkv = cache._shape[1]
+    if D != cache._shape[3]:
+        raise ValueError(f"q{tuple(q.shape)} does not fit pages {cache._shape}")
     if H == 0 or H % hkv:
         raise ValueError(f"H={H} must be a multiple of the K/V heads {hkv}")
     if q.requires_grad and torch.is_grad_enabled():
@@ -229,28 +239,32 @@ def flash_attention_paged(q: torch.Tensor, cache: PagedKVCache, block_table: tor
     sspec = score_spec_of(score_mod)
     if sspec is None or sspec.flags & ~(L.FA_SCORE_ALIBI | L.FA_SCORE_SOFTCAP):
         raise NotImplementedError("paged attention takes alibi_score_mod, softcap_score_mod or their composition")
-    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    o = torch.empty((B, H, Tq, D), dtype=torch.bfloat16, device=dev)
     lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
     if B == 0 or Tq == 0:
         return o, lse
-    q = _last_contig(q)
+    q = _rows(q)
     table, lens = _table(block_table, B, dev), _lengths("kv_lens", kv_lens, B, dev)
     qlen = None if q_lens is None else _lengths("q_lens", q_lens, B, dev)
-    p = L.FaPagedAttnParams()
-    p.B, p.H, p.Tq = B, H, Tq
-    p.q, p.o = _fa_tensor(q), _fa_tensor(o)
-    p.lse = lse.data_ptr()
-    p.kv_lens = lens.data_ptr()
-    p.q_lens = None if qlen is None else qlen.data_ptr()
-    p.scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    p.mask = mspec.to_c(dev, Tq, Tq)
-    p.score = sspec.to_c(dev, H, Tq, Tq)
-    p.cache = cache._to_c(table)
-    p.status = device_status(dev).data_ptr()
-    lib = L.lib()
-    size = C.c_size_t(0)
-    with torch.cuda.device(dev):
-        L.check(lib.fa_paged_attn_workspace_size(C.byref(p), C.byref(size)))
-        ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
-        L.check(lib.fa_paged_attn(C.byref(p), ws.data_ptr(), size.value, torch.cuda.current_stream(dev).cuda_stream))
+    slopes = 0
+    if sspec.flags & L.FA_SCORE_ALIBI:
+        t = sspec.device_tensors(dev)["slopes"]
+        if t.numel() != H:
+            raise ValueError(f"ALiBi has {t.numel()} slopes for {H} heads")
+        slopes = t.data_ptr()
+    block = _PACK_ATTN.pack(B, H, Tq, *_fields(q), *_fields(o), lse.data_ptr(), lens.data_ptr(),
+                            0 if qlen is None else qlen.data_ptr(), scale if scale is not None else 1.0 / math.sqrt(D),
+                            mspec.flags, mspec.window_left, mspec.window_right, *_NO_MASK_TABLES,
+                            sspec.flags, sspec.softcap, slopes, 0, 0, 0, *cache._packed(table), status_ptr(dev.index))
+    with on_device(dev) as stream:
+        key = (B, H, Tq, table.shape[1])
+        size = cache._ws.get(key)
+        if size is None:
+            n = C.c_size_t(0)
+            L.packed_call("fa_paged_attn_workspace_size", block, C.byref(n))
+            if len(cache._ws) >= 256:
+                cache._ws.clear()
+            size = cache._ws[key] = n.value
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        L.packed_call("fa_paged_attn", block, ws.data_ptr(), size, stream)
     return o, lse

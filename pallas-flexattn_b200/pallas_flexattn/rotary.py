@@ -17,7 +17,6 @@ dimension (rows that 16-byte accesses do not fit take a slower kernel).  There i
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 from dataclasses import dataclass, field
 from fractions import Fraction
@@ -26,7 +25,7 @@ from typing import Callable, List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib as L
-from .flash_attn import _DTYPES, _fa_tensor, _last_contig
+from .flash_attn import _DTYPES, on_device
 
 _PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
 
@@ -92,18 +91,19 @@ class RotarySpec:
 
     def turns(self, device: torch.device) -> torch.Tensor:
         """Fractions of a turn per position, in units of 2^-64 turns, on `device` (cached)."""
-        key = (device.type, device.index)
-        t = self._dev.get(key)
+        t = self._dev.get(device)
         if t is None:
-            bits = [round(Fraction(f) / (2 * _PI) * (1 << 64)) % (1 << 64) for f in self.frequencies]
-            t = torch.tensor([b - (1 << 64) if b >> 63 else b for b in bits], dtype=torch.int64).to(device)
-            self._dev[key] = t
+            t = self._dev[device] = self._dev["host"].to(device)
         return t
 
-    def to_c(self, device: torch.device, inverse: bool = False) -> L.FaRotarySpec:
-        layout = L.FA_ROTARY_INTERLEAVED if self.interleaved else L.FA_ROTARY_HALF
-        turns = self.turns(device).data_ptr() if self.rotary_dim else None
-        return L.FaRotarySpec(self.rotary_dim, layout, turns, self.magnitude)
+    def __post_init__(self):
+        bits = [round(Fraction(f) / (2 * _PI) * (1 << 64)) % (1 << 64) for f in self.frequencies]
+        self._dev["host"] = torch.tensor([b - (1 << 64) if b >> 63 else b for b in bits], dtype=torch.int64)
+
+    def packed(self, device: torch.device) -> tuple:
+        """The fields of an FaRotarySpec on `device`."""
+        return (self.rotary_dim, int(self.interleaved), self.turns(device).data_ptr() if self.rotary_dim else 0,
+                self.magnitude)
 
 
 def rotary_spec(head_dim: int, *, rotary_dim: Optional[int] = None, base: float = 10000.0, interleaved: bool = False,
@@ -141,10 +141,17 @@ def _check_qk(q, k, spec):
         raise ValueError("rotary_embedding runs on CUDA tensors of one device only (there is no CPU path)")
     if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
         raise ValueError("q, k must share dtype bf16 or fp32")
-    if k is not None and (k.shape[0], k.shape[2], k.shape[3]) != (q.shape[0], q.shape[2], q.shape[3]):
-        raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)}")
-    if q.shape[3] != spec.head_dim:
-        raise ValueError(f"head dim {q.shape[3]}, but the rotary_spec is for {spec.head_dim}")
+    B, _, T, D = q.shape
+    if k is not None:
+        Bk, _, Tk, Dk = k.shape
+        if Bk != B or Tk != T or Dk != D:
+            raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)}")
+    if D != spec.head_dim:
+        raise ValueError(f"head dim {D}, but the rotary_spec is for {spec.head_dim}")
+
+
+_PACK = L.packer(L.FaRotaryParams)
+_NONE = (0, 0, 0, 0)
 
 
 def _launch(q, k, spec: RotarySpec, positions: Positions, inverse: bool):
@@ -152,34 +159,36 @@ def _launch(q, k, spec: RotarySpec, positions: Positions, inverse: bool):
     x = q if q is not None else k
     B, _, T, D = x.shape
     dev = x.device
-    p = L.FaRotaryParams()
-    p.dtype, p.B, p.T, p.D = _DTYPES[x.dtype], B, T, D
-    out = []
-    keep = []
-    for name, t in (("q", q), ("k", k)):
+    heads, tensors, out, keep = [], [], [], []
+    for t in (q, k):
         if t is None or t.numel() == 0:
             out.append(t if t is None else torch.empty_like(t))
+            heads.append(0)
+            tensors += (_NONE, _NONE)
             continue
-        t = _last_contig(t)
+        if t.stride(3) != 1:
+            t = t.contiguous()
         o = torch.empty_like(t)
-        if o.stride(-1) != 1:  # an overlapping or broadcast input
+        st = o.stride()
+        if st[3] != 1:  # an overlapping or broadcast input
             o = torch.empty(t.shape, dtype=t.dtype, device=dev)
-        setattr(p, name, _fa_tensor(t))
-        setattr(p, name + "_out", _fa_tensor(o))
-        setattr(p, "H" if name == "q" else "H_kv", t.shape[1])
+            st = o.stride()
+        heads.append(t.shape[1])
+        tensors += ((t.data_ptr(), *t.stride()[:3]), (o.data_ptr(), *st[:3]))
         out.append(o)
         keep.append(t)
     if not keep:
         return tuple(out)
+    pos, pos_stride, offset = 0, 0, 0
     if isinstance(positions, torch.Tensor):
-        p.positions = positions.data_ptr()
-        p.pos_stride_b = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
-    else:
-        p.pos_offset = positions or 0
-    p.inverse = int(inverse)
-    p.rotary = spec.to_c(dev)
-    with torch.cuda.device(dev):
-        L.check(L.lib().fa_rotary(C.byref(p), torch.cuda.current_stream(dev).cuda_stream))
+        pos = positions.data_ptr()
+        pos_stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
+    elif positions:
+        offset = positions
+    block = _PACK.pack(_DTYPES[x.dtype], B, *heads, T, D, *tensors[0], *tensors[2], *tensors[1], *tensors[3], pos,
+                       pos_stride, offset, inverse, *spec.packed(dev))
+    with on_device(dev) as stream:
+        L.packed_call("fa_rotary", block, stream)
     return tuple(out)
 
 
@@ -196,7 +205,8 @@ class _Rotary(torch.autograd.Function):
         if dq is None and dk is None:
             return None, None, None, None, None
         # linear, so its own gradient is the same operator turned back
-        gq, gk = _Rotary.apply(dq, dk, spec, positions, not inverse)
+        turn = _Rotary.apply if torch.is_grad_enabled() else _launch
+        gq, gk = turn(dq, dk, spec, positions, not inverse)
         return gq, gk, None, None, None
 
 

@@ -147,7 +147,7 @@ def test_workspace_does_not_grow_with_lengths():
         p.cache.table_cols = cols
         assert L.lib().fa_paged_attn_workspace_size(C.byref(p), C.byref(size)) == 0
         got.append(size.value)
-    assert got[0] == got[1] == got[2] == 2 * 148 * (8 * 129 * 4 + 4) + 256
+    assert got[0] == got[1] == got[2] == 2 * 148 * 8 * 129 * 4 + 256
 
 
 def test_rotary_spec_turns_are_exact():
