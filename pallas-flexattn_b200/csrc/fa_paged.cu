@@ -123,7 +123,8 @@ template <int R> struct RowConst {
   float slope[R];   // ALiBi slope in the same domain
   int lo[R], hi[R]; // positions the row may see; hi < lo: none
   int qpos[R];
-  int64_t orow[R];  // element offset of the row in o, -1: no such row
+  int64_t qoff[R];  // element offset of the row in q, -1: nothing to read
+  int64_t orow[R];  // the same in o, -1: no such row
   int64_t lrow[R];  // index of the row in lse
 };
 // Running state of one softmax group: its rows, or its share of the tiles.
@@ -237,6 +238,7 @@ template <int R> struct Smem {
   // the unit whose first part this CTA holds: how many parts it has (0: no such unit), the first one's
   // slot (the others' is 2 k of the CTAs k that follow), its entry and K/V head
   int join_parts, join_slot, join_entry, join_hk;
+  int empties, empty_entry[64];  // entries without a tile of which this CTA writes heads cta - entry, + CTAs, ...
   uint32_t tmem;
   int abort_flag, never;
 };
@@ -337,54 +339,53 @@ __device__ __forceinline__ float warp_col_sums(float (&v)[C], int lane) {
   return r;
 }
 
-// Rows from n0 on of a Q operand: zeros that see nothing.
-template <int D, int ES, int R, int NT>
-__device__ __forceinline__ void zero_rows(unsigned char* q, RowConst<R>& rc, int n0, int t) {
-  using S = Shape<D, ES, R>;
-  constexpr int CH = S::SW / 16;  // 16-byte chunks of a row in a panel
-#pragma unroll 1
-  for (int k = t; k < (R - n0) * (S::ROWB / 16) * (ES == 1 ? 2 : 1); k += NT) {
-    const int part = k / ((R - n0) * (S::ROWB / 16)), in = k % ((R - n0) * (S::ROWB / 16));
-    const int n = n0 + in / (S::ROWB / 16), c = in % (S::ROWB / 16);
-    *reinterpret_cast<uint4*>(q + part * (S::SIDE ? R * S::SW : S::QPART) + (c / CH) * S::QPANEL + n * S::SW + (c % CH) * 16) =
-        make_uint4(0u, 0u, 0u, 0u);
-  }
-  for (int n = n0 + t; n < R; n += NT) {
-    rc.xs[n] = rc.slope[n] = 0.f;
-    rc.lo[n] = 1;
-    rc.hi[n] = rc.qpos[n] = 0;
-    rc.orow[n] = -1;
+// Row constants of a unit's row group and K/V head but for xs, and where its rows of q are (in qoff):
+// one thread a row.
+template <int R>
+__device__ __forceinline__ void build_rows(const PagedArgs& a, const Entry& e, int hk, RowConst<R>& rc, int t, int nt) {
+  const float dom = (a.score.flags & FA_SCORE_SOFTCAP) ? 1.f : kLog2e;
+  for (int n = t; n < R; n += nt) {
+    const int m = e.rg * R + n, i = m / a.G, h = hk * a.G + (m - i * a.G);
+    const bool real = m < a.M, live = real && i < e.ql;
+    const int qpos = e.len - e.ql + i;
+    int lo = 0, hi = e.len - 1;
+    if (a.mask.flags & FA_MASK_CAUSAL) hi = min(hi, qpos);
+    if (a.mask.flags & FA_MASK_WINDOW) {
+      if (a.mask.window_left >= 0) lo = max(lo, qpos - a.mask.window_left);
+      if (a.mask.window_right >= 0) hi = (int)min((int64_t)hi, (int64_t)qpos + a.mask.window_right);
+    }
+    rc.slope[n] = live && (a.score.flags & FA_SCORE_ALIBI) ? __ldg(a.score.alibi_slopes + h) * dom : 0.f;
+    rc.lo[n] = live ? lo : 1;
+    rc.hi[n] = live ? hi : 0;
+    rc.qpos[n] = qpos;
+    rc.qoff[n] = live ? (int64_t)e.b * a.q.stride_b + (int64_t)h * a.q.stride_h + (int64_t)i * a.q.stride_t : -1;
+    rc.orow[n] = real ? (int64_t)e.b * a.o.stride_b + (int64_t)h * a.o.stride_h + (int64_t)i * a.o.stride_t : -1;
+    rc.lrow[n] = ((int64_t)e.b * a.H + h) * a.Tq + i;
   }
 }
 
-// The Q operand and the row constants of a unit's row group and K/V head, by NT threads.
+// The Q operand of the rows that build_rows described, and their xs, by NT threads; rows that do not
+// exist become zeros.
 template <int D, int ES, int R, int NT>
-__device__ __forceinline__ void build_q(const PagedArgs& a, const Entry& e, int hk, unsigned char* q, RowConst<R>& rc,
-                                        int t) {
+__device__ __forceinline__ void build_q(const PagedArgs& a, unsigned char* q, RowConst<R>& rc, int t) {
   using S = Shape<D, ES, R>;
   constexpr int SW = S::SW;
   constexpr int TPR = D / 8;      // threads per row, 8 elements each
   constexpr int ROWS = NT / TPR;  // rows at once
   constexpr int PASSES = (R + ROWS - 1) / ROWS;
-  // rows in flight per thread: a lone warp waits for memory, many warps for instructions
-  constexpr int UN = PASSES < 2 ? 1 : (NT == 32 && PASSES >= 8 ? 8 : 2);
+  constexpr int UN = PASSES < 4 ? PASSES : 4;  // rows in flight per thread
   const int d0 = (t % TPR) * 8;
-  const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0;
-  const float dom = capped ? 1.f : kLog2e;
+  const float dom = (a.score.flags & FA_SCORE_SOFTCAP) ? 1.f : kLog2e;
 #pragma unroll 1
   for (int p0 = 0; p0 < PASSES; p0 += UN) {
-    if (p0 > 0 && e.rg * R + p0 * ROWS >= a.M) {  // rows that do not exist: an operand of zeros
-      zero_rows<D, ES, R, NT>(q, rc, p0 * ROWS, t);
-      break;
-    }
     uint4 raws[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int n = (p0 + u) * ROWS + t / TPR, m = e.rg * R + n, i = m / a.G;
+      const int n = (p0 + u) * ROWS + t / TPR;
       raws[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (n < R && m < a.M && i < e.ql) {
-        const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.ptr) + (int64_t)e.b * a.q.stride_b +
-                             (int64_t)(hk * a.G + (m - i * a.G)) * a.q.stride_h + (int64_t)i * a.q.stride_t + d0;
+      const int64_t off = n < R ? rc.qoff[n] : -1;
+      if (off >= 0) {
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.ptr) + off + d0;
         if (a.q_vec) {
           raws[u] = __ldg(reinterpret_cast<const uint4*>(qp));
         } else {
@@ -397,37 +398,28 @@ __device__ __forceinline__ void build_q(const PagedArgs& a, const Entry& e, int 
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int n = (p0 + u) * ROWS + t / TPR, m = e.rg * R + n, i = m / a.G, h = hk * a.G + (m - i * a.G);
+      const int n = (p0 + u) * ROWS + t / TPR;
       const uint4 raw = raws[u];
       float fix = 1.f;  // undoes the row's power of two
       if constexpr (ES == 2) {
         if (n < R) *reinterpret_cast<uint4*>(q + (d0 * 2 / SW) * S::QPANEL + panel_off<SW>(n, (d0 * 2 % SW) >> 4)) = raw;
       } else {
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        float f[8], top = 0.f;
-        bool odd = false;
+        // The largest magnitude: bf16 magnitudes compare as integers, NaN and infinity come out above all.
+        uint32_t top = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f[2 * k] = __uint_as_float(w[k] << 16);
-          f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-        }
+        for (int k = 0; k < 4; ++k) top = max(top, max((w[k] << 16) & 0x7fff0000u, w[k] & 0x7fff0000u));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          top = fmaxf(top, fabsf(f[k]));
-          odd = odd | !(fabsf(f[k]) < INFINITY);
-        }
-        if (odd) top = INFINITY;
-#pragma unroll
-        for (int o = TPR / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // 2^sh brings the largest magnitude into [128, 256) (at most 2^100: tinier rows stay small)
-        const int ex = (int)(__float_as_uint(top) >> 23) - 127;
-        const int sh = top > 0.f && top < INFINITY ? min(7 - ex, 100) : 0;
+        for (int o = TPR / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // 2^sh brings it into [128, 256) (at most 2^100: tinier rows stay small)
+        const bool finite = top < 0x7f800000u;
+        const int sh = top > 0 && finite ? min(7 + 127 - (int)(top >> 23), 100) : 0;
         const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
-        fix = __uint_as_float((uint32_t)(127 - sh) << 23);
-        if (top == INFINITY) fix = __uint_as_float(0x7fc00000u);  // NaN or infinity in q: the row is NaN
+        fix = finite ? __uint_as_float((uint32_t)(127 - sh) << 23) : __uint_as_float(0x7fc00000u);  // such a row is NaN
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) hi[k] = split_e4m3x2(f[2 * k] * up, f[2 * k + 1] * up, &lo[k]);
+        for (int k = 0; k < 4; ++k)
+          hi[k] = split_e4m3x2(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xffff0000u) * up, &lo[k]);
         if (n < R) {
           unsigned char* at = q + (d0 / SW) * S::QPANEL + (d0 & 8);
           const int c = (d0 % SW) >> 4;
@@ -436,28 +428,30 @@ __device__ __forceinline__ void build_q(const PagedArgs& a, const Entry& e, int 
               make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
         }
       }
-      if (d0 == 0 && n < R) {
-        const bool real = m < a.M, live = real && i < e.ql;
-        const int qpos = e.len - e.ql + i;
-        int lo = 0, hi = e.len - 1;
-        if (a.mask.flags & FA_MASK_CAUSAL) hi = min(hi, qpos);
-        if (a.mask.flags & FA_MASK_WINDOW) {
-          if (a.mask.window_left >= 0) lo = max(lo, qpos - a.mask.window_left);
-          if (a.mask.window_right >= 0) hi = (int)min((int64_t)hi, (int64_t)qpos + a.mask.window_right);
-        }
-        rc.xs[n] = a.scale * fix * dom;
-        rc.slope[n] = live && (a.score.flags & FA_SCORE_ALIBI) ? __ldg(a.score.alibi_slopes + h) * dom : 0.f;
-        rc.lo[n] = live ? lo : 1;
-        rc.hi[n] = live ? hi : 0;
-        rc.qpos[n] = qpos;
-        rc.orow[n] = real ? (int64_t)e.b * a.o.stride_b + (int64_t)h * a.o.stride_h + (int64_t)i * a.o.stride_t : -1;
-        rc.lrow[n] = ((int64_t)e.b * a.H + h) * a.Tq + i;
-      }
+      if (d0 == 0 && n < R) rc.xs[n] = a.scale * fix * dom;
     }
   }
 }
 
-template <int D, int ES, int R>
+// o = 0 and lse = -inf for the rows of an entry without a tile, those heads that are this CTA's.
+template <int D, int R>
+__device__ __forceinline__ void empty_rows(const PagedArgs& a, int e, int cta, int warp, int warps, int lane) {
+  const int b = a.groups == 1 ? e : e / a.groups, m0 = (e - b * a.groups) * R, rows = min(R, a.M - m0);
+  int hk = cta - e % (int)gridDim.x;
+  if (hk < 0) hk += gridDim.x;
+  for (; hk < a.Hkv; hk += gridDim.x)
+    for (int r = warp; r < rows; r += warps) {
+      const int m = m0 + r, i = m / a.G, h = hk * a.G + m - i * a.G;
+      uint16_t* o = reinterpret_cast<uint16_t*>(a.o.ptr) + (int64_t)b * a.o.stride_b + (int64_t)h * a.o.stride_h +
+                    (int64_t)i * a.o.stride_t;
+#pragma unroll
+      for (int d = 0; d < D; d += 32) o[d + lane] = 0;
+      if (lane == 0) a.lse[((int64_t)b * a.H + h) * a.Tq + i] = -INFINITY;
+    }
+}
+
+// MODS: ALiBi or softcap (their code in the common loop costs the plain kernel a third of its time).
+template <int D, int ES, int R, bool MODS>
 __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                       const PagedArgs a) {
@@ -499,6 +493,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     sm.abort_flag = 0;
     sm.never = 0;
     sm.join_parts = 0;
+    sm.empties = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
@@ -540,6 +535,16 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     const int start = (int)min((int64_t)cta * per, (int64_t)total);
     my_start = start;
     my_tiles = min(per, total - start);
+    for (int e = e0; e < e1; ++e) {
+      if (run > 1) x = entry_of<R>(a, e);
+      if (x.nt) continue;
+      int hk = cta - e % (int)gridDim.x;  // some of its heads' rows are this CTA's to write
+      if (hk < 0) hk += gridDim.x;
+      if (hk < a.Hkv) {
+        const int k = atomicAdd(&sm.empties, 1);
+        if (k < 64) sm.empty_entry[k] = e;
+      }
+    }
     int at = before + inc - mine;
     if (start < total && at <= start && start < at + mine) {  // the range begins in one of this thread's entries
       for (int e = e0; e < e1; ++e) {
@@ -754,7 +759,9 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       } else {
         if (seg >= 2) ok = wait_for_w(sm.q_empty + buf, (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
         if (!ok) break;
-        build_q<D, ES, R, 32>(a, wk.e, sg.hk, sQ + buf * S::QBUF, sm.rc[buf], lane);
+        build_rows<R>(a, wk.e, sg.hk, sm.rc[buf], lane, 32);
+        __syncwarp();
+        build_q<D, ES, R, 32>(a, sQ + buf * S::QBUF, sm.rc[buf], lane);
         fence_proxy_async_smem();
       }
       __syncwarp();
@@ -773,12 +780,15 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     constexpr float LIFT = lift_of(ES), SLACK = slack_of(ES), HEAD = head_of(ES);
     constexpr int PW = 16 / ES;  // rows per 16-byte store of P
     constexpr bool KEEP = NG < 4;
+    constexpr bool SKIP = TURNS;  // (elsewhere the branches cost more than the rows that they would spare)
     constexpr int CH = 4;        // rows worked on together; the ones behind the last real row are left out
     int j = 0;
     for (int seg = 0; wk.next(a, &sg); ++seg) {
       const RowConst<R>& rc = sm.rc[seg & 1];
       if (seg == 0) {
-        build_q<D, ES, R, NSM>(a, wk.e, sg.hk, sQ, sm.rc[0], tid);
+        build_rows<R>(a, wk.e, sg.hk, sm.rc[0], tid, NSM);
+        named_bar_sync(5, NSM);
+        build_q<D, ES, R, NSM>(a, sQ, sm.rc[0], tid);
         fence_proxy_async_smem();
         named_bar_sync(6, NSM + 32);
       }
@@ -817,11 +827,10 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         const bool inside = p0 >= wk.e.in_lo && p0 + kTile - 1 <= wk.e.in_hi && !odd;
         tmem_ld_wait();
         reg_pin(r);
-        const bool special = alibi | capped | !inside;
         float z[C], top = -INFINITY;
 #pragma unroll
         for (int c = 0; c < C; c += CH) {
-          if (c >= rr) {
+          if (SKIP && c >= rr) {
 #pragma unroll
             for (int n = c; n < c + CH; ++n) z[n] = -INFINITY;
             continue;
@@ -834,20 +843,26 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           for (int n = c; n < c + CH; ++n) {
             float x = __uint_as_float(r[n]);
             if constexpr (S::SIDE) x += __uint_as_float(r[8 + n]);
-            z[n] = ES == 1 ? fmaf(x, ks * xs[n], lv) : x * xs[n];
-          }
-          if (special) {
-#pragma unroll
-            for (int n = c; n < c + CH; ++n) {
-              float x = __uint_as_float(r[n]);
-              if constexpr (S::SIDE) x += __uint_as_float(r[8 + n]);
-              x *= ES == 1 ? ks * xs[n] : xs[n];
+            const float k = ES == 1 ? ks * xs[n] : xs[n];
+            if constexpr (!MODS) {
+              z[n] = ES == 1 ? fmaf(x, k, lv) : x * k;
+            } else {
+              x *= k;
               if (alibi) x = fmaf(rc.slope[c0 + n], (float)(pos - rc.qpos[c0 + n]), x);
               // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))), in log2 units
               if (capped) x = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + ex2_approx(x * cap_k)), cap2);
-              z[n] = (!shown | (pos < rc.lo[c0 + n]) | (pos > rc.hi[c0 + n])) ? -INFINITY : x + lv;
+              z[n] = x + lv;
             }
           }
+        }
+        if (!inside) {
+#pragma unroll
+          for (int n = 0; n < C; ++n)
+            if (!shown | (pos < rc.lo[c0 + n]) | (pos > rc.hi[c0 + n])) z[n] = -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < C; c += CH) {
+          if (SKIP && c >= rr) continue;
           if constexpr (!KEEP) {
             const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
             bias[c] = b4.x, bias[c + 1] = b4.y, bias[c + 2] = b4.z, bias[c + 3] = b4.w;
@@ -904,7 +919,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
 #pragma unroll
           for (int k = 0; k < ES; ++k) hi[c / 4 * ES + k] = 0u;
           lo[c / 4] = 0u;
-          if (c >= rr) continue;
+          if (SKIP && c >= rr) continue;
           if constexpr (!KEEP) {
             const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
             bias[c] = b4.x, bias[c + 1] = b4.y, bias[c + 2] = b4.z, bias[c + 3] = b4.w;
@@ -1045,19 +1060,12 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     tmem_dealloc(tmem, S::TM_COLS);
   }
   // ---------------------------------------------------------------- entries without a tile: rows that see nothing
-  for (int e = cta; e < a.entries; e += gridDim.x) {
-    const Entry x = entry_of<R>(a, e);
-    if (x.nt) continue;
-    const int m0 = x.rg * R, rows = min(R, a.M - m0);
-    for (int r = warp; r < a.Hkv * rows; r += NT / 32) {
-      const int hk = r / rows, m = m0 + r - hk * rows, i = m / a.G, h = hk * a.G + m - i * a.G;
-      uint16_t* o = reinterpret_cast<uint16_t*>(a.o.ptr) + (int64_t)x.b * a.o.stride_b + (int64_t)h * a.o.stride_h +
-                    (int64_t)i * a.o.stride_t;
-#pragma unroll
-      for (int d = 0; d < D; d += 32) o[d + lane] = 0;
-      if (lane == 0) a.lse[((int64_t)x.b * a.H + h) * a.Tq + i] = -INFINITY;
-    }
-  }
+  // Head hk of entry e is CTA (e + hk) % CTAs's.
+  const int noted = min(sm.empties, 64);
+  for (int k = 0; k < noted; ++k) empty_rows<D, R>(a, sm.empty_entry[k], cta, warp, NT / 32, lane);
+  if (sm.empties > 64)  // more than the list holds: look again
+    for (int e = 0; e < a.entries; ++e)
+      if (entry_of<R>(a, e).nt == 0) empty_rows<D, R>(a, e, cta, warp, NT / 32, lane);
   if (!a.joins) return;
   // ---------------------------------------------------------------- units that cross CTAs
   const auto grid = cooperative_groups::this_grid();
@@ -1176,14 +1184,14 @@ int check_paged(const FaPagedAttnParams* p) {
   return FA_OK;
 }
 
-template <int D, int ES, int R>
+template <int D, int ES, int R, bool MODS>
 cudaError_t launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedArgs& a, const PagedPlan& pl,
                          cudaStream_t stream) {
   const size_t fixed = paged_smem_bytes<D, ES, R>(0), limit = 232448;
   a.slots = (int)std::min<size_t>(kMaxSlots, (limit - fixed) / Shape<D, ES, R>::SLOT);
   const size_t smem = paged_smem_bytes<D, ES, R>(a.slots);
   cudaError_t e =
-      cudaFuncSetAttribute(paged_attn_kernel<D, ES, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      cudaFuncSetAttribute(paged_attn_kernel<D, ES, R, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   a.joins = (a.cols << a.ps_log) > kTile && pl.ctas > 1;  // (a unit of one tile lies in one CTA)
   cudaLaunchConfig_t cfg = {};
@@ -1196,7 +1204,13 @@ cudaError_t launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedArgs
   at.val.cooperative = a.joins;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<D, ES, R>, tk, tv, (const PagedArgs)a);
+  return cudaLaunchKernelEx(&cfg, paged_attn_kernel<D, ES, R, MODS>, tk, tv, (const PagedArgs)a);
+}
+
+template <int D, int ES, int R>
+cudaError_t launch_mods(const CUtensorMap& tk, const CUtensorMap& tv, PagedArgs& a, const PagedPlan& pl,
+                        cudaStream_t st) {
+  return a.score.flags ? launch_paged<D, ES, R, true>(tk, tv, a, pl, st) : launch_paged<D, ES, R, false>(tk, tv, a, pl, st);
 }
 
 template <int D>
@@ -1204,15 +1218,15 @@ cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, PagedArgs&
                         cudaStream_t st) {
   if (f8) {
     switch (pl.R) {
-      case 8: return launch_paged<D, 1, 8>(tk, tv, a, pl, st);
-      case 16: return launch_paged<D, 1, 16>(tk, tv, a, pl, st);
-      case 32: return launch_paged<D, 1, 32>(tk, tv, a, pl, st);
-      default: return launch_paged<D, 1, 64>(tk, tv, a, pl, st);
+      case 8: return launch_mods<D, 1, 8>(tk, tv, a, pl, st);
+      case 16: return launch_mods<D, 1, 16>(tk, tv, a, pl, st);
+      case 32: return launch_mods<D, 1, 32>(tk, tv, a, pl, st);
+      default: return launch_mods<D, 1, 64>(tk, tv, a, pl, st);
     }
   }
-  if (pl.R == 16) return launch_paged<D, 2, 16>(tk, tv, a, pl, st);
-  if (D == 256 || pl.R == 32) return launch_paged<D, 2, 32>(tk, tv, a, pl, st);
-  if constexpr (D < 256) return launch_paged<D, 2, 64>(tk, tv, a, pl, st);
+  if (pl.R == 16) return launch_mods<D, 2, 16>(tk, tv, a, pl, st);
+  if (D == 256 || pl.R == 32) return launch_mods<D, 2, 32>(tk, tv, a, pl, st);
+  if constexpr (D < 256) return launch_mods<D, 2, 64>(tk, tv, a, pl, st);
   return cudaErrorInvalidValue;
 }
 
