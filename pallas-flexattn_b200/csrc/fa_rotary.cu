@@ -27,11 +27,21 @@ namespace {
 constexpr int kScaleFloor = -100;  // least exponent of a page's scale
 
 // ------------------------------------------------------------------ elements
+// Eight elements as they lie in memory (16 or 32 bytes), and as floats.  Streaming loads: nothing
+// is read twice.
 template <typename T> struct Io;
 template <> struct Io<__nv_bfloat16> {
-  static __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  struct Raw { uint4 v; };
+  static __device__ __forceinline__ Raw fetch(const __nv_bfloat16* p) {
+    return {__ldcs(reinterpret_cast<const uint4*>(p))};
+  }
+  static __device__ __forceinline__ Raw gather(const __nv_bfloat16* p) {  // any alignment
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    return {make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                       h[6] | (uint32_t)h[7] << 16)};
+  }
+  static __device__ __forceinline__ void floats(const Raw& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f[2 * i] = __uint_as_float(w[i] << 16);
@@ -51,10 +61,16 @@ template <> struct Io<__nv_bfloat16> {
   static __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 };
 template <> struct Io<float> {
-  static __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  struct Raw { float4 a, b; };
+  static __device__ __forceinline__ Raw fetch(const float* p) {
+    return {__ldcs(reinterpret_cast<const float4*>(p)), __ldcs(reinterpret_cast<const float4*>(p) + 1)};
+  }
+  static __device__ __forceinline__ Raw gather(const float* p) {
+    return {make_float4(p[0], p[1], p[2], p[3]), make_float4(p[4], p[5], p[6], p[7])};
+  }
+  static __device__ __forceinline__ void floats(const Raw& r, float (&f)[8]) {
+    f[0] = r.a.x; f[1] = r.a.y; f[2] = r.a.z; f[3] = r.a.w;
+    f[4] = r.b.x; f[5] = r.b.y; f[6] = r.b.z; f[7] = r.b.w;
   }
   static __device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
@@ -63,13 +79,19 @@ template <> struct Io<float> {
   static __device__ __forceinline__ float get(const float* p) { return *p; }
   static __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 };
-
-// cos and sin of pair i at position pos, times the magnitude.
+// cos and sin of pair i at position pos, times the magnitude.  fp32 tensors get sincospi (2 ulp); for
+// bf16 ones the special-function unit's sine and cosine of the reduced angle (2^-21 on [-pi, pi])
+// lie as far below the rounding of the result, at a fifth of the instructions.
+template <typename T>
 __device__ __forceinline__ void pair_turn(const FaRotarySpec& r, int i, int pos, float sign, float* c, float* s) {
   const uint64_t phase = (uint64_t)(int64_t)pos * __ldg(r.turns + i);
-  const float half_turns = (float)(int32_t)(phase >> 32) * 4.656612873077393e-10f;  // 2^-31: in [-1, 1)
+  const float half_turns = (float)(int32_t)(phase >> 32) * 4.656612873077393e-10f;  // 2^-31: in [-1, 1]
   float sn, cs;
-  sincospif(half_turns, &sn, &cs);
+  if constexpr (sizeof(T) == 4) {
+    sincospif(half_turns, &sn, &cs);
+  } else {
+    __sincosf(half_turns * 3.14159265358979f, &sn, &cs);
+  }
   *c = cs * r.magnitude;
   *s = sn * (r.magnitude * sign);
 }
@@ -123,7 +145,8 @@ __device__ __forceinline__ T* head_row(const FaTensor& q, const FaTensor& k, int
          (int64_t)t * x.stride_t;
 }
 
-// Heads [h0, h1) of one unit of one token.  Four heads' loads are issued before the first use.
+// Heads [h0, h1) of one unit of one token.  Two heads (one of fp32) are in work and the next two on
+// their way, as they lie in memory: few registers, so that many warps share an SM.
 template <typename T>
 __device__ __forceinline__ void rotate_heads(const FaTensor& q, const FaTensor& k, const FaTensor& qo,
                                              const FaTensor& ko, const FaRotarySpec& r, int H, int h0, int h1, int b,
@@ -131,33 +154,44 @@ __device__ __forceinline__ void rotate_heads(const FaTensor& q, const FaTensor& 
   int e0, e1;
   const bool rot = unit_span(r, u, &e0, &e1);
   const bool inter = r.layout == FA_ROTARY_INTERLEAVED;
+  constexpr int UN = sizeof(T) == 4 ? 1 : 2;
+  typename Io<T>::Raw raw[UN][2];
+  auto fetch = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < UN; ++i)
+      if (h + i < h1) {
+        const T* x = head_row<const T>(q, k, H, h + i, b, t);
+        raw[i][0] = Io<T>::fetch(x + e0);
+        raw[i][1] = Io<T>::fetch(x + e1);
+      }
+  };
+  fetch(h0);
   float c[8], s[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     c[j] = 1.f;
     s[j] = 0.f;
+    if (rot) pair_turn<T>(r, 8 * u + j, pos, sign, &c[j], &s[j]);  // behind the first loads, which it overlaps
   }
-  constexpr int UN = 4;
+#pragma unroll 1
   for (int h = h0; h < h1; h += UN) {
-    float g0[UN][8], g1[UN][8];
+    typename Io<T>::Raw now[UN][2];
 #pragma unroll
-    for (int i = 0; i < UN; ++i)
-      if (h + i < h1) {
-        const T* x = head_row<const T>(q, k, H, h + i, b, t);
-        Io<T>::load8(x + e0, g0[i]);
-        Io<T>::load8(x + e1, g1[i]);
-      }
-    if (h == h0 && rot) {  // behind the first loads, which it overlaps
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pair_turn(r, 8 * u + j, pos, sign, &c[j], &s[j]);
+    for (int i = 0; i < UN; ++i) {
+      now[i][0] = raw[i][0];
+      now[i][1] = raw[i][1];
     }
+    fetch(h + UN);
 #pragma unroll
     for (int i = 0; i < UN; ++i)
       if (h + i < h1) {
-        if (rot) turn16(g0[i], g1[i], c, s, inter);
+        float g0[8], g1[8];
+        Io<T>::floats(now[i][0], g0);
+        Io<T>::floats(now[i][1], g1);
+        if (rot) turn16(g0, g1, c, s, inter);
         T* y = head_row<T>(qo, ko, H, h + i, b, t);
-        Io<T>::store8(y + e0, g0[i]);
-        Io<T>::store8(y + e1, g1[i]);
+        Io<T>::store8(y + e0, g0);
+        Io<T>::store8(y + e1, g1);
       }
   }
 }
@@ -185,7 +219,7 @@ __global__ void __launch_bounds__(256) rotary_pair_kernel(const RotaryArgs a) {
   const bool rot = u < half, inter = a.r.layout == FA_ROTARY_INTERLEAVED;
   const int e0 = rot && !inter ? u : 2 * u, e1 = rot && !inter ? half + u : 2 * u + 1;
   float c = 1.f, s = 0.f;
-  if (rot) pair_turn(a.r, u, pos, a.sign, &c, &s);
+  if (rot) pair_turn<T>(a.r, u, pos, a.sign, &c, &s);
   const int h0 = blockIdx.y * a.heads_per_thread, h1 = min(h0 + a.heads_per_thread, a.H + a.Hkv);
   for (int h = h0; h < h1; ++h) {
     const T* x = head_row<const T>(a.q, a.k, a.H, h, b, t);
@@ -242,8 +276,10 @@ __device__ __forceinline__ float page_scale(float top) {
 }
 
 // One team (a warp, or the block) takes the rows of one (sequence, touched page, K/V head) of K
-// or of V.  Its new rows stay in registers between the search for the largest magnitude and the
-// store, so they are read once; teams share nothing, and no atomic decides a value.
+// or of V.  Its new rows stay in registers as they lie in memory between the search for the largest
+// magnitude and the store (a key is turned twice, which costs less than the registers of its fp32
+// values: half as many teams would share an SM), so they are read once; teams share nothing, and no
+// atomic decides a value.  The page's number and its scale are fetched behind the rows' loads.
 constexpr int kAppendPasses = 4;  // row groups a team holds: 4 x 16 values a thread
 
 template <typename T, bool E4M3, bool WARP>
@@ -256,10 +292,6 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
   const int first = col * a.ps;  // position of the page's row 0
   if (first >= len || start == len) return;
   const int page = __ldg(a.table + (int64_t)b * a.table_stride + col);
-  if ((unsigned)page >= (unsigned)a.num_pages) {
-    if (tid == 0) report_status(a.status, FA_ERR_INVALID);
-    return;
-  }
   const int r0 = max(start - first, 0), r1 = min(len - first, a.ps);  // rows the new tokens take
   const int u = tid % a.units, rows_at_once = nt / a.units, row_in = tid / a.units;
   int e0, e1;
@@ -268,66 +300,70 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
   const FaTensor& x = which ? a.v : a.k;
   const FaTensor& cache = which ? a.vc : a.kc;
   const T* src = reinterpret_cast<const T*>(x.ptr) + (int64_t)b * x.stride_b + (int64_t)hk * x.stride_h;
-  const int64_t base = (int64_t)page * cache.stride_b + (int64_t)hk * cache.stride_h;
 
-  float g0[kAppendPasses][8], g1[kAppendPasses][8], top = 0.f;
+  typename Io<T>::Raw raw[kAppendPasses][2];
 #pragma unroll
   for (int p = 0; p < kAppendPasses; ++p) {
     const int row = r0 + p * rows_at_once + row_in;
     if (row_in < rows_at_once && row < r1) {
       const T* s = src + (int64_t)(first + row - start) * x.stride_t;
-      if (a.vec) {
-        Io<T>::load8(s + e0, g0[p]);
-        Io<T>::load8(s + e1, g1[p]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          g0[p][j] = Io<T>::get(s + e0 + j);
-          g1[p][j] = Io<T>::get(s + e1 + j);
-        }
-      }
+      raw[p][0] = a.vec ? Io<T>::fetch(s + e0) : Io<T>::gather(s + e0);
+      raw[p][1] = a.vec ? Io<T>::fetch(s + e1) : Io<T>::gather(s + e1);
     }
   }
-#pragma unroll
-  for (int p = 0; p < kAppendPasses; ++p) {
-    const int row = r0 + p * rows_at_once + row_in;
-    if (row_in < rows_at_once && row < r1) {
-      if (rot) {
-        float c[8], s[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pair_turn(a.r, 8 * u + j, first + row, 1.f, &c[j], &s[j]);
-        turn16(g0[p], g1[p], c, s, inter);
-      }
-      if constexpr (E4M3) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float m0 = fabsf(g0[p][j]), m1 = fabsf(g1[p][j]);
-          top = fmaxf(top, m0 < INFINITY ? m0 : 0.f);  // NaN and infinities do not set the scale
-          top = fmaxf(top, m1 < INFINITY ? m1 : 0.f);
-        }
-      }
-    }
+  const bool known = (unsigned)page < (unsigned)a.num_pages;
+  float* scale = (which ? a.v_scale : a.k_scale) + (int64_t)page * a.Hkv + hk;
+  const float was = E4M3 && known ? *scale : 0.f;  // read by every thread before the barrier, written after it
+  if (!known) {  // the same page for the whole team
+    if (tid == 0) report_status(a.status, FA_ERR_INVALID);
+    return;
   }
+  const int64_t base = (int64_t)page * cache.stride_b + (int64_t)hk * cache.stride_h;
+  auto values = [&](int p, float (&g0)[8], float (&g1)[8]) {  // of this thread's row of pass p
+    Io<T>::floats(raw[p][0], g0);
+    Io<T>::floats(raw[p][1], g1);
+    if (rot) {
+      const int pos = first + r0 + p * rows_at_once + row_in;
+      float c[8], s[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pair_turn<T>(a.r, 8 * u + j, pos, 1.f, &c[j], &s[j]);
+      turn16(g0, g1, c, s, inter);
+    }
+  };
   if constexpr (!E4M3) {
     __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(cache.ptr) + base;
 #pragma unroll
     for (int p = 0; p < kAppendPasses; ++p) {
       const int row = r0 + p * rows_at_once + row_in;
       if (row_in < rows_at_once && row < r1) {
-        Io<__nv_bfloat16>::store8(dst + (int64_t)row * cache.stride_t + e0, g0[p]);
-        Io<__nv_bfloat16>::store8(dst + (int64_t)row * cache.stride_t + e1, g1[p]);
+        float g0[8], g1[8];
+        values(p, g0, g1);
+        Io<__nv_bfloat16>::store8(dst + (int64_t)row * cache.stride_t + e0, g0);
+        Io<__nv_bfloat16>::store8(dst + (int64_t)row * cache.stride_t + e1, g1);
       }
     }
-    return;
   } else {
+    float top = 0.f;
+#pragma unroll
+    for (int p = 0; p < kAppendPasses; ++p) {
+      const int row = r0 + p * rows_at_once + row_in;
+      if (row_in < rows_at_once && row < r1) {
+        float g0[8], g1[8];
+        values(p, g0, g1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float m0 = fabsf(g0[j]), m1 = fabsf(g1[j]);
+          top = fmaxf(top, m0 < INFINITY ? m0 : 0.f);  // NaN and infinities do not set the scale
+          top = fmaxf(top, m1 < INFINITY ? m1 : 0.f);
+        }
+      }
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float* scale = (which ? a.v_scale : a.k_scale) + (int64_t)page * a.Hkv + hk;
-    const float was = *scale;  // read by every thread before the barrier, written after it
     if constexpr (!WARP) {
       if ((tid & 31) == 0) red[tid >> 5] = top;
       __syncthreads();
-      for (int w = 0; w < (nt + 31) / 32; ++w) top = fmaxf(top, red[w]);
+      for (int w = 0; w < nt / 32; ++w) top = fmaxf(top, red[w]);
     } else {
       __syncwarp();
     }
@@ -337,6 +373,7 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
     if (r0 > 0 && s > was) {  // requantise them: exact but for what falls below the smallest step
       const float ratio = was / s;
       const int chunks = a.D / 16;
+#pragma unroll 1
       for (int e = tid; e < r0 * chunks; e += nt) {
         uint4* w = reinterpret_cast<uint4*>(dst + (int64_t)(e / chunks) * cache.stride_t + (e % chunks) * 16);
         uint4 v = *w;
@@ -354,30 +391,34 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
     for (int p = 0; p < kAppendPasses; ++p) {
       const int row = r0 + p * rows_at_once + row_in;
       if (row_in < rows_at_once && row < r1) {
+        float g0[8], g1[8];
+        values(p, g0, g1);
         uint8_t* d = dst + (int64_t)row * cache.stride_t;
-        *reinterpret_cast<uint2*>(d + e0) = to_e4m3x8(g0[p], inv);
-        *reinterpret_cast<uint2*>(d + e1) = to_e4m3x8(g1[p], inv);
+        *reinterpret_cast<uint2*>(d + e0) = to_e4m3x8(g0, inv);
+        *reinterpret_cast<uint2*>(d + e1) = to_e4m3x8(g1, inv);
       }
     }
     if (tid == 0 && s != was) *scale = s;
   }
 }
 
-// Blocks [0, kv_blocks) append; the rest rotate q.
+// kv_blocks blocks append and the rest rotate q, spread evenly over the grid: appends wait for memory
+// most of the time, and q's stream of loads and stores fills it.
 template <typename T, bool E4M3, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 512) append_kernel(const AppendArgs a) {
   __shared__ float red[16];
-  if ((int)blockIdx.x < a.kv_blocks) {
+  const int before = (int)((int64_t)blockIdx.x * a.kv_blocks / gridDim.x);  // appending blocks before this one
+  if ((int)((int64_t)(blockIdx.x + 1) * a.kv_blocks / gridDim.x) > before) {
     const int teams = a.B * a.pages_per_seq * a.Hkv * 2;
     if constexpr (WARP) {
-      const int team = blockIdx.x * 4 + (threadIdx.x >> 5);
+      const int team = before * 4 + (threadIdx.x >> 5);
       if (team < teams) append_team<T, E4M3, true>(a, team, threadIdx.x & 31, 32, red);
     } else {
-      append_team<T, E4M3, false>(a, blockIdx.x, threadIdx.x, blockDim.x, red);
+      append_team<T, E4M3, false>(a, before, threadIdx.x, blockDim.x, red);
     }
     return;
   }
-  const unsigned qb = blockIdx.x - a.kv_blocks;  // (token block, head chunk), head chunk outermost
+  const unsigned qb = blockIdx.x - before;  // (token block, head chunk), head chunk outermost
   const unsigned idx = (qb % a.q_blocks) * blockDim.x + threadIdx.x;
   if (idx >= (unsigned)a.B * a.T * a.units) return;
   const unsigned tok = idx / a.units, b = tok / a.T;
@@ -394,7 +435,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) append_kernel(const AppendAr
   float c[8], s[8];
   if (ok && start + t < len && rot) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) pair_turn(a.r, 8 * u + j, start + t, 1.f, &c[j], &s[j]);
+    for (int j = 0; j < 8; ++j) pair_turn<T>(a.r, 8 * u + j, start + t, 1.f, &c[j], &s[j]);
   }
   for (int h = h0; h < h1; ++h) {  // padding rows, and tensors that 16-byte accesses do not fit
     float g0[8] = {0.f}, g1[8] = {0.f};
@@ -422,10 +463,10 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) append_kernel(const AppendAr
 }
 
 // Heads a thread takes: its cosines and sines serve all of them, but the grid should still fill
-// the SMs (148 x 2048 threads), and a single token spreads over as many threads as it has heads.
+// the SMs (148 x 512 threads, a quarter of what they hold), and a single token spreads over as many threads as it has heads.
 int heads_per_thread(int64_t token_units, int heads) {
   int n = 1;
-  while (n < 8 && token_units * ((heads + 2 * n - 1) / (2 * n)) >= 148 * 2048) n *= 2;
+  while (n < 8 && token_units * ((heads + 2 * n - 1) / (2 * n)) >= 148 * 512) n *= 2;
   return n;
 }
 

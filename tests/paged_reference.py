@@ -20,9 +20,10 @@ def rotate64(x, spec, pos, inverse=False):
     """x (..., T, D) turned by pos (T,) in 64 bits, and the error bound of the kernel's result.
 
     The phase is exact; its conversion to fp32 is off by 2^-24 relative, at most 2^-24 pi in the
-    angle; sincospi is within 2 ulp (2^-22) and the magnitude's product adds 2^-24: each of cos and
-    sin is off by less than e = m (2^-22 + 2^-22 + 2^-24).  Two products and a sum round at most three
-    times (3 * 2^-24 of m (|a| + |b|)), then the result is rounded once to x's type."""
+    angle.  fp32: sincospi is within 2 ulp (2^-22).  bf16: the angle's product with pi adds 2^-23 pi, and
+    the hardware's sine and cosine are within 2^-21 on [-pi, pi].  The magnitude's product adds 2^-24.
+    Two products and a sum round at most three times (3 * 2^-24 of m (|a| + |b|)), then the result is
+    rounded once to x's type."""
     rd, m = spec.rotary_dim, spec.magnitude
     x64 = x.double()
     f = torch.tensor(spec.frequencies, dtype=torch.float64, device=x.device)
@@ -33,9 +34,11 @@ def rotate64(x, spec, pos, inverse=False):
     else:
         a, b = x64[..., : rd // 2], x64[..., rd // 2: rd]
     ra, rb = a * c - b * s, b * c + a * s
-    e = (a.abs() + b.abs()) * m * (2.0 ** -22 + 2.0 ** -22 + 2.0 ** -24 + 3 * U_F32)
+    turn = 2.0 ** -22 + (2.0 ** -22 if x.dtype == torch.float32 else 2.0 ** -21 + 2.0 ** -21) + 2.0 ** -24
+    e = (a.abs() + b.abs()) * m * (turn + 3 * U_F32)
     # the reference's own angle: a 64-bit product of a position below 2^31 is off by 2^-53 * 2^31 = 2^-22
-    e = e + (a.abs() + b.abs()) * m * pos.double().abs().max().item() * 2.0 ** -52 if pos.numel() else e
+    if pos.numel():
+        e = e + (a.abs() + b.abs()) * m * pos.double().abs().max().item() * 2.0 ** -52
     if spec.interleaved:
         out, err = torch.stack((ra, rb), -1).flatten(-2), torch.stack((e, e), -1).flatten(-2)
     else:
