@@ -404,8 +404,9 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
 
 // kv_blocks blocks append and the rest rotate q, spread evenly over the grid: appends wait for memory
 // most of the time, and q's stream of loads and stores fills it.
-template <typename T, bool E4M3, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 512) append_kernel(const AppendArgs a) {
+// NT: the most threads a block may have.
+template <typename T, bool E4M3, bool WARP, int NT>
+__global__ void __launch_bounds__(NT, NT == 512 || sizeof(T) == 4 ? 512 / NT : 768 / NT) append_kernel(const AppendArgs a) {
   __shared__ float red[16];
   const int before = (int)((int64_t)blockIdx.x * a.kv_blocks / gridDim.x);  // appending blocks before this one
   if ((int)((int64_t)(blockIdx.x + 1) * a.kv_blocks / gridDim.x) > before) {
@@ -520,8 +521,9 @@ cudaError_t launch_append(AppendArgs& a, cudaStream_t stream) {
     qb = a.q_blocks * ((a.H + a.heads_per_thread - 1) / a.heads_per_thread);
   }
   const unsigned grid = (unsigned)(a.kv_blocks + qb);
-  if (warp) append_kernel<T, E4M3, true><<<grid, nt, 0, stream>>>(a);
-  else append_kernel<T, E4M3, false><<<grid, nt, 0, stream>>>(a);
+  if (warp) append_kernel<T, E4M3, true, 128><<<grid, nt, 0, stream>>>(a);
+  else if (nt <= 256) append_kernel<T, E4M3, false, 256><<<grid, nt, 0, stream>>>(a);
+  else append_kernel<T, E4M3, false, 512><<<grid, nt, 0, stream>>>(a);
   return cudaGetLastError();
 }
 

@@ -77,7 +77,7 @@ class PagedKVCache:
         self._fields = (_CACHE_DTYPES[k.dtype], n, hkv, ps, d, k.data_ptr(), *k.stride()[:3], v.data_ptr(),
                         *v.stride()[:3], *((k_scale.data_ptr(), v_scale.data_ptr()) if k_scale is not None else (0, 0)))
         self._shape, self._device = (n, hkv, ps, d), k.device
-        self._ws: dict = {}  # workspace bytes by the shape of a call
+        self._plans: dict = {}  # by the shape of a call: see _plan
 
     @classmethod
     def empty(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,
@@ -120,6 +120,12 @@ def _fields(t: torch.Tensor) -> tuple:
     """The fields of an FaTensor."""
     st = t.stride()
     return t.data_ptr(), st[0], st[1], st[2]
+
+
+def _out_like(t: torch.Tensor) -> torch.Tensor:
+    """A dense tensor like `t` with a contiguous last dimension."""
+    o = torch.empty_like(t)
+    return o if o.stride(3) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -182,7 +188,7 @@ def paged_kv_append(cache: PagedKVCache, block_table: torch.Tensor, kv_lens: Len
         raise ValueError("paged_kv_append has no gradient: call it under torch.no_grad()")
     out, heads, fq, fo = None, 0, _NONE, _NONE
     if q is not None:
-        out = torch.empty(q.shape, dtype=dtype, device=dev)
+        out = _out_like(q)
     if B == 0 or T == 0:
         return out
     if q is not None and q.shape[1]:
@@ -198,6 +204,26 @@ def paged_kv_append(cache: PagedKVCache, block_table: torch.Tensor, kv_lens: Len
     with on_device(dev) as stream:
         L.packed_call("fa_paged_append", block, stream)
     return out
+
+
+def _plan(cache: PagedKVCache, B: int, H: int, Tq: int, table: torch.Tensor) -> tuple:
+    """(workspace bytes, patterns of lse and of the workspace) for calls of this shape, kept with the cache.
+    The patterns are one element expanded: torch.empty_like of them costs less than torch.empty."""
+    p = L.FaPagedAttnParams()
+    p.B, p.H, p.Tq = B, H, Tq
+    c = p.cache
+    (c.dtype, c.num_pages, c.H_kv, c.page_size, c.D, c.k.ptr, c.k.stride_b, c.k.stride_h, c.k.stride_t, c.v.ptr,
+     c.v.stride_b, c.v.stride_h, c.v.stride_t, c.k_scale, c.v_scale, c.block_table, c.table_cols,
+     c.table_stride) = cache._packed(table)
+    n = C.c_size_t(0)
+    with on_device(cache._device):
+        L.check(L.lib().fa_paged_attn_workspace_size(C.byref(p), C.byref(n)))
+    if len(cache._plans) >= 256:
+        cache._plans.clear()
+    plan = (n.value, torch.empty(1, dtype=torch.float32, device=cache._device).expand(B, H, Tq),
+            torch.empty(1, dtype=torch.uint8, device=cache._device).expand(n.value))
+    cache._plans[(B, H, Tq, table.shape[1])] = plan
+    return plan
 
 
 def flash_attention_paged(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, kv_lens: Lengths,
@@ -239,13 +265,16 @@ def flash_attention_paged(q: torch.Tensor, cache: PagedKVCache, block_table: tor
     sspec = score_spec_of(score_mod)
     if sspec is None or sspec.flags & ~(L.FA_SCORE_ALIBI | L.FA_SCORE_SOFTCAP):
         raise NotImplementedError("paged attention takes alibi_score_mod, softcap_score_mod or their composition")
-    o = torch.empty((B, H, Tq, D), dtype=torch.bfloat16, device=dev)
-    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
     if B == 0 or Tq == 0:
-        return o, lse
+        return torch.empty_like(q), torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
     q = _rows(q)
     table, lens = _table(block_table, B, dev), _lengths("kv_lens", kv_lens, B, dev)
     qlen = None if q_lens is None else _lengths("q_lens", q_lens, B, dev)
+    plan = cache._plans.get((B, H, Tq, table.shape[1]))
+    if plan is None:
+        plan = _plan(cache, B, H, Tq, table)
+    size, lse_like, ws_like = plan
+    o, lse, ws = _out_like(q), torch.empty_like(lse_like), torch.empty_like(ws_like)
     slopes = 0
     if sspec.flags & L.FA_SCORE_ALIBI:
         t = sspec.device_tensors(dev)["slopes"]
@@ -257,14 +286,5 @@ def flash_attention_paged(q: torch.Tensor, cache: PagedKVCache, block_table: tor
                             mspec.flags, mspec.window_left, mspec.window_right, *_NO_MASK_TABLES,
                             sspec.flags, sspec.softcap, slopes, 0, 0, 0, *cache._packed(table), status_ptr(dev.index))
     with on_device(dev) as stream:
-        key = (B, H, Tq, table.shape[1])
-        size = cache._ws.get(key)
-        if size is None:
-            n = C.c_size_t(0)
-            L.packed_call("fa_paged_attn_workspace_size", block, C.byref(n))
-            if len(cache._ws) >= 256:
-                cache._ws.clear()
-            size = cache._ws[key] = n.value
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         L.packed_call("fa_paged_attn", block, ws.data_ptr(), size, stream)
     return o, lse

@@ -151,7 +151,25 @@ def _check_qk(q, k, spec):
 
 
 _PACK = L.packer(L.FaRotaryParams)
-_NONE = (0, 0, 0, 0)
+_NONE = (None, 0, (0, 0, 0, 0), (0, 0, 0, 0))
+
+
+def _in_out(t: Optional[torch.Tensor]):
+    """(output tensor, heads, FaTensor of the input, FaTensor of the output), and the input to keep."""
+    if t is None:
+        return _NONE, None
+    if t.numel() == 0:
+        return (torch.empty_like(t), *_NONE[1:]), None
+    sb, sh, st, sd = t.stride()
+    if sd != 1:
+        t = t.contiguous()
+        sb, sh, st, sd = t.stride()
+    o = torch.empty_like(t)
+    ob, oh, ot, od = o.stride()
+    if od != 1:  # an overlapping or broadcast input
+        o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        ob, oh, ot, od = o.stride()
+    return (o, t.shape[1], (t.data_ptr(), sb, sh, st), (o.data_ptr(), ob, oh, ot)), t
 
 
 def _launch(q, k, spec: RotarySpec, positions: Positions, inverse: bool):
@@ -159,37 +177,21 @@ def _launch(q, k, spec: RotarySpec, positions: Positions, inverse: bool):
     x = q if q is not None else k
     B, _, T, D = x.shape
     dev = x.device
-    heads, tensors, out, keep = [], [], [], []
-    for t in (q, k):
-        if t is None or t.numel() == 0:
-            out.append(t if t is None else torch.empty_like(t))
-            heads.append(0)
-            tensors += (_NONE, _NONE)
-            continue
-        if t.stride(3) != 1:
-            t = t.contiguous()
-        o = torch.empty_like(t)
-        st = o.stride()
-        if st[3] != 1:  # an overlapping or broadcast input
-            o = torch.empty(t.shape, dtype=t.dtype, device=dev)
-            st = o.stride()
-        heads.append(t.shape[1])
-        tensors += ((t.data_ptr(), *t.stride()[:3]), (o.data_ptr(), *st[:3]))
-        out.append(o)
-        keep.append(t)
-    if not keep:
-        return tuple(out)
-    pos, pos_stride, offset = 0, 0, 0
-    if isinstance(positions, torch.Tensor):
-        pos = positions.data_ptr()
-        pos_stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
-    elif positions:
-        offset = positions
-    block = _PACK.pack(_DTYPES[x.dtype], B, *heads, T, D, *tensors[0], *tensors[2], *tensors[1], *tensors[3], pos,
-                       pos_stride, offset, inverse, *spec.packed(dev))
-    with on_device(dev) as stream:
-        L.packed_call("fa_rotary", block, stream)
-    return tuple(out)
+    (oq, hq, fq, foq), q = _in_out(q)
+    (ok, hk, fk, fok), k = _in_out(k)
+    if hq or hk:
+        pos, pos_stride, offset = 0, 0, 0
+        if positions is not None:
+            if isinstance(positions, torch.Tensor):
+                pos = positions.data_ptr()
+                pos_stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
+            else:
+                offset = positions
+        block = _PACK.pack(_DTYPES[x.dtype], B, hq, hk, T, D, *fq, *fk, *foq, *fok, pos, pos_stride, offset, inverse,
+                           *spec.packed(dev))
+        with on_device(dev) as stream:
+            L.packed_call("fa_rotary", block, stream)
+    return oq, ok
 
 
 class _Rotary(torch.autograd.Function):
