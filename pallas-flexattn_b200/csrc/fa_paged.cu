@@ -18,8 +18,8 @@
 // (R >= 16), or for R = 8 the parts lie side by side in the MMA's smallest N of 16 and are added
 // when read.  q is scaled by a power of two per row so that its largest magnitude lies in [128, 256):
 // a bf16 has 8 significant bits, each part 4, so the split is exact down to 2^-17 of the row's largest
-// element.  Probabilities lie in [0, 431], the largest of a tile that moved the reference at 64: hi
-// is P cut to 4 bits, lo the rest rounded to 4, off by 2^-8 relative (as a bf16 P is) or by 2^-16 of
+// element.  Probabilities lie in [0, 431], the largest of a tile that moved the reference at 32: hi
+// is P cut to 4 bits, lo the rest rounded to 4, off by 2^-8 relative (as a bf16 P is) or by 2^-15 of
 // the largest below that.
 //
 // Scales.  ks multiplies the thread's logits.  vs goes into the exponent: with z = x + log2 vs and
@@ -66,9 +66,9 @@ constexpr int kScaleRing = 16;     // tiles whose scales may be live at once (> 
 // A reference moves when exceeded by more than slack (log2 units), to head above the tile's largest z;
 // P = 2^(z - reference + lift).  8-bit: P in units of 2^-8, so that fp16's exponents line up with
 // e4m3's (split_e4m3x4), at most 2^(7 + 1.75) = 431, below e4m3's 448; the head spares most moves
-// (each costs about half a tile's time) for one bit at the small end.  bf16 holds 2^60 as well as 1.
+// (each costs about half a tile's time) for two bits at the small end.  bf16 holds 2^60 as well as 1.
 __host__ __device__ constexpr float slack_of(int ES) { return ES == 1 ? 1.75f : 60.f; }
-__host__ __device__ constexpr float head_of(int ES) { return ES == 1 ? 1.f : 0.f; }
+__host__ __device__ constexpr float head_of(int ES) { return ES == 1 ? 2.f : 0.f; }
 __host__ __device__ constexpr float lift_of(int ES) { return ES == 1 ? 7.f - 8.f : 0.f; }
 constexpr float kUnset = -1e30f;   // reference of a row that has seen nothing yet
 
@@ -249,19 +249,17 @@ size_t paged_smem_bytes(int slots) {
   return 1024 + (size_t)slots * S::SLOT + 2 * S::QBUF + 2 * S::PBUF + sizeof(Smem<R>);
 }
 
-// mbar_wait that looks at the clock only now and then: most waits here are short.
+// Bounded wait for a barrier's phase; false when the CTA gave up or after kSpins polls (some 0.1 s of
+// immediate answers, longer as the hardware lets a poll sleep: far above any legitimate wait here).  A
+// few instructions, since two dozen waits in line are what fills the instruction cache.
+constexpr int kSpins = 1 << 22;
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
-  uint64_t t0 = 0;
-  for (uint32_t it = 1;; ++it) {
+#pragma unroll 1
+  for (int n = 0; n < kSpins; ++n) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 15u) == 0u) {
-      if (*abort_flag) return false;
-      const uint64_t t = globaltimer_ns();
-      if (t0 == 0) t0 = t;
-      else if (t - t0 > FA_WAIT_TIMEOUT_NS) return false;
-    }
+    if (*abort_flag) return false;
   }
+  return false;
 }
 __device__ __forceinline__ bool wait_for_w(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   const int ok = wait_for(bar, parity, abort_flag) ? 1 : 0;

@@ -145,9 +145,9 @@ def attend64(q, cache, table, lens, qlens, kind, window, slopes, cap, scale, hid
             rel = U_BF16 + 2.1 * dx[..., None] + (n + 64) * 2.0 ** -23
             tol = pv * rel + oo.abs() * U_BF16
             if f8:
-                # parts below e4m3's smallest step: 2^-10 of P, where the largest p vs is at least 2^6
+                # parts below e4m3's smallest step: 2^-10 of P, where the largest p vs is at least 2^5
                 big = (p * vs).amax(-1, keepdim=True)
-                tol = tol + 2.0 ** -16 * big * v0.div(vs.clamp(min=2.0 ** -100)[:, None]).abs().sum(0)
+                tol = tol + 2.0 ** -15 * big * v0.div(vs.clamp(min=2.0 ** -100)[:, None]).abs().sum(0)
             sl = slice(hk * G, (hk + 1) * G)
             o[b, sl, :t] = oo
             lse[b, sl, :t] = torch.where(some, top[..., 0] + torch.log(z), torch.full_like(z, -math.inf))
