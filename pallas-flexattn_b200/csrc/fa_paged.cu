@@ -117,8 +117,18 @@ struct Shape {
   static_assert(USED <= 512 && N % 16 == 0 && N <= 256 && (ES == 1 || R >= 16), "operand shape");
 };
 
-// Row constants of one unit (double-buffered with Q).
+// One CTA's part of a unit, as the walk finds it.
+struct Seg {
+  int hk, t0, nt;      // K/V head, first tile taken (they go down from there), tiles
+  int first, last;     // holds the unit's first / last tile in that order
+  int rows;            // query rows of the group
+  int lo, hi, in_lo, in_hi;  // of its entry
+  int entry, entry_nt;
+};
+
+// Description and row constants of one unit (double-buffered with Q).
 template <int R> struct RowConst {
+  Seg sg;
   float xs[R];      // logit = dot * (ks * xs): scale, the row's power of two, and log2(e) unless softcapped
   float slope[R];   // ALiBi slope in the same domain
   int lo[R], hi[R]; // positions the row may see; hi < lo: none
@@ -181,11 +191,8 @@ __device__ __forceinline__ Entry entry_of(const PagedArgs& a, int e) {
   return x;
 }
 
-// One CTA's range of tiles, unit by unit.  Every role walks the same sequence by itself.
-struct Seg {
-  int hk, t0, nt;   // K/V head, first tile taken (they go down from there), tiles
-  bool first, last; // holds the unit's first / last tile in that order
-};
+// One CTA's range of tiles, unit by unit, is walked by the producer (each lane for itself) and by the
+// warp that builds Q, which describes each unit's part to the others.
 struct Start {  // where a CTA's range begins
   Entry e;
   int idx, hk, off;
@@ -223,6 +230,13 @@ struct Walker {
     off += s->nt;
     s->last = off == e.nt;
     left -= s->nt;
+    s->rows = a.M - e.rg * R;
+    s->lo = e.lo;
+    s->hi = e.hi;
+    s->in_lo = e.in_lo;
+    s->in_hi = e.in_hi;
+    s->entry = idx;
+    s->entry_nt = e.nt;
     return true;
   }
 };
@@ -485,7 +499,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       mbar_init(sm.p_full + i, TURNS ? 4 : 4 * NG);
       mbar_init(sm.o_full + i, 1);
       mbar_init(sm.q_full + i, 1);
-      mbar_init(sm.q_empty + i, 1 + 4 * NG);  // the S issuer's commit and the softmax warps
+      mbar_init(sm.q_empty + i, 2 + 4 * NG);  // the S issuer's commit, the P V issuer and the softmax warps
       mbar_init(sm.fin_bar + i, 1);
     }
     sm.abort_flag = 0;
@@ -563,9 +577,6 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  Walker<R> wk;
-  wk.begin(sm.start, my_tiles);
-  Seg sg;
 
   if (warp == W_LOAD) {
     // ---------------------------------------------------------------- producer
@@ -576,6 +587,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       int page, hk, active;
       float ks, vs;
     };
+    Walker<R> wk;
+    wk.begin(sm.start, my_tiles);
     int at = sub;  // this lane's tile in the CTA's range
     auto fetch = [&](Page& x) {
       x.active = 0;
@@ -666,10 +679,11 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     int slot = 0, j = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int seg = 0; ok && wk.next(a, &sg); ++seg) {
+    for (int seg = 0; ok && j < my_tiles; ++seg) {
       ok = wait_for_w(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag);
+      const int nt = ok ? sm.rc[seg & 1].sg.nt : 0;
       const uint32_t qb = q_lo + (uint32_t)(((seg & 1) * S::QBUF) >> 4);
-      for (int it = 0; ok && it < sg.nt; ++it, ++j) {
+      for (int it = 0; ok && it < nt; ++it, ++j) {
         if (j >= 2) ok = wait_for_w(sm.p_full + (j & 1), (uint32_t)(((j >> 1) - 1) & 1), abort_flag);
         ok = ok && wait_for_w(sm.full + slot, phase, abort_flag);
         if (!ok) break;
@@ -712,8 +726,12 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     int slot = 1 % NS, j = 0;
     uint32_t phase = 0;
     bool ok = true;
-    while (ok && wk.next(a, &sg)) {
-      for (int it = 0; ok && it < sg.nt; ++it, ++j) {
+    for (int seg = 0; ok && j < my_tiles; ++seg) {
+      ok = wait_for_w(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag);
+      const int nt = ok ? sm.rc[seg & 1].sg.nt : 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sm.q_empty + (seg & 1));
+      for (int it = 0; ok && it < nt; ++it, ++j) {
         ok = wait_for_w(sm.full + slot, phase, abort_flag) &&
              wait_for_w(sm.p_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag);
         if (!ok) break;
@@ -749,14 +767,18 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
   } else if (warp == W_Q) {
     // ---------------------------------------------------------------- Q operand and row constants
     // The softmax warps build the first unit's (they have nothing else to do yet).
+    Walker<R> wk;
+    wk.begin(sm.start, my_tiles);
+    Seg sg;
     bool ok = true;
     for (int seg = 0; ok && wk.next(a, &sg); ++seg) {
       const int buf = seg & 1;
+      if (seg >= 2) ok = wait_for_w(sm.q_empty + buf, (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
+      if (!ok) break;
+      if (lane == 0) sm.rc[buf].sg = sg;
       if (seg == 0) {
         named_bar_sync(6, NSM + 32);
       } else {
-        if (seg >= 2) ok = wait_for_w(sm.q_empty + buf, (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
-        if (!ok) break;
         build_rows<R>(a, wk.e, sg.hk, sm.rc[buf], lane, 32);
         __syncwarp();
         build_q<D, ES, R, 32>(a, sQ + buf * S::QBUF, sm.rc[buf], lane);
@@ -780,25 +802,31 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     constexpr bool KEEP = NG < 4;
     constexpr bool SKIP = TURNS;  // (elsewhere the branches cost more than the rows that they would spare)
     constexpr int CH = 4;        // rows worked on together; the ones behind the last real row are left out
+    if (my_tiles > 0) {
+      build_rows<R>(a, sm.start.e, sm.start.hk, sm.rc[0], tid, NSM);
+      named_bar_sync(5, NSM);
+      build_q<D, ES, R, NSM>(a, sQ, sm.rc[0], tid);
+      fence_proxy_async_smem();
+      named_bar_sync(6, NSM + 32);
+    }
     int j = 0;
-    for (int seg = 0; wk.next(a, &sg); ++seg) {
+#pragma unroll 1
+    for (int seg = 0; j < my_tiles; ++seg) {
       const RowConst<R>& rc = sm.rc[seg & 1];
-      if (seg == 0) {
-        build_rows<R>(a, wk.e, sg.hk, sm.rc[0], tid, NSM);
-        named_bar_sync(5, NSM);
-        build_q<D, ES, R, NSM>(a, sQ, sm.rc[0], tid);
-        fence_proxy_async_smem();
-        named_bar_sync(6, NSM + 32);
-      }
-      const int rr = min(a.M - wk.e.rg * R - c0, C);  // this thread's real rows
       if (t < C) {
         rs.m[t] = kUnset;
         rs.bias[t] = LIFT - kUnset;
       }
-      // No wait leaves the loops: after a time-out every later wait returns at once and nothing is
-      // written at the end.
-      if (!wait_for(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag)) *abort_flag = 1;
-      named_bar_sync(bar, 128);
+      // Inside a unit no wait leaves the loops: after a time-out every later wait returns at once and
+      // nothing is written at the end.
+      // The threads that share barriers agree on whether the unit is known, so that they leave together.
+      const bool lost = !wait_for(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag);
+      if (vote_or(TURNS ? 5 : bar, TURNS ? NSM : 128, lost)) {
+        *abort_flag = 1;
+        break;
+      }
+      const Seg sg = rc.sg;
+      const int rr = min(sg.rows - c0, C);  // this thread's real rows
       float l[C], xs[C], bias[C];  // (640 threads have no registers for the constants: read per tile)
 #pragma unroll
       for (int n = 0; n < C; ++n) {
@@ -822,7 +850,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         // a value scale below 2^-100 counts as zero: its codes are cleared below
         const float lv = ES == 1 ? fmaxf(lg2_approx(sc.y), -100.f) : 0.f;
         const float inv_vs = ES == 1 ? ex2_approx(-lv) : 1.f;
-        const bool inside = p0 >= wk.e.in_lo && p0 + kTile - 1 <= wk.e.in_hi && !odd;
+        const bool inside = p0 >= sg.in_lo && p0 + kTile - 1 <= sg.in_hi && !odd;
         tmem_ld_wait();
         reg_pin(r);
         float z[C], top = -INFINITY;
@@ -941,14 +969,14 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           if constexpr (ES == 1) *reinterpret_cast<uint4*>(pw + S::PPART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           else *reinterpret_cast<uint4*>(pw + 2048) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
         }
-        if (p0 < wk.e.lo || p0 + kTile - 1 > wk.e.hi || odd) {
+        if (p0 < sg.lo || p0 + kTile - 1 > sg.hi || odd) {
           // Positions that no row sees may hold anything (a zero probability times NaN is NaN), and
           // value scales of zero make no contribution: these rows of V become zero when the tile
           // has landed.
           const int ld = 2 * j + 1, slot = ld % NS;
           if (!wait_for(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
           const bool mine = TURNS || grp == 0;  // one group clears
-          if (mine && (pos < wk.e.lo || pos > wk.e.hi || (ES == 1 && !(sc.y >= 0x1p-100f)))) {
+          if (mine && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sc.y >= 0x1p-100f)))) {
             unsigned char* v = base + (size_t)slot * S::SLOT + t * SW;
 #pragma unroll 1
             for (int p = 0; p < S::ROWB / SW; ++p)
@@ -971,10 +999,10 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       const bool whole = sg.first && sg.last;
       const int part = 2 * cta + (seg == 0 ? 0 : 1);
       if (tid == 0 && sg.first && !sg.last) {  // the CTA's last unit, which goes on in the next CTAs
-        const int end = my_start + my_tiles - sg.nt + wk.e.nt;
+        const int end = my_start + my_tiles - sg.nt + sg.entry_nt;
         sm.join_parts = (end - 1) / per - cta + 1;
         sm.join_slot = part;
-        sm.join_entry = wk.idx;
+        sm.join_entry = sg.entry;
         sm.join_hk = sg.hk;
       }
       if (t < C) {
