@@ -141,7 +141,7 @@ template <int R> struct RowConst {
 struct RowState {
   float m[16], bias[16];  // reference; lift - reference
   float move[16];         // factor of the last move
-  float red[4][16];
+  float4 red[16];         // a value of each warp
   float fin[16];          // factor of O at the end
 };
 // What one (sequence, row group) has to visit.
@@ -816,6 +816,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       if (t < C) {
         rs.m[t] = kUnset;
         rs.bias[t] = LIFT - kUnset;
+        rs.move[t] = 1.f;
       }
       // Inside a unit no wait leaves the loops: after a time-out every later wait returns at once and
       // nothing is written at the end.
@@ -898,14 +899,19 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         if (vote_or(bar, 128, top > LIFT + SLACK)) {
           // ---- a reference has to move to the tile's largest z of its row
 #pragma unroll
-          for (int n = 0; n < C; ++n) {
-            const float m = warp_max(z[n]);
-            if (lane == n) rs.red[warp & 3][n] = m;
+          for (int c = 0; c < C; c += CH) {
+            if (SKIP && c >= rr) continue;
+#pragma unroll
+            for (int n = c; n < c + CH; ++n) {
+              const float m = warp_max(z[n]);
+              if (lane == n) reinterpret_cast<float*>(&rs.red[n])[warp & 3] = m;
+            }
           }
           named_bar_sync(bar, 128);
-          if (t < C) {
+          if (t < rr) {
             const float old = rs.m[t];
-            const float nm = fmaxf(fmaxf(rs.red[0][t], rs.red[1][t]), fmaxf(rs.red[2][t], rs.red[3][t]));
+            const float4 w = rs.red[t];
+            const float nm = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
             const float m = nm > old + SLACK ? nm + HEAD : old;
             rs.move[t] = m != old ? ex2_approx(old - m) : 1.f;
             rs.m[t] = m;
@@ -913,9 +919,12 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           }
           named_bar_sync(bar, 128);
 #pragma unroll
-          for (int n = 0; n < C; ++n) {
-            l[n] *= rs.move[n];
-            bias[n] = rs.bias[n];
+          for (int c = 0; c < C; c += CH) {
+            if (SKIP && c >= rr) continue;
+            const float4 mv = *reinterpret_cast<const float4*>(rs.move + c);
+            const float4 b4 = *reinterpret_cast<const float4*>(rs.bias + c);
+            l[c] *= mv.x, l[c + 1] *= mv.y, l[c + 2] *= mv.z, l[c + 3] *= mv.w;
+            bias[c] = b4.x, bias[c + 1] = b4.y, bias[c + 2] = b4.z, bias[c + 3] = b4.w;
           }
           if (filled) {  // this O's last P V must have retired
             const int jo = j - (TURNS ? 2 : 1);
@@ -993,7 +1002,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       // ---- end of the unit's part: join the threads' sums (and the groups', where they took turns),
       //      scale O and write it
       const float ls = warp_col_sums<C>(l, lane);
-      if (lane % (32 / C) == 0) rs.red[warp & 3][lane / (32 / C)] = ls;
+      if (lane % (32 / C) == 0) reinterpret_cast<float*>(&rs.red[lane / (32 / C)])[warp & 3] = ls;
       if (TURNS) named_bar_sync(5, NSM);
       else named_bar_sync(bar, 128);
       const bool whole = sg.first && sg.last;
@@ -1006,24 +1015,26 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         sm.join_hk = sg.hk;
       }
       if (t < C) {
-        float m = rs.m[t], sum = (rs.red[0][t] + rs.red[1][t]) + (rs.red[2][t] + rs.red[3][t]), f = 1.f;
+        const float4 w = rs.red[t];
+        float m = rs.m[t], sum = (w.x + w.y) + (w.z + w.w), f = 1.f;
         if (TURNS) {  // the other group's partial sums, reference and O
           const RowState& ro = sm.rs[grp ^ 1];
-          const float so = (ro.red[0][t] + ro.red[1][t]) + (ro.red[2][t] + ro.red[3][t]);
-          const float top = fmaxf(m, ro.m[t]);
+          const float4 wo = ro.red[t];
+          const float mo = ro.m[t], so = (wo.x + wo.y) + (wo.z + wo.w);
+          const float top = fmaxf(m, mo);
           f = ex2_approx(m - top);
           // the same order in both groups: they have to agree on the sum
-          const float mine = sum * f, other = so * ex2_approx(ro.m[t] - top);
+          const float mine = sum * f, other = so * ex2_approx(mo - top);
           sum = grp == 0 ? mine + other : other + mine;
           m = top;
         }
         // a NaN stays one; a row that may see nothing took part in the tiles that needed no mask
         const bool some = !(sum == 0.f) && rc.lo[c0 + t] <= rc.hi[c0 + t];
         rs.fin[t] = some ? f / sum * (ES == 1 ? 0x1p-8f : 1.f) : 0.f;  // (8-bit P is 2^8 times what the sum adds)
-        const float lse = some ? (m - LIFT + log2f(sum)) * kLn2 : -INFINITY;
+        const float lse = some ? (m - LIFT + lg2_approx(sum)) * kLn2 : -INFINITY;
         if (!*abort_flag && (!TURNS || grp == 0)) {
           if (!whole) a.part_lse[(int64_t)part * R + c0 + t] = lse;
-          else if (rc.orow[c0 + t] >= 0) a.lse[rc.lrow[c0 + t]] = lse;
+          else if (t < rr) a.lse[rc.lrow[c0 + t]] = lse;
         }
       }
       // the last P V of each O
@@ -1040,25 +1051,33 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         const int w0 = TURNS ? grp * (C / 2) : 0, w1 = min(TURNS ? w0 + C / 2 : C, rr);
         const RowState &r0 = sm.rs[TURNS ? 0 : grp], &r1 = sm.rs[1];
 #pragma unroll 1
-        for (int k = 0; k < S::NO * C / 4; ++k) {
-          const int db = k / (C / 4), n0 = (k % (C / 4)) * 4, d = db * 128 + t;
-          if (n0 < w0 || n0 >= w1) continue;
+        for (int n0 = w0; n0 < w1; n0 += 4)
+#pragma unroll 1
+        for (int db = 0; db < S::NO; ++db) {
+          const int d = db * 128 + t;
           const uint32_t at = t_lane + S::TM_O + db * N + c0 + n0;
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t x[2][4] = {}, y[2][4] = {};
+          if (has0) {
+            tmem_ld4(at, x[0]);
+            if constexpr (S::SIDE) tmem_ld4(at + 8, y[0]);
+          }
+          if (has1) {
+            tmem_ld4(at + S::ON, x[1]);
+            if constexpr (S::SIDE) tmem_ld4(at + S::ON + 8, y[1]);
+          }
+          tmem_ld_wait();
+          float v[4];
 #pragma unroll
           for (int g = 0; g < (TURNS ? 2 : 1); ++g) {
-            if (!(g ? has1 : has0)) continue;
-            uint32_t x[4], y[4];
-            tmem_ld4(at + g * S::ON, x);
-            if constexpr (S::SIDE) tmem_ld4(at + g * S::ON + 8, y);
-            tmem_ld_wait();
-            reg_pin(x);
-            if constexpr (S::SIDE) reg_pin(y);
+            reg_pin(x[g]);
+            if constexpr (S::SIDE) reg_pin(y[g]);
+            const float4 f4 = *reinterpret_cast<const float4*>((g ? r1 : r0).fin + n0);
+            const float f[4] = {f4.x, f4.y, f4.z, f4.w};
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-              float o = __uint_as_float(x[u]);
-              if constexpr (S::SIDE) o += __uint_as_float(y[u]);
-              v[u] = fmaf(o, (g ? r1 : r0).fin[n0 + u], v[u]);
+              float o = __uint_as_float(x[g][u]);
+              if constexpr (S::SIDE) o += __uint_as_float(y[g][u]);
+              v[u] = g ? fmaf(o, f[u], v[u]) : o * f[u];
             }
           }
           if (!good) continue;
@@ -1066,7 +1085,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           for (int u = 0; u < 4; ++u) {
             const int n = c0 + n0 + u;
             if (!whole) a.part_o[((int64_t)part * R + n) * D + d] = v[u];
-            else if (rc.orow[n] >= 0) reinterpret_cast<__nv_bfloat16*>(a.o.ptr)[rc.orow[n] + d] = __float2bfloat16_rn(v[u]);
+            else if (n0 + u < rr) reinterpret_cast<__nv_bfloat16*>(a.o.ptr)[rc.orow[n] + d] = __float2bfloat16_rn(v[u]);
           }
         }
       }
