@@ -40,9 +40,11 @@
 // Warps: softmax groups of four (thread = position of a tile; at the end = element of D), then one
 // that produces (lane = page of a tile), one that issues S, one that issues P V, and one that builds
 // the next unit's Q operand and row constants.  Up to 16 rows there are two groups that take the tiles
-// in turn, each with its own O, references and sums, joined when the unit ends: a tile's chain
-// (wait, TMEM read, vote, exponentials, store, fence) takes longer than its bytes take to arrive, so
-// two tiles have to be in work at once.  With more rows each group takes 16 of them.
+// in turn, each with its own O, references and sums: a tile's chain (wait, TMEM read, vote,
+// exponentials, store, fence) takes longer than its bytes take to arrive, so two tiles have to be in
+// work at once.  The group that took a unit's last tile joins and writes its two O, while the other
+// one, having posted its sums, is already in the next unit (O and sums are double-buffered for that).
+// With more rows each group takes 16 of them.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -111,8 +113,8 @@ struct Shape {
   static constexpr int PPART = N * kTile * ES, PBUF = PARTS * PPART;
   static constexpr int NO = D <= 128 ? 1 : D / 128; // blocks of 128 elements of O
   static constexpr int ON = NO * N;                 // TMEM columns of one O
-  static constexpr uint32_t TM_O = 2 * N;           // TMEM: two S buffers, then one O or one per group
-  static constexpr int USED = 2 * N + (TURNS ? 2 : 1) * ON;
+  static constexpr uint32_t TM_O = 2 * N;           // TMEM: two S buffers, then one O, or one per group and unit parity
+  static constexpr int USED = 2 * N + (TURNS ? 4 : 1) * ON;
   static constexpr uint32_t TM_COLS = USED <= 32 ? 32 : USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
   static_assert(USED <= 512 && N % 16 == 0 && N <= 256 && (ES == 1 || R >= 16), "operand shape");
 };
@@ -142,7 +144,11 @@ struct RowState {
   float m[16], bias[16];  // reference; lift - reference
   float move[16];         // factor of the last move
   float4 red[16];         // a value of each warp
-  float fin[16];          // factor of O at the end
+  float fin[2][16];       // factors of the O (of both groups) at the end
+};
+struct Posted {  // what a group knows of a unit when it leaves it
+  float m[16];
+  float4 sum[16];  // a part of each warp
 };
 // What one (sequence, row group) has to visit.
 struct Entry {
@@ -244,9 +250,10 @@ struct Walker {
 template <int R> struct Smem {
   RowConst<R> rc[2];
   RowState rs[R <= 16 ? 2 : R / 16];
+  Posted post[2][R <= 16 ? 2 : R / 16];  // by unit parity and group
   float2 scales[kScaleRing][8];  // (ks, vs) of a tile's pages; ks = -inf hides the page
   int odd[kScaleRing];           // the tile has a hidden page, or one of a scale below 2^-100
-  uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], fin_bar[2];
+  uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], posted[2], done[2], fin_bar[2];
   int scan[24];
   Start start;
   // the unit whose first part this CTA holds: how many parts it has (0: no such unit), the first one's
@@ -500,6 +507,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       mbar_init(sm.o_full + i, 1);
       mbar_init(sm.q_full + i, 1);
       mbar_init(sm.q_empty + i, 2 + 4 * NG);  // the S issuer's commit, the P V issuer and the softmax warps
+      mbar_init(sm.posted + i, 4);  // a group's warps: the one that does not write the unit
+      mbar_init(sm.done + i, 4);    // the other one's: the unit is written
       mbar_init(sm.fin_bar + i, 1);
     }
     sm.abort_flag = 0;
@@ -731,13 +740,15 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       const int nt = ok ? sm.rc[seg & 1].sg.nt : 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.q_empty + (seg & 1));
+      // the unit before last, which used the same O, has been written
+      if (TURNS && seg >= 2) ok = ok && wait_for_w(sm.done + (seg & 1), (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
       for (int it = 0; ok && it < nt; ++it, ++j) {
         ok = wait_for_w(sm.full + slot, phase, abort_flag) &&
              wait_for_w(sm.p_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag);
         if (!ok) break;
         tc_fence_after();
         const uint32_t acc0 = it >= (TURNS ? 2 : 1) ? 1u : 0u;  // the first tile that this O takes overwrites it
-        const uint32_t o = tmem + S::TM_O + (TURNS ? (j & 1) * S::ON : 0);
+        const uint32_t o = tmem + S::TM_O + (TURNS ? ((seg & 1) * 2 + (j & 1)) * S::ON : 0);
         const uint32_t pb = p_lo + (uint32_t)(((j & 1) * S::PBUF) >> 4);
 #pragma unroll
         for (int db = 0; db < S::NO; ++db) {
@@ -793,7 +804,6 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     RowState& rs = sm.rs[grp];
     const int c0 = TURNS ? 0 : grp * C;  // this thread's rows are [c0, c0 + C)
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_o = t_lane + S::TM_O + (TURNS ? grp * S::ON : c0);
     const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0, alibi = (a.score.flags & FA_SCORE_ALIBI) != 0;
     const float cap2 = capped ? a.score.softcap * kLog2e : 0.f, cap_k = capped ? 2.f * kLog2e / a.score.softcap : 0.f;
     const int my_page = t >> a.ps_log;
@@ -810,6 +820,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       named_bar_sync(6, NSM + 32);
     }
     int j = 0;
+    uint32_t posts = 0;  // parity of the next phase of the `posted` barriers, one bit each
 #pragma unroll 1
     for (int seg = 0; j < my_tiles; ++seg) {
       const RowConst<R>& rc = sm.rc[seg & 1];
@@ -820,9 +831,9 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       }
       // Inside a unit no wait leaves the loops: after a time-out every later wait returns at once and
       // nothing is written at the end.
-      // The threads that share barriers agree on whether the unit is known, so that they leave together.
+      // The threads of a group agree on whether the unit is known, so that they leave together.
       const bool lost = !wait_for(sm.q_full + (seg & 1), (uint32_t)((seg >> 1) & 1), abort_flag);
-      if (vote_or(TURNS ? 5 : bar, TURNS ? NSM : 128, lost)) {
+      if (vote_or(bar, 128, lost)) {
         *abort_flag = 1;
         break;
       }
@@ -836,7 +847,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         bias[n] = LIFT - kUnset;
       }
       bool filled = false;  // this group's O holds something of this unit
-      const int j0 = j;     // the unit's first tile
+      const uint32_t t_o = t_lane + S::TM_O + (TURNS ? ((seg & 1) * 2 + grp) * S::ON : c0);
       for (int it = 0; it < sg.nt; ++it, ++j) {
         if (TURNS && (j & 1) != grp) continue;
         const int p0 = (sg.t0 - it) * kTile, pos = p0 + t;
@@ -984,8 +995,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           // has landed.
           const int ld = 2 * j + 1, slot = ld % NS;
           if (!wait_for(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
-          const bool mine = TURNS || grp == 0;  // one group clears
-          if (mine && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sc.y >= 0x1p-100f)))) {
+          const bool clears = TURNS || grp == 0;  // one group does
+          if (clears && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sc.y >= 0x1p-100f)))) {
             unsigned char* v = base + (size_t)slot * S::SLOT + t * SW;
 #pragma unroll 1
             for (int p = 0; p < S::ROWB / SW; ++p)
@@ -1001,100 +1012,108 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       }
       // ---- end of the unit's part: join the threads' sums (and the groups', where they took turns),
       //      scale O and write it
-      const float ls = warp_col_sums<C>(l, lane);
-      if (lane % (32 / C) == 0) reinterpret_cast<float*>(&rs.red[lane / (32 / C)])[warp & 3] = ls;
-      if (TURNS) named_bar_sync(5, NSM);
-      else named_bar_sync(bar, 128);
-      const bool whole = sg.first && sg.last;
-      const int part = 2 * cta + (seg == 0 ? 0 : 1);
-      if (tid == 0 && sg.first && !sg.last) {  // the CTA's last unit, which goes on in the next CTAs
-        const int end = my_start + my_tiles - sg.nt + sg.entry_nt;
-        sm.join_parts = (end - 1) / per - cta + 1;
-        sm.join_slot = part;
-        sm.join_entry = sg.entry;
-        sm.join_hk = sg.hk;
-      }
-      if (t < C) {
-        const float4 w = rs.red[t];
-        float m = rs.m[t], sum = (w.x + w.y) + (w.z + w.w), f = 1.f;
-        if (TURNS) {  // the other group's partial sums, reference and O
-          const RowState& ro = sm.rs[grp ^ 1];
-          const float4 wo = ro.red[t];
-          const float mo = ro.m[t], so = (wo.x + wo.y) + (wo.z + wo.w);
-          const float top = fmaxf(m, mo);
-          f = ex2_approx(m - top);
-          // the same order in both groups: they have to agree on the sum
-          const float mine = sum * f, other = so * ex2_approx(mo - top);
-          sum = grp == 0 ? mine + other : other + mine;
-          m = top;
-        }
-        // a NaN stays one; a row that may see nothing took part in the tiles that needed no mask
-        const bool some = !(sum == 0.f) && rc.lo[c0 + t] <= rc.hi[c0 + t];
-        rs.fin[t] = some ? f / sum * (ES == 1 ? 0x1p-8f : 1.f) : 0.f;  // (8-bit P is 2^8 times what the sum adds)
-        const float lse = some ? (m - LIFT + lg2_approx(sum)) * kLn2 : -INFINITY;
-        if (!*abort_flag && (!TURNS || grp == 0)) {
-          if (!whole) a.part_lse[(int64_t)part * R + c0 + t] = lse;
-          else if (t < rr) a.lse[rc.lrow[c0 + t]] = lse;
+      Posted& mine = sm.post[seg & 1][grp];
+      const bool both = TURNS && sg.nt >= 2;               // the other group has tiles of this unit too
+      const bool writer = !TURNS || ((j - 1) & 1) == grp;  // this one has the last tile
+      if (writer || both) {
+        if (both && !writer && seg >= 2 &&  // what was posted two units ago has been read
+            !wait_for(sm.done + (seg & 1), (uint32_t)(((seg >> 1) - 1) & 1), abort_flag))
+          *abort_flag = 1;
+        const float ls = warp_col_sums<C>(l, lane);
+        if (lane % (32 / C) == 0) reinterpret_cast<float*>(&mine.sum[lane / (32 / C)])[warp & 3] = ls;
+        if (t < C) mine.m[t] = rs.m[t];
+        if (!writer) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sm.posted + (seg & 1));
         }
       }
-      // the last P V of each O
-      for (int k = max(j0, j - 2); k < j; ++k)
-        if (!wait_for(sm.o_full + (k & 1), (uint32_t)((k >> 1) & 1), abort_flag)) *abort_flag = 1;
-      tc_fence_after();
-      if (TURNS) named_bar_sync(5, NSM);
-      else named_bar_sync(bar, 128);
-      const bool good = !*abort_flag;
-      // which of the two O hold something
-      const bool has0 = !TURNS || j - j0 >= 2 || (j0 & 1) == 0, has1 = TURNS && (j - j0 >= 2 || (j0 & 1) == 1);
-      if (D >= 128 || (warp & 3) < 2) {
-        // rows [w0, w1) of this thread's c0.. are written by it; four at a time
-        const int w0 = TURNS ? grp * (C / 2) : 0, w1 = min(TURNS ? w0 + C / 2 : C, rr);
-        const RowState &r0 = sm.rs[TURNS ? 0 : grp], &r1 = sm.rs[1];
-#pragma unroll 1
-        for (int n0 = w0; n0 < w1; n0 += 4)
-#pragma unroll 1
-        for (int db = 0; db < S::NO; ++db) {
-          const int d = db * 128 + t;
-          const uint32_t at = t_lane + S::TM_O + db * N + c0 + n0;
-          uint32_t x[2][4] = {}, y[2][4] = {};
-          if (has0) {
-            tmem_ld4(at, x[0]);
-            if constexpr (S::SIDE) tmem_ld4(at + 8, y[0]);
+      if (writer) {
+        named_bar_sync(bar, 128);
+        if (both && !wait_for(sm.posted + (seg & 1), (posts >> (seg & 1)) & 1u, abort_flag)) *abort_flag = 1;
+        const bool whole = sg.first && sg.last;
+        const int part = 2 * cta + (seg == 0 ? 0 : 1);
+        if (t == 0 && (TURNS || grp == 0) && sg.first && !sg.last) {  // the CTA's last unit, which goes on in the next CTAs
+          const int end = my_start + my_tiles - sg.nt + sg.entry_nt;
+          sm.join_parts = (end - 1) / per - cta + 1;
+          sm.join_slot = part;
+          sm.join_entry = sg.entry;
+          sm.join_hk = sg.hk;
+        }
+        if (t < C) {
+          const float4 w = mine.sum[t];
+          float m = mine.m[t], sum = (w.x + w.y) + (w.z + w.w), f = 1.f, fo = 0.f;
+          if (both) {  // the other group's partial sums, reference and O
+            const Posted& other = sm.post[seg & 1][grp ^ 1];
+            const float4 wo = other.sum[t];
+            const float mo = other.m[t], so = (wo.x + wo.y) + (wo.z + wo.w), top = fmaxf(m, mo);
+            f = ex2_approx(m - top);
+            fo = ex2_approx(mo - top);
+            sum = sum * f + so * fo;
+            m = top;
           }
-          if (has1) {
-            tmem_ld4(at + S::ON, x[1]);
-            if constexpr (S::SIDE) tmem_ld4(at + S::ON + 8, y[1]);
+          // a NaN stays one; a row that may see nothing took part in the tiles that needed no mask
+          const bool some = !(sum == 0.f) && rc.lo[c0 + t] <= rc.hi[c0 + t];
+          const float inv = some ? (ES == 1 ? 0x1p-8f : 1.f) / sum : 0.f;  // (8-bit P is 2^8 times what the sum adds)
+          rs.fin[0][t] = f * inv;
+          rs.fin[1][t] = fo * inv;
+          const float lse = some ? (m - LIFT + lg2_approx(sum)) * kLn2 : -INFINITY;
+          if (!*abort_flag) {
+            if (!whole) a.part_lse[(int64_t)part * R + c0 + t] = lse;
+            else if (t < rr) a.lse[rc.lrow[c0 + t]] = lse;
           }
-          tmem_ld_wait();
-          float v[4];
+        }
+        // The last P V, and so all before it (one thread's MMAs end in order).
+        if (!wait_for(sm.o_full + ((j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag)) *abort_flag = 1;
+        tc_fence_after();
+        named_bar_sync(bar, 128);
+        const bool good = !*abort_flag;
+        if (D >= 128 || (warp & 3) < 2) {
+          const uint32_t t_other = t_lane + S::TM_O + ((seg & 1) * 2 + (grp ^ 1)) * S::ON;
+#pragma unroll 1
+          for (int n0 = 0; n0 < rr; n0 += 4)
+#pragma unroll 1
+            for (int db = 0; db < S::NO; ++db) {
+              const int d = db * 128 + t, at = db * N + n0;
+              uint32_t x[4], y[4] = {}, x2[4] = {}, y2[4] = {};
+              tmem_ld4(t_o + at, x);
+              if constexpr (S::SIDE) tmem_ld4(t_o + at + 8, y);
+              if (both) {
+                tmem_ld4(t_other + at, x2);
+                if constexpr (S::SIDE) tmem_ld4(t_other + at + 8, y2);
+              }
+              tmem_ld_wait();
+              reg_pin(x);
+              reg_pin(y);
+              reg_pin(x2);
+              reg_pin(y2);
+              if (!good) continue;
+              const float4 f4 = *reinterpret_cast<const float4*>(rs.fin[0] + n0), g4 = *reinterpret_cast<const float4*>(rs.fin[1] + n0);
+              const float f[4] = {f4.x, f4.y, f4.z, f4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w};
 #pragma unroll
-          for (int g = 0; g < (TURNS ? 2 : 1); ++g) {
-            reg_pin(x[g]);
-            if constexpr (S::SIDE) reg_pin(y[g]);
-            const float4 f4 = *reinterpret_cast<const float4*>((g ? r1 : r0).fin + n0);
-            const float f[4] = {f4.x, f4.y, f4.z, f4.w};
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              float o = __uint_as_float(x[g][u]);
-              if constexpr (S::SIDE) o += __uint_as_float(y[g][u]);
-              v[u] = g ? fmaf(o, f[u], v[u]) : o * f[u];
+              for (int u = 0; u < 4; ++u) {
+                const int n = c0 + n0 + u;
+                float v = __uint_as_float(x[u]), o = __uint_as_float(x2[u]);
+                if constexpr (S::SIDE) {
+                  v += __uint_as_float(y[u]);
+                  o += __uint_as_float(y2[u]);
+                }
+                v *= f[u];
+                if constexpr (TURNS) v = fmaf(o, g[u], v);
+                if (!whole) a.part_o[((int64_t)part * R + n) * D + d] = v;
+                else if (n0 + u < rr) reinterpret_cast<__nv_bfloat16*>(a.o.ptr)[rc.orow[n] + d] = __float2bfloat16_rn(v);
+              }
             }
-          }
-          if (!good) continue;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int n = c0 + n0 + u;
-            if (!whole) a.part_o[((int64_t)part * R + n) * D + d] = v[u];
-            else if (n0 + u < rr) reinterpret_cast<__nv_bfloat16*>(a.o.ptr)[rc.orow[n] + d] = __float2bfloat16_rn(v[u]);
-          }
         }
+        tc_fence_before();
       }
-      tc_fence_before();
+      if (both) posts ^= 1u << (seg & 1);
       __syncwarp();
-      if (lane == 0) mbar_arrive(sm.q_empty + (seg & 1));
-      // O may be overwritten, and the sums and references set anew, when all of its readers are here
-      if (TURNS) named_bar_sync(5, NSM);
-      else named_bar_sync(bar, 128);
+      if (lane == 0) {
+        if (TURNS && writer) mbar_arrive(sm.done + (seg & 1));
+        mbar_arrive(sm.q_empty + (seg & 1));
+      }
+      // The references are set anew when all of their readers are here.
+      named_bar_sync(bar, 128);
     }
     if (tid == 0 && *abort_flag) report_status(a.status, FA_ERR_TIMEOUT);
   }
