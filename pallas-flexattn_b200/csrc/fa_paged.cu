@@ -37,8 +37,8 @@
 // joins its parts in CTA order.  A second kernel for that took 5-6 us more on the device and 6 us
 // on the host; counters or flags in the workspace would have to be zero before the call.
 //
-// Warps: softmax groups of four (thread = position of a tile; at the end = element of D), then one
-// that produces (lane = page of a tile), one that issues S, one that issues P V, and one that builds
+// Warps: softmax groups of four (thread = position of a tile; at the end = element of D), then two
+// that produce K and V (lane = page of a tile), one that issues S, one that issues P V, and one that builds
 // the next unit's Q operand and row constants.  Up to 16 rows there are two groups that take the tiles
 // in turn, each with its own O, references and sums: a tile's chain (wait, TMEM read, vote,
 // exponentials, store, fence) takes longer than its bytes take to arrive, so two tiles have to be in
@@ -100,7 +100,8 @@ struct Shape {
   static constexpr bool TURNS = R <= 16;            // the softmax groups take tiles in turn, else 16 rows each
   static constexpr int NG = TURNS ? 2 : R / 16;     // softmax groups
   static constexpr int NSM = 128 * NG;              // softmax threads
-  static constexpr int NT = NSM + 128;
+  static constexpr int LOADERS = R == 8 ? 2 : 1;    // warps that produce: K and V, or both
+  static constexpr int NT = NSM + 32 * (LOADERS + 3);
   static constexpr int N = SIDE ? 16 : R;           // columns of S and O
   static constexpr int C = R < 16 ? R : 16;         // rows per softmax thread
   static constexpr int PARTS = ES == 1 && !SIDE ? 2 : 1;  // operands of Q and P (hi, lo)
@@ -270,13 +271,15 @@ size_t paged_smem_bytes(int slots) {
   return 1024 + (size_t)slots * S::SLOT + 2 * S::QBUF + 2 * S::PBUF + sizeof(Smem<R>);
 }
 
-// Bounded wait for a barrier's phase; false when the CTA gave up or after kSpins polls (some 0.1 s of
-// immediate answers, longer as the hardware lets a poll sleep: far above any legitimate wait here).  A
-// few instructions, since two dozen waits in line are what fills the instruction cache.
-constexpr int kSpins = 1 << 22;
+// Bounded wait for a barrier's phase; false when the CTA gave up or after kSpins polls: between 50 ms
+// (every poll answers at once) and some seconds (the hardware lets polls sleep), where the longest
+// legitimate wait of this kind is that of a tile or a unit's Q operand, microseconds.  Only the warp
+// that builds Q waits for whole units, with mbar_wait's bound on time.  No clock here: two dozen waits
+// in line fill the instruction cache, and the shorter one took 10 % off the windowed case.
+constexpr uint32_t kSpins = 1u << 20;
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
 #pragma unroll 1
-  for (int n = 0; n < kSpins; ++n) {
+  for (uint32_t n = 0; n < kSpins; ++n) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
   }
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
                       const PagedArgs a) {
   using S = Shape<D, ES, R>;
   constexpr int N = S::N, SW = S::SW, C = S::C, NG = S::NG, NSM = S::NSM, NT = S::NT;
-  constexpr int W_LOAD = 4 * NG, W_S = W_LOAD + 1, W_PV = W_LOAD + 2, W_Q = W_LOAD + 3;  // warps behind the softmax
+  constexpr int W_LOAD = 4 * NG, W_S = W_LOAD + S::LOADERS, W_PV = W_S + 1, W_Q = W_S + 2;  // warps behind the softmax
   constexpr bool TURNS = S::TURNS;
   constexpr uint32_t LAYOUT = SW == 128 ? SMEM_SWIZZLE_128B : SMEM_SWIZZLE_64B;
   constexpr int KPOS = 32 / ES;  // positions per PV MMA
@@ -587,10 +590,15 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
 
-  if (warp == W_LOAD) {
-    // ---------------------------------------------------------------- producer
+  if (warp >= W_LOAD && warp < W_S) {
+    // ---------------------------------------------------------------- producers
     // A batch of 32 pages (32 / pages-per-tile tiles): each lane holds the number and the scales of one
-    // page, and fetches the next batch's while this one's loads go out.
+    // page, and fetches the next batch's while this one's loads go out.  With two loaders K and V have a
+    // warp each: a lane's load takes some 100 cycles to issue.  (Where the softmax threads need more than
+    // 128 registers a thirteenth warp would make them spill, which costs more: the L1 cache that would
+    // hold what they spill is shared memory here.)
+    constexpr int STEP = S::LOADERS;  // loads from one of this warp's to the next (K of tile j: 2 j, V: 2 j + 1)
+    const int kv0 = STEP == 1 ? 0 : warp - W_LOAD;
     const int ppt_log = 7 - a.ps_log, ppt = 1 << ppt_log, batch = 32 >> ppt_log, sub = lane >> ppt_log, pg = lane & (ppt - 1);
     struct Page {
       int page, hk, active;
@@ -616,7 +624,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     auto fetch_scales = [&](Page& x) {
       x.ks = -INFINITY;
       x.vs = 1.f;
-      if (x.active && (unsigned)x.page < (unsigned)a.num_pages) {
+      if (kv0 == 0 && x.active && (unsigned)x.page < (unsigned)a.num_pages) {
         if constexpr (ES == 1) {
           x.ks = __ldg(a.k_scale + (int64_t)x.page * a.Hkv + x.hk);
           x.vs = __ldg(a.v_scale + (int64_t)x.page * a.Hkv + x.hk);
@@ -625,8 +633,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         }
       }
     };
-    int issued = 0, slot = 0;  // slots filled so far (K and V of a tile take one each); the next one
-    uint32_t phase = 1;        // parity of the empty barriers' phase that frees it (the first is free)
+    int issued = kv0, slot = kv0 % NS;  // load number and its slot
+    uint32_t phase = 1;               // parity of the empty barriers' phase that frees it (the first is free)
     Page x, y;
     wk.off += sub;
     fetch(x);
@@ -641,11 +649,10 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       const int n = min(batch, my_tiles - j0);
       const unsigned pages = (1u << ppt) - 1u;
       unsigned small = 0;
-      for (int k = 0; ok && k < n; ++k) {
-        const int ring = (j0 + k) % kScaleRing;
+      for (int k = 0; k < n; ++k) {
         const uint32_t bytes = ((uint32_t)__popc((act >> (k << ppt_log)) & pages) << a.ps_log) * S::ROWB;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
+        for (int kv = kv0; kv < 2; kv += STEP) {
           ok = wait_for_w(sm.empty + slot, phase, abort_flag);
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(sm.full + slot, bytes);
@@ -657,28 +664,40 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
               tma_load_4d(dst + p * S::PANEL, kv ? &tv : &tk, sm.full + slot, p * (SW / ES), 0, x.hk, page);
           }
           if (kv == 0) {
-            // This slot being free says that the tile whose scales lay here is done.  The scales are
-            // there before the slot's barrier can complete.
+            // The scales are there before the slot's barrier can complete.  Their place in the ring is
+            // free: the tile that used it lies further back than the ring of slots reaches.
+            const int ring = (j0 + k) % kScaleRing;
             if (ES == 1 && k == 0) small = __ballot_sync(0xffffffffu, x.active && !(x.vs >= 0x1p-100f));
             if (sub == k) sm.scales[ring][pg] = make_float2(x.ks, x.vs);
             if (lane == 0) sm.odd[ring] = (((hid | small) >> (k << ppt_log)) & pages) != 0;
             __syncwarp();
           }
           if (lane == 0) mbar_arrive(sm.full + slot);
-          ++issued;
-          if (++slot == NS) {
-            slot = 0;
+          issued += STEP;
+          slot += STEP;
+          if (slot >= NS) {
+            slot -= NS;
             phase ^= 1u;
           }
         }
+        if (!ok) break;
         if (k == 0) fetch_scales(y);
       }
       x = y;
     }
     if (!ok && lane == 0) *abort_flag = 1;
-    // every slot's latest load lands before the CTA may exit
-    for (int ld = max(0, issued - NS); ld < issued; ++ld)
-      wait_for_w(sm.full + ld % NS, (uint32_t)((ld / NS) & 1), never);
+    // Every slot's latest load lands before the CTA may exit: the last NS ones of both warps (an earlier
+    // one was consumed, and its barrier has moved on).  After an abort the counts of the two warps may
+    // differ, and a load that another one followed is not to be waited for: a few polls each instead.
+    const int end = 2 * my_tiles;
+    for (int ld = issued - STEP; ld >= 0 && ld >= (ok ? end : issued) - NS; ld -= STEP) {
+      if (ok) {
+        wait_for_w(sm.full + ld % NS, (uint32_t)((ld / NS) & 1), never);
+      } else {
+        for (int n = 0; n < 1000 && !mbar_try_wait(sm.full + ld % NS, (uint32_t)((ld / NS) & 1)); ++n) __nanosleep(1000);
+        __syncwarp();
+      }
+    }
   } else if (warp == W_S) {
     // ---------------------------------------------------------------- S issue
     // S(j) goes into buffer j & 1 once the softmax of j - 2 has read it (it has written P(j - 2)).
@@ -784,7 +803,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     bool ok = true;
     for (int seg = 0; ok && wk.next(a, &sg); ++seg) {
       const int buf = seg & 1;
-      if (seg >= 2) ok = wait_for_w(sm.q_empty + buf, (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
+      if (seg >= 2) ok = mbar_wait_w(sm.q_empty + buf, (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
       if (!ok) break;
       if (lane == 0) sm.rc[buf].sg = sg;
       if (seg == 0) {
@@ -809,7 +828,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     const int my_page = t >> a.ps_log;
     constexpr float LIFT = lift_of(ES), SLACK = slack_of(ES), HEAD = head_of(ES);
     constexpr int PW = 16 / ES;  // rows per 16-byte store of P
-    constexpr bool KEEP = NG < 4;
+    constexpr bool KEEP = TURNS;
     constexpr bool SKIP = TURNS;  // (elsewhere the branches cost more than the rows that they would spare)
     constexpr int CH = 4;        // rows worked on together; the ones behind the last real row are left out
     if (my_tiles > 0) {
@@ -839,7 +858,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       }
       const Seg sg = rc.sg;
       const int rr = min(sg.rows - c0, C);  // this thread's real rows
-      float l[C], xs[C], bias[C];  // (640 threads have no registers for the constants: read per tile)
+      float l[C], xs[C], bias[C];  // (where the threads have no registers for the constants: read per tile)
 #pragma unroll
       for (int n = 0; n < C; ++n) {
         l[n] = 0.f;
@@ -919,7 +938,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
             }
           }
           named_bar_sync(bar, 128);
-          if (t < rr) {
+          if (t < (SKIP ? (rr + CH - 1) & -CH : C)) {  // (rows worked on, real or not: an unset one would ask to move again)
             const float old = rs.m[t];
             const float4 w = rs.red[t];
             const float nm = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
