@@ -39,12 +39,12 @@
 //
 // Warps: softmax groups of four (thread = position of a tile; at the end = element of D), then two
 // that produce K and V (lane = page of a tile), one that issues S, one that issues P V, and one that builds
-// the next unit's Q operand and row constants.  Up to 16 rows there are two groups that take the tiles
-// in turn, each with its own O, references and sums: a tile's chain (wait, TMEM read, vote,
-// exponentials, store, fence) takes longer than its bytes take to arrive, so two tiles have to be in
-// work at once.  The group that took a unit's last tile joins and writes its two O, while the other
-// one, having posted its sums, is already in the next unit (O and sums are double-buffered for that).
-// With more rows each group takes 16 of them.
+// the next unit's Q operand and row constants.  A group works on up to 16 rows.  Up to 32 rows there
+// are two sets of groups that take the tiles in turn, each with its own O, references and sums: a
+// tile's chain (wait, TMEM read, vote, exponentials, store, fence) takes longer than its bytes take to
+// arrive, so two tiles have to be in work at once.  The set that took a unit's last tile joins and
+// writes its two O, while the other one, having posted its sums, is already in the next unit (O and
+// sums are double-buffered for that).  64 rows leave threads for one set only.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -97,8 +97,9 @@ struct PagedArgs {
 template <int D, int ES, int R>
 struct Shape {
   static constexpr bool SIDE = ES == 1 && R == 8;   // hi and lo parts side by side in N
-  static constexpr bool TURNS = R <= 16;            // the softmax groups take tiles in turn, else 16 rows each
-  static constexpr int NG = TURNS ? 2 : R / 16;     // softmax groups
+  static constexpr bool TURNS = R <= 32;            // two sets of softmax groups take the tiles in turn
+  static constexpr int H = R <= 16 ? 1 : R / 16;    // groups in a set, 16 rows (or all) each
+  static constexpr int NG = TURNS ? 2 * H : H;
   static constexpr int NSM = 128 * NG;              // softmax threads
   static constexpr int LOADERS = R == 8 ? 2 : 1;    // warps that produce: K and V, or both
   static constexpr int NT = NSM + 32 * (LOADERS + 3);
@@ -250,8 +251,8 @@ struct Walker {
 
 template <int R> struct Smem {
   RowConst<R> rc[2];
-  RowState rs[R <= 16 ? 2 : R / 16];
-  Posted post[2][R <= 16 ? 2 : R / 16];  // by unit parity and group
+  RowState rs[R <= 16 ? 2 : 4];
+  Posted post[2][R <= 16 ? 2 : 4];  // by unit parity and group
   float2 scales[kScaleRing][8];  // (ks, vs) of a tile's pages; ks = -inf hides the page
   int odd[kScaleRing];           // the tile has a hidden page, or one of a scale below 2^-100
   uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], posted[2], done[2], fin_bar[2];
@@ -506,12 +507,12 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(sm.s_full + i, 1);
-      mbar_init(sm.p_full + i, TURNS ? 4 : 4 * NG);
+      mbar_init(sm.p_full + i, 4 * S::H);
       mbar_init(sm.o_full + i, 1);
       mbar_init(sm.q_full + i, 1);
       mbar_init(sm.q_empty + i, 2 + 4 * NG);  // the S issuer's commit, the P V issuer and the softmax warps
-      mbar_init(sm.posted + i, 4);  // a group's warps: the one that does not write the unit
-      mbar_init(sm.done + i, 4);    // the other one's: the unit is written
+      mbar_init(sm.posted + i, 4 * S::H);  // a set's warps: the one that does not write the unit
+      mbar_init(sm.done + i, 4 * S::H);    // the other one's: the unit is written
       mbar_init(sm.fin_bar + i, 1);
     }
     sm.abort_flag = 0;
@@ -821,15 +822,16 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     // ---------------------------------------------------------------- softmax (thread = position)
     const int grp = warp >> 2, t = tid & 127, bar = 1 + grp;
     RowState& rs = sm.rs[grp];
-    const int c0 = TURNS ? 0 : grp * C;  // this thread's rows are [c0, c0 + C)
+    const int set = TURNS ? grp / S::H : 0, half = grp - set * S::H;
+    const int c0 = half * C;  // this thread's rows are [c0, c0 + C)
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const bool capped = (a.score.flags & FA_SCORE_SOFTCAP) != 0, alibi = (a.score.flags & FA_SCORE_ALIBI) != 0;
     const float cap2 = capped ? a.score.softcap * kLog2e : 0.f, cap_k = capped ? 2.f * kLog2e / a.score.softcap : 0.f;
     const int my_page = t >> a.ps_log;
     constexpr float LIFT = lift_of(ES), SLACK = slack_of(ES), HEAD = head_of(ES);
     constexpr int PW = 16 / ES;  // rows per 16-byte store of P
-    constexpr bool KEEP = TURNS;
-    constexpr bool SKIP = TURNS;  // (elsewhere the branches cost more than the rows that they would spare)
+    constexpr bool KEEP = R <= 16;
+    constexpr bool SKIP = R <= 16;  // (elsewhere the branches cost more than the rows that they would spare)
     constexpr int CH = 4;        // rows worked on together; the ones behind the last real row are left out
     if (my_tiles > 0) {
       build_rows<R>(a, sm.start.e, sm.start.hk, sm.rc[0], tid, NSM);
@@ -866,9 +868,9 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         bias[n] = LIFT - kUnset;
       }
       bool filled = false;  // this group's O holds something of this unit
-      const uint32_t t_o = t_lane + S::TM_O + (TURNS ? ((seg & 1) * 2 + grp) * S::ON : c0);
+      const uint32_t t_o = t_lane + S::TM_O + (TURNS ? ((seg & 1) * 2 + set) * S::ON : 0) + c0;
       for (int it = 0; it < sg.nt; ++it, ++j) {
-        if (TURNS && (j & 1) != grp) continue;
+        if (TURNS && (j & 1) != set) continue;
         const int p0 = (sg.t0 - it) * kTile, pos = p0 + t;
         if (!wait_for(sm.s_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag)) *abort_flag = 1;
         tc_fence_after();
@@ -1014,7 +1016,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           // has landed.
           const int ld = 2 * j + 1, slot = ld % NS;
           if (!wait_for(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
-          const bool clears = TURNS || grp == 0;  // one group does
+          const bool clears = half == 0;  // one group does
           if (clears && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sc.y >= 0x1p-100f)))) {
             unsigned char* v = base + (size_t)slot * S::SLOT + t * SW;
 #pragma unroll 1
@@ -1032,8 +1034,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       // ---- end of the unit's part: join the threads' sums (and the groups', where they took turns),
       //      scale O and write it
       Posted& mine = sm.post[seg & 1][grp];
-      const bool both = TURNS && sg.nt >= 2;               // the other group has tiles of this unit too
-      const bool writer = !TURNS || ((j - 1) & 1) == grp;  // this one has the last tile
+      const bool both = TURNS && sg.nt >= 2;               // the other set has tiles of this unit too
+      const bool writer = !TURNS || ((j - 1) & 1) == set;  // this one has the last tile
       if (writer || both) {
         if (both && !writer && seg >= 2 &&  // what was posted two units ago has been read
             !wait_for(sm.done + (seg & 1), (uint32_t)(((seg >> 1) - 1) & 1), abort_flag))
@@ -1051,7 +1053,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         if (both && !wait_for(sm.posted + (seg & 1), (posts >> (seg & 1)) & 1u, abort_flag)) *abort_flag = 1;
         const bool whole = sg.first && sg.last;
         const int part = 2 * cta + (seg == 0 ? 0 : 1);
-        if (t == 0 && (TURNS || grp == 0) && sg.first && !sg.last) {  // the CTA's last unit, which goes on in the next CTAs
+        if (t == 0 && half == 0 && sg.first && !sg.last) {  // the CTA's last unit, which goes on in the next CTAs
           const int end = my_start + my_tiles - sg.nt + sg.entry_nt;
           sm.join_parts = (end - 1) / per - cta + 1;
           sm.join_slot = part;
@@ -1061,8 +1063,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         if (t < C) {
           const float4 w = mine.sum[t];
           float m = mine.m[t], sum = (w.x + w.y) + (w.z + w.w), f = 1.f, fo = 0.f;
-          if (both) {  // the other group's partial sums, reference and O
-            const Posted& other = sm.post[seg & 1][grp ^ 1];
+          if (both) {  // the other set's partial sums, references and O
+            const Posted& other = sm.post[seg & 1][(set ^ 1) * S::H + half];
             const float4 wo = other.sum[t];
             const float mo = other.m[t], so = (wo.x + wo.y) + (wo.z + wo.w), top = fmaxf(m, mo);
             f = ex2_approx(m - top);
@@ -1087,7 +1089,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         named_bar_sync(bar, 128);
         const bool good = !*abort_flag;
         if (D >= 128 || (warp & 3) < 2) {
-          const uint32_t t_other = t_lane + S::TM_O + ((seg & 1) * 2 + (grp ^ 1)) * S::ON;
+          const uint32_t t_other = t_lane + S::TM_O + ((seg & 1) * 2 + (set ^ 1)) * S::ON + c0;
 #pragma unroll 1
           for (int n0 = 0; n0 < rr; n0 += 4)
 #pragma unroll 1
@@ -1224,20 +1226,24 @@ struct PagedPlan {
   size_t workspace;
 };
 
-// Rows per group: the smallest operand width that holds every query row of a K/V head, or 64
-// (32 for bf16 pages of head dim 256, whose tiles leave no room for more) with as many groups as
-// it takes, each reading the cache again.
+// Rows per group: the smallest operand width that holds every query row of a K/V head, or 64 with as
+// many groups as it takes, each reading the cache again.  32 instead of 64 where bf16 pages of head dim
+// 256 leave no room for more, and where the table's whole width makes at most eight tiles per SM: there
+// the latency of a unit counts, not the cache's bytes (40 rows at head dim 256, five users of 2777
+// positions: 27 against 34 us; 32 users of 8192: 93 against 78; a prompt chunk of 141 tiles per SM: 316
+// against 228).
 PagedPlan plan_paged(const FaPagedAttnParams* p) {
   PagedPlan pl;
   const bool f8 = p->cache.dtype == FA_DTYPE_E4M3;
+  const int sms = sm_count();
   const int64_t M = (int64_t)(p->H / p->cache.H_kv) * p->Tq;
-  const int top = !f8 && p->cache.D == 256 ? 32 : 64;
+  const int64_t tiles = (int64_t)p->B * p->cache.H_kv *
+                        (((int64_t)p->cache.table_cols * p->cache.page_size + kTile - 1) / kTile);  // of one row group
   pl.R = f8 ? 8 : 16;
-  while (pl.R < M && pl.R < top) pl.R *= 2;
+  while (pl.R < M && pl.R < 64) pl.R *= 2;
+  if (pl.R == 64 && ((!f8 && p->cache.D == 256) || tiles * ((M + 63) / 64) <= (int64_t)8 * sms)) pl.R = 32;
   pl.groups = (int)((M + pl.R - 1) / pl.R);
-  const int64_t tiles = (int64_t)p->B * pl.groups * p->cache.H_kv *
-                        (((int64_t)p->cache.table_cols * p->cache.page_size + kTile - 1) / kTile);
-  pl.ctas = (int)std::min<int64_t>(sm_count(), tiles);
+  pl.ctas = (int)std::min<int64_t>(sms, tiles * pl.groups);
   pl.workspace = (size_t)2 * pl.ctas * pl.R * (p->cache.D + 1) * 4 + 256;
   return pl;
 }

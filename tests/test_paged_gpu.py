@@ -104,6 +104,19 @@ def test_attention_matches_the_formula(name):
     check_attend(*attend_case(name))
 
 
+@pytest.mark.parametrize("name", ["r64_f8_d128", "r64_f8_d256", "groups_f8", "bf16_r64_d128", "bf16_r64_d64",
+                                  "window_groups", "groups_bf16_d256", "ragged_q", "long_and_short"])
+def test_wide_tables(name):
+    """Room for far longer sequences than there are: more query rows share a tile then, and nothing of the
+    columns behind the lengths is read."""
+    q, cache, table, lens, mod, kw, ref = attend_case(name)
+    wide = torch.full((table.shape[0], 5000), -3, dtype=torch.int32, device=DEV)
+    for b, n in enumerate(lens):
+        used = -(-n // cache.page_size)
+        wide[b, :used] = table[b, :used]
+    check_attend(q, cache, wide[:, :4999], lens, mod, kw, ref)
+
+
 @pytest.mark.parametrize("name", ["gqa4_t1_f8", "bf16_r16_d128", "r64_f8_d256"])
 def test_pages_stored_token_major(name):
     check_attend(*attend_case(name, layout="nhd"))
