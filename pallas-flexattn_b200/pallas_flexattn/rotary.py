@@ -198,12 +198,17 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, spec, positions, inverse):
         ctx.set_materialize_grads(False)
-        ctx.args = (spec, positions, inverse)
+        tensor = isinstance(positions, torch.Tensor)
+        if tensor:  # saved, so that a change in place before the backward pass is an error
+            ctx.save_for_backward(positions)
+        ctx.args = (spec, None if tensor else positions, inverse)
         return _launch(q, k, spec, positions, inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
         spec, positions, inverse = ctx.args
+        if ctx.saved_tensors:
+            positions, = ctx.saved_tensors
         if dq is None and dk is None:
             return None, None, None, None, None
         # linear, so its own gradient is the same operator turned back

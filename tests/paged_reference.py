@@ -111,6 +111,8 @@ def attend64(q, cache, table, lens, qlens, kind, window, slopes, cap, scale, hid
                 see = pos[None] <= qpos[:, None]
             if kind == "window":
                 see = see & (qpos[:, None] - pos[None] <= window)
+            if kind == "band":  # a window to both sides
+                see = (qpos[:, None] - pos[None] <= window[0]) & (pos[None] - qpos[:, None] <= window[1])
             see = see & ~gone[None]
             s = torch.einsum("gtd,nd->gtn", qq, kk) * scale
             # S: D exact products summed in fp32 (each addition off by 2^-23 of the terms' sum at most), an

@@ -229,6 +229,75 @@ def test_nan_in_one_query_stays_in_its_row():
         assert torch.isnan(o[hit]).all() and torch.equal(o[~hit], want[0][~hit]) and torch.equal(lse[~hit], want[1][~hit])
 
 
+@pytest.mark.parametrize("left,right", [(20, 3), (0, 0), (-1, 2), (1 << 30, 1 << 30), ((1 << 31) - 1, (1 << 31) - 1)])
+def test_windows_to_both_sides(left, right):
+    q, cache, table, lens, _, kw, _ = attend_case("ragged_q")
+    wl, wr = (1 << 40 if left < 0 else left), right
+    check_attend(q, cache, table, lens, pf.sliding_window_mask(left, right), kw,
+                 lambda: attend64(q, cache, table, lens, kw["q_lens"], "band", (wl, wr), None, 0, 1 / math.sqrt(64)))
+
+
+def test_thousands_of_sequences_most_of_them_empty():
+    """More sequences than threads, and more empty ones than a CTA's list of them holds."""
+    g = torch.Generator().manual_seed(2)
+    B, H, hkv, ps = 4000, 4, 4, 16
+    cache = make_cache(50, hkv, ps, 64, F8, g)
+    table = torch.randint(0, 50, (B, 2), generator=g).to(DEV, torch.int32)  # pages shared by sequences
+    lens = [0] * B
+    for i in range(0, B, 97):
+        lens[i] = 1 + i % 32
+    q = torch.randn(B, H, 1, 64, generator=g).to(DEV, BF16)
+    o, lse = pf.flash_attention_paged(q, cache, table, torch.tensor(lens, dtype=torch.int32, device=DEV), pf.causal_mask)
+    check_device_status(DEV)
+    some = [i for i in range(B) if lens[i]]
+    idx = torch.tensor(some, device=DEV)
+    ro, rl, to, tl = attend64(q[idx], cache, table[idx], [lens[i] for i in some], [1] * len(some), "causal", 0, None, 0,
+                              1 / math.sqrt(64))
+    assert_within("o", o[idx], ro, to)
+    assert_within("lse", lse[idx], rl, tl)
+    empty = torch.ones(B, dtype=torch.bool, device=DEV)
+    empty[idx] = False
+    assert torch.all(o[empty] == 0) and torch.all(lse[empty] == -math.inf)
+
+
+def test_many_heads_share_one_key_head():
+    g = torch.Generator().manual_seed(12)
+    for dtype in (F8, BF16):
+        cache = make_cache(12, 1, 64, 128, dtype, g)
+        table = make_table(2, 5, 12, g)
+        q = torch.randn(2, 128, 1, 128, generator=g).to(DEV, BF16)  # two row groups of 64, or four of 32
+        check_attend(q, cache, table, [300, 129], pf.causal_mask, {},
+                     lambda: attend64(q, cache, table, [300, 129], [1, 1], "causal", 0, None, 0, 1 / math.sqrt(128)))
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+def test_nan_that_a_row_sees_reaches_it(dtype):
+    """A NaN key makes every row that sees it NaN, a NaN value only its element of D."""
+    g = torch.Generator().manual_seed(6)
+    cache = make_cache(10, 2, 32, 64, dtype, g)
+    table = make_table(1, 8, 10, g)
+    q = torch.randn(1, 4, 1, 64, generator=g).to(DEV, BF16)
+    want = pf.flash_attention_paged(q, cache, table, [250], pf.causal_mask)
+    nan = torch.full((1,), math.nan, device=DEV).to(dtype)
+    page = int(table[0, 3])
+    cache.v[page, 1, 5, 7:8] = nan
+    o, lse = pf.flash_attention_paged(q, cache, table, [250], pf.causal_mask)
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[0, 2:, 0, 7] = True
+    assert torch.isnan(o[hit]).all() and torch.equal(o[~hit], want[0][~hit]) and torch.equal(lse, want[1])
+    cache.k[page, 0, 9, 0:1] = nan
+    o, lse = pf.flash_attention_paged(q, cache, table, [250], pf.causal_mask)
+    assert torch.isnan(o[0, :2]).all() and torch.isnan(lse[0, :2]).all() and torch.equal(lse[0, 2:], want[1][0, 2:])
+
+
+def test_other_device_is_not_needed_to_be_current_and_python_lists_work():
+    q, cache, table, lens, mod, kw, _ = attend_case("gqa4_t1_f8")
+    a = pf.flash_attention_paged(q, cache, table.long(), lens, mod, **kw)
+    b = pf.flash_attention_paged(q, cache, table.cpu(), torch.tensor(lens), mod, **kw)
+    c = pf.flash_attention_paged(q, cache, table, torch.tensor(lens, device=DEV, dtype=torch.int32), mod, **kw)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and all(torch.equal(x, y) for x, y in zip(a, c))
+
+
 def test_runs_are_bitwise_repeatable_and_streams_independent():
     q, cache, table, lens, mod, kw, _ = attend_case("long_and_short")
     want = pf.flash_attention_paged(q, cache, table, lens, mod, **kw)

@@ -118,6 +118,25 @@ def test_second_gradient_and_unused_outputs():
     assert_within("hv", hv, 2 * v.double(), torch.full_like(v, 64 * 2.0 ** -22 * float(v.abs().max())).double())
 
 
+def test_positions_changed_before_the_gradient_are_an_error():
+    spec = pf.rotary_spec(64)
+    q = torch.randn(1, 2, 4, 64, device=DEV, requires_grad=True)
+    pos = torch.arange(4, device=DEV, dtype=torch.int32)
+    r, _ = pf.rotary_embedding(q, None, spec, pos)
+    pos += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.sum().backward()
+
+
+def test_expanded_gradient():
+    spec = pf.rotary_spec(64, interleaved=True)
+    q = torch.randn(1, 2, 4, 64, device=DEV, requires_grad=True)
+    r, _ = pf.rotary_embedding(q, None, spec, 9)
+    r.sum().backward()
+    full = (torch.arange(4, device=DEV) + 9).expand(1, -1)
+    assert_within("dq", q.grad, *_ref(torch.ones_like(q), spec, full, inverse=True))
+
+
 def test_strided_broadcast_and_misaligned_inputs():
     spec = pf.rotary_spec(64, interleaved=True)
     base = torch.randn(2, 9, 6, 64, device=DEV).to(BF16)
