@@ -37,14 +37,20 @@
 // joins its parts in CTA order.  A second kernel for that took 5-6 us more on the device and 6 us
 // on the host; counters or flags in the workspace would have to be zero before the call.
 //
-// Warps: softmax groups of four (thread = position of a tile; at the end = element of D), then two
-// that produce K and V (lane = page of a tile), one that issues S, one that issues P V, and one that builds
+// Warps: softmax groups of four (thread = position of a tile; at the end = element of D), then one or
+// two that produce K and V (lane = page of a tile), one that issues S, one that issues P V, and one that builds
 // the next unit's Q operand and row constants.  A group works on up to 16 rows.  Up to 32 rows there
 // are two sets of groups that take the tiles in turn, each with its own O, references and sums: a
 // tile's chain (wait, TMEM read, vote, exponentials, store, fence) takes longer than its bytes take to
 // arrive, so two tiles have to be in work at once.  The set that took a unit's last tile joins and
 // writes its two O, while the other one, having posted its sums, is already in the next unit (O and
 // sums are double-buffered for that).  64 rows leave threads for one set only.
+//
+// Measured on the device (8-bit pages, H 32, H_kv 8, D 128, ragged lengths): 64 users of up to 4096
+// positions, one token each: 74 us, 5.4 TB/s, 0.83 of the measured copy rate; eight of up to 32768: 72 us,
+// 5.6 TB/s; one of 1000: 9.4 us, the launch, one tile's chain and the join.  Chunks of 512 tokens of four
+// users on up to 4096 positions: 228 us, bound by the chain of one set of softmax groups at 64 rows.
+// bf16, H 16, D 64, window 1024, ALiBi, 32 users: 45 us.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_bf16.h>

@@ -2,8 +2,9 @@
 
 Same public names as the reference package (src/pallas_flexattn/__init__.py);
 the compute runs in libflexattn.so (hand-written sm_100a CUDA).  Extensions:
-score_mod functors, composable mask_mods, GPU-built block tables and measured
-autotuning.
+score_mod functors, composable mask_mods, GPU-built block tables, measured
+autotuning, and the serving side: decode against a contiguous cache, rotary
+positions, and paged caches (bf16 or 8-bit) with their appends and attention.
 """
 from .flash_attn import (
     check_device_status,
