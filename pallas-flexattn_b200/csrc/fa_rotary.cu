@@ -9,8 +9,9 @@
 //
 // Measured (bf16, D 128, 32 + 8 heads): rotation of 2 x 8192 tokens with its gradient 117 us,
 // 5.7 TB/s; one token each of 64 sequences 2.3 us, the launch.  Append of eight prompts of up to
-// 2048 tokens to 8-bit pages with q's rotation 70 us, 3.1 TB/s: issue-bound, a key is turned twice
-// and rounded, and a page's 8 KB are one team's work; one token each of 64 sequences 4.1 us.
+// 2048 tokens to 8-bit pages with q's rotation (padding rows become zeros) 69 us, of which q takes
+// half at 4.8 TB/s; the rest is a team's chain (lengths, rows, largest magnitude, store: some 4 us with
+// 16 KB on their way, and six teams an SM).  One token each of 64 sequences 4.4 us.
 //
 // A thread owns a unit of 16 elements of a row: 8 + 8 elements rotary_dim / 2 apart for the half
 // layout, 16 neighbours for interleaved pairs and for the copied tail.  It computes the 8 cosines
@@ -126,7 +127,7 @@ __device__ __forceinline__ uint64_t both(float x) { return pack2(x, x); }
 // where the special-function unit's error puts more of them on the wrong side of a border (68 of 16 M
 // codes against 15; cosines and sines rounded from 64 bits: 12).  The angle is reduced to the nearest
 // quarter turn, exactly; then the Taylor series of |y| <= pi / 4, whose first terms left out are
-// y^11 / 11! = 2^-29 and y^10 / 10! = 2^-25.  Eight prompts of 2048 tokens: 70 us, 67 with that unit, 78
+// y^11 / 11! = 2^-29 and y^10 / 10! = 2^-25.  It cost 3 us in 70 for eight prompts of 2048 tokens, 11
 // without the packed instructions.
 __device__ __forceinline__ void pair_turns(const FaRotarySpec& r, int i, uint32_t pos, float* c, float* s) {
   uint32_t quarter[2];
@@ -337,13 +338,14 @@ __device__ __forceinline__ float page_scale(float top) {
 
 // One team (a warp, or the block) takes the rows of one (sequence, touched page, K/V head) of K
 // or of V.  Its new rows stay in registers as they lie in memory between the search for the largest
-// magnitude and the store (a key is turned twice, which costs less than the registers of its fp32
-// values: half as many teams would share an SM), so they are read once; teams share nothing, and no
-// atomic decides a value.  The page's number and its scale are fetched behind the rows' loads.
+// magnitude and the store, so they are read once; teams share nothing, and no atomic decides a value.
+// A key's turned values, fp32, wait in shared memory, where each thread reads what it wrote itself (in
+// registers, half as many teams would share an SM; turned twice, eight prompts with as many heads of q as
+// of K took 45 us, now 38; a warp's team, of few rows, turns them twice).  The page's number and its scale are fetched behind the rows' loads.
 constexpr int kAppendPasses = 4;  // row groups a team holds: 4 x 16 values a thread
 
 template <typename T, bool E4M3, bool WARP>
-__device__ __forceinline__ void append_team(const AppendArgs& a, int team, int tid, int nt, float* red) {
+__device__ __forceinline__ void append_team(const AppendArgs& a, int team, int tid, int nt, float* red, float4* stash) {
   const int which = team & 1, hk = (team >> 1) % a.Hkv, bp = (team >> 1) / a.Hkv;
   const int b = bp / a.pages_per_seq;
   int start, len;
@@ -417,6 +419,15 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
       if (row_in < rows_at_once && row < r1) {
         float g0[8], g1[8];
         values(p, g0, g1);
+        if constexpr (!WARP) {
+          if (rot) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+              stash[(4 * p + j / 4) * nt + tid] = make_float4(g0[j], g0[j + 1], g0[j + 2], g0[j + 3]);
+              stash[(4 * p + 2 + j / 4) * nt + tid] = make_float4(g1[j], g1[j + 1], g1[j + 2], g1[j + 3]);
+            }
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float m0 = fabsf(g0[j]), m1 = fabsf(g1[j]);
@@ -459,7 +470,16 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
       const int row = r0 + p * rows_at_once + row_in;
       if (row_in < rows_at_once && row < r1) {
         float g0[8], g1[8];
-        values(p, g0, g1);
+        if (WARP || !rot) {
+          values(p, g0, g1);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            const float4 w0 = stash[(4 * p + j / 4) * nt + tid], w1 = stash[(4 * p + 2 + j / 4) * nt + tid];
+            g0[j] = w0.x, g0[j + 1] = w0.y, g0[j + 2] = w0.z, g0[j + 3] = w0.w;
+            g1[j] = w1.x, g1[j + 1] = w1.y, g1[j + 2] = w1.z, g1[j + 3] = w1.w;
+          }
+        }
         uint8_t* d = dst + (int64_t)row * cache.stride_t;
         *reinterpret_cast<uint2*>(d + e0) = to_e4m3x8(g0, inv);
         *reinterpret_cast<uint2*>(d + e1) = to_e4m3x8(g1, inv);
@@ -475,14 +495,15 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
 template <typename T, bool E4M3, bool WARP, int NT>
 __global__ void __launch_bounds__(NT, NT == 512 || sizeof(T) == 4 ? 512 / NT : 768 / NT) append_kernel(const AppendArgs a) {
   __shared__ float red[16];
+  extern __shared__ float4 stash[];  // blocks that append 8-bit rows: 4 x kAppendPasses a thread
   const int before = (int)((int64_t)blockIdx.x * a.kv_blocks / gridDim.x);  // appending blocks before this one
   if ((int)((int64_t)(blockIdx.x + 1) * a.kv_blocks / gridDim.x) > before) {
     const int teams = a.B * a.pages_per_seq * a.Hkv * 2;
     if constexpr (WARP) {
       const int team = before * 4 + (threadIdx.x >> 5);
-      if (team < teams) append_team<T, E4M3, true>(a, team, threadIdx.x & 31, 32, red);
+      if (team < teams) append_team<T, E4M3, true>(a, team, threadIdx.x & 31, 32, red, stash);
     } else {
-      append_team<T, E4M3, false>(a, before, threadIdx.x, blockDim.x, red);
+      append_team<T, E4M3, false>(a, before, threadIdx.x, blockDim.x, red, stash);
     }
     return;
   }
@@ -588,9 +609,17 @@ cudaError_t launch_append(AppendArgs& a, cudaStream_t stream) {
     qb = a.q_blocks * ((a.H + a.heads_per_thread - 1) / a.heads_per_thread);
   }
   const unsigned grid = (unsigned)(a.kv_blocks + qb);
-  if (warp) append_kernel<T, E4M3, true, 128><<<grid, nt, 0, stream>>>(a);
-  else if (nt <= 256) append_kernel<T, E4M3, false, 256><<<grid, nt, 0, stream>>>(a);
-  else append_kernel<T, E4M3, false, 512><<<grid, nt, 0, stream>>>(a);
+  if (warp) {
+    append_kernel<T, E4M3, true, 128><<<grid, nt, 0, stream>>>(a);
+    return cudaGetLastError();
+  }
+  const auto kernel = nt <= 256 ? append_kernel<T, E4M3, false, 256> : append_kernel<T, E4M3, false, 512>;
+  const size_t smem = E4M3 && a.r.rotary_dim ? (size_t)nt * kAppendPasses * 4 * sizeof(float4) : 0;  // up to 128 KB
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<grid, nt, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
