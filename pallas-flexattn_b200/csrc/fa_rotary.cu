@@ -9,9 +9,9 @@
 //
 // Measured (bf16, D 128, 32 + 8 heads): rotation of 2 x 8192 tokens with its gradient 117 us,
 // 5.7 TB/s; one token each of 64 sequences 2.3 us, the launch.  Append of eight prompts of up to
-// 2048 tokens to 8-bit pages with q's rotation (padding rows become zeros) 69 us, of which q takes
+// 2048 tokens to 8-bit pages with q's rotation (padding rows become zeros) 68 us, of which q takes
 // half at 4.8 TB/s; the rest is a team's chain (lengths, rows, largest magnitude, store: some 4 us with
-// 16 KB on their way, and six teams an SM).  One token each of 64 sequences 4.4 us.
+// 16 KB on their way, and six teams an SM).  One token each of 64 sequences 4.3 us.
 //
 // A thread owns a unit of 16 elements of a row: 8 + 8 elements rotary_dim / 2 apart for the half
 // layout, 16 neighbours for interleaved pairs and for the copied tail.  It computes the 8 cosines
@@ -130,14 +130,14 @@ __device__ __forceinline__ uint64_t both(float x) { return pack2(x, x); }
 // y^11 / 11! = 2^-29 and y^10 / 10! = 2^-25.  It cost 3 us in 70 for eight prompts of 2048 tokens, 11
 // without the packed instructions.
 __device__ __forceinline__ void pair_turns(const FaRotarySpec& r, int i, uint32_t pos, float* c, float* s) {
-  uint32_t quarter[2];
+  uint32_t w[2];  // phase + 1/8: its two upper bits are the quarter, the others the angle from its middle
   float yf[2], snf[2], csf[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const uint64_t turns = __ldg(r.turns + i + k);
     const uint32_t phase = __umulhi(pos, (uint32_t)turns) + pos * (uint32_t)(turns >> 32);
-    quarter[k] = (phase + 0x20000000u) >> 30;
-    yf[k] = (float)(int32_t)(phase - (quarter[k] << 30)) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+    w[k] = phase + 0x20000000u;
+    yf[k] = (float)((int32_t)(w[k] & 0x3fffffffu) - 0x20000000) * 1.4629180792671596e-9f;  // 2 pi / 2^32
   }
   const uint64_t y = pack2(yf[0], yf[1]), z = mul2(y, y);
   uint64_t sn = fma2(z, both(1.f / 362880), both(-1.f / 5040)), cs = fma2(z, both(1.f / 40320), both(-1.f / 720));
@@ -151,9 +151,9 @@ __device__ __forceinline__ void pair_turns(const FaRotarySpec& r, int i, uint32_
   unpack2(cs, &csf[0], &csf[1]);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const bool odd = quarter[k] & 1;  // the quarters' signs: - in 1 and 2 for the cosine, in 2 and 3 for the sine
-    c[k] = __uint_as_float(__float_as_uint(odd ? snf[k] : csf[k]) ^ ((quarter[k] + 1) & 2) << 30);
-    s[k] = __uint_as_float(__float_as_uint(odd ? csf[k] : snf[k]) ^ (quarter[k] & 2) << 30);
+    const bool odd = w[k] & 0x40000000u;  // negative: the cosine in quarters 1 and 2, the sine in 2 and 3
+    c[k] = __uint_as_float(__float_as_uint(odd ? snf[k] : csf[k]) ^ ((w[k] + 0x40000000u) & 0x80000000u));
+    s[k] = __uint_as_float(__float_as_uint(odd ? csf[k] : snf[k]) ^ (w[k] & 0x80000000u));
   }
 }
 
@@ -341,11 +341,12 @@ __device__ __forceinline__ float page_scale(float top) {
 // magnitude and the store, so they are read once; teams share nothing, and no atomic decides a value.
 // A key's turned values, fp32, wait in shared memory, where each thread reads what it wrote itself (in
 // registers, half as many teams would share an SM; turned twice, eight prompts with as many heads of q as
-// of K took 45 us, now 38; a warp's team, of few rows, turns them twice).  The page's number and its scale are fetched behind the rows' loads.
+// of K took 45 us, now 37; a warp's team, of few rows, turns them twice).  The page's number and its
+// scale are fetched behind the rows' loads.
 constexpr int kAppendPasses = 4;  // row groups a team holds: 4 x 16 values a thread
 
 template <typename T, bool E4M3, bool WARP>
-__device__ __forceinline__ void append_team(const AppendArgs& a, int team, int tid, int nt, float* red, float4* stash) {
+__device__ __forceinline__ void append_team(const AppendArgs& a, int team, int tid, int nt, int* red, float4* stash) {
   const int which = team & 1, hk = (team >> 1) % a.Hkv, bp = (team >> 1) / a.Hkv;
   const int b = bp / a.pages_per_seq;
   int start, len;
@@ -412,11 +413,24 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
       }
     }
   } else {
-    float top = 0.f;
+    // The largest finite magnitude, as integers: fp32 or bf16 bits without the sign, plus one step of the
+    // exponent, which makes infinities and NaN negative.
+    constexpr int kStep = 0x00800000;
+    int most = kStep;
+    uint32_t most2 = 0x00800080u;  // bf16 values that are not turned: two at once
 #pragma unroll
     for (int p = 0; p < kAppendPasses; ++p) {
       const int row = r0 + p * rows_at_once + row_in;
       if (row_in < rows_at_once && row < r1) {
+        if (sizeof(T) == 2 && !rot) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[p][i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most2 = __viaddmax_s16x2(w[j] & 0x7fff7fffu, 0x00800080u, most2);
+          }
+          continue;
+        }
         float g0[8], g1[8];
         values(p, g0, g1);
         if constexpr (!WARP) {
@@ -430,21 +444,21 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float m0 = fabsf(g0[j]), m1 = fabsf(g1[j]);
-          top = fmaxf(top, m0 < INFINITY ? m0 : 0.f);  // NaN and infinities do not set the scale
-          top = fmaxf(top, m1 < INFINITY ? m1 : 0.f);
+          most = __viaddmax_s32(__float_as_int(g0[j]) & 0x7fffffff, kStep, most);
+          most = __viaddmax_s32(__float_as_int(g1[j]) & 0x7fffffff, kStep, most);
         }
       }
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    most = max(most, max((int)(most2 << 16), (int)(most2 & 0xffff0000u)));
+    most = __reduce_max_sync(0xffffffffu, most);
     if constexpr (!WARP) {
-      if ((tid & 31) == 0) red[tid >> 5] = top;
+      if ((tid & 31) == 0) red[tid >> 5] = most;
       __syncthreads();
-      for (int w = 0; w < nt / 32; ++w) top = fmaxf(top, red[w]);
+      for (int w = 0; w < nt / 32; ++w) most = max(most, red[w]);
     } else {
       __syncwarp();
     }
+    const float top = __int_as_float(most - kStep);
     float s = page_scale(top);
     if (r0 > 0) s = fmaxf(s, was);  // rows of the sequence are held: the scale only grows
     uint8_t* dst = reinterpret_cast<uint8_t*>(cache.ptr) + base;
@@ -494,7 +508,7 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
 // NT: the most threads a block may have.
 template <typename T, bool E4M3, bool WARP, int NT>
 __global__ void __launch_bounds__(NT, NT == 512 || sizeof(T) == 4 ? 512 / NT : 768 / NT) append_kernel(const AppendArgs a) {
-  __shared__ float red[16];
+  __shared__ int red[16];
   extern __shared__ float4 stash[];  // blocks that append 8-bit rows: 4 x kAppendPasses a thread
   const int before = (int)((int64_t)blockIdx.x * a.kv_blocks / gridDim.x);  // appending blocks before this one
   if ((int)((int64_t)(blockIdx.x + 1) * a.kv_blocks / gridDim.x) > before) {

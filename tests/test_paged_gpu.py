@@ -327,6 +327,9 @@ APPEND = {
     "prompt_f8": (3, 8, 2, 300, 128, BF16, F8, 64, 128, False, [0, 77, 64], [300, 123, 299]),
     "prompt_bf16_part": (2, 3, 3, 131, 64, BF16, BF16, 16, 32, True, [9, 0], [131, 64]),
     "prompt_fp32_d256": (2, 2, 1, 150, 256, F32, F8, 128, 64, False, [100, 3], None),
+    "prompt_d256": (2, 2, 1, 150, 256, BF16, F8, 128, 256, True, [100, 3], None),
+    "prompt_large_pages": (2, 2, 2, 200, 128, BF16, F8, 128, 128, False, [60, 0], [200, 129]),
+    "far_f8": (1, 2, 1, 70, 128, BF16, F8, 128, 128, False, [200001], None),
     "fp32_into_bf16": (1, 2, 2, 40, 128, F32, BF16, 32, 128, True, [30], None),
     "no_rotary": (2, 2, 1, 50, 128, BF16, F8, 16, 0, False, [7, 0], None),
     "small_pages_d64": (2, 1, 1, 100, 64, BF16, F8, 16, 64, False, [3, 16], [100, 1]),
