@@ -9,9 +9,9 @@
 //
 // Measured (bf16, D 128, 32 + 8 heads): rotation of 2 x 8192 tokens with its gradient 117 us,
 // 5.7 TB/s; one token each of 64 sequences 2.3 us, the launch.  Append of eight prompts of up to
-// 2048 tokens to 8-bit pages with q's rotation (padding rows become zeros) 68 us, of which q takes
-// half at 4.8 TB/s; the rest is a team's chain (lengths, rows, largest magnitude, store: some 4 us with
-// 16 KB on their way, and six teams an SM).  One token each of 64 sequences 4.3 us.
+// 2048 tokens to 8-bit pages with q's rotation 62 us (3.5 TB/s, the zeros of q's padding rows left out;
+// 36 us with 8 + 8 heads): a team's chain of lengths, rows, largest magnitude and stores takes some 4 us.
+// One token each of 64 sequences 4.0 us.
 //
 // A thread owns a unit of 16 elements of a row: 8 + 8 elements rotary_dim / 2 apart for the half
 // layout, 16 neighbours for interleaved pairs and for the copied tail.  It computes the 8 cosines
@@ -343,9 +343,8 @@ __device__ __forceinline__ float page_scale(float top) {
 // registers, half as many teams would share an SM; turned twice, eight prompts with as many heads of q as
 // of K took 45 us, now 37; a warp's team, of few rows, turns them twice).  The page's number and its
 // scale are fetched behind the rows' loads.
-constexpr int kAppendPasses = 4;  // row groups a team holds: 4 x 16 values a thread
-
-template <typename T, bool E4M3, bool WARP>
+// PASSES: row groups that a team holds, 16 values a thread each.
+template <typename T, bool E4M3, bool WARP, int PASSES>
 __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int tid, int nt, int* red, float4* stash) {
   const int which = team & 1, hk = (team >> 1) % a.Hkv, bp = (team >> 1) / a.Hkv;
   const int b = bp / a.pages_per_seq;
@@ -364,9 +363,9 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
   const FaTensor& cache = which ? a.vc : a.kc;
   const T* src = reinterpret_cast<const T*>(x.ptr) + (int64_t)b * x.stride_b + (int64_t)hk * x.stride_h;
 
-  typename Io<T>::Raw raw[kAppendPasses][2];
+  typename Io<T>::Raw raw[PASSES][2];
 #pragma unroll
-  for (int p = 0; p < kAppendPasses; ++p) {
+  for (int p = 0; p < PASSES; ++p) {
     const int row = r0 + p * rows_at_once + row_in;
     if (row_in < rows_at_once && row < r1) {
       const T* s = src + (int64_t)(first + row - start) * x.stride_t;
@@ -403,7 +402,7 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
   if constexpr (!E4M3) {
     __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(cache.ptr) + base;
 #pragma unroll
-    for (int p = 0; p < kAppendPasses; ++p) {
+    for (int p = 0; p < PASSES; ++p) {
       const int row = r0 + p * rows_at_once + row_in;
       if (row_in < rows_at_once && row < r1) {
         float g0[8], g1[8];
@@ -419,7 +418,7 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
     int most = kStep;
     uint32_t most2 = 0x00800080u;  // bf16 values that are not turned: two at once
 #pragma unroll
-    for (int p = 0; p < kAppendPasses; ++p) {
+    for (int p = 0; p < PASSES; ++p) {
       const int row = r0 + p * rows_at_once + row_in;
       if (row_in < rows_at_once && row < r1) {
         if (sizeof(T) == 2 && !rot) {
@@ -480,7 +479,7 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
     }
     const float inv = 1.f / s;
 #pragma unroll
-    for (int p = 0; p < kAppendPasses; ++p) {
+    for (int p = 0; p < PASSES; ++p) {
       const int row = r0 + p * rows_at_once + row_in;
       if (row_in < rows_at_once && row < r1) {
         float g0[8], g1[8];
@@ -506,18 +505,18 @@ __device__ __forceinline__ void append_team(const AppendArgs& a, int team, int t
 // kv_blocks blocks append and the rest rotate q, spread evenly over the grid: appends wait for memory
 // most of the time, and q's stream of loads and stores fills it.
 // NT: the most threads a block may have.
-template <typename T, bool E4M3, bool WARP, int NT>
-__global__ void __launch_bounds__(NT, NT == 512 || sizeof(T) == 4 ? 512 / NT : 768 / NT) append_kernel(const AppendArgs a) {
+template <typename T, bool E4M3, bool WARP, int PASSES, int NT>
+__global__ void __launch_bounds__(NT, (NT == 512 || sizeof(T) == 4 ? 512 : PASSES == 4 ? 768 : 1024) / NT) append_kernel(const AppendArgs a) {
   __shared__ int red[16];
-  extern __shared__ float4 stash[];  // blocks that append 8-bit rows: 4 x kAppendPasses a thread
+  extern __shared__ float4 stash[];  // blocks that append 8-bit rows: 4 x PASSES a thread
   const int before = (int)((int64_t)blockIdx.x * a.kv_blocks / gridDim.x);  // appending blocks before this one
   if ((int)((int64_t)(blockIdx.x + 1) * a.kv_blocks / gridDim.x) > before) {
     const int teams = a.B * a.pages_per_seq * a.Hkv * 2;
     if constexpr (WARP) {
       const int team = before * 4 + (threadIdx.x >> 5);
-      if (team < teams) append_team<T, E4M3, true>(a, team, threadIdx.x & 31, 32, red, stash);
+      if (team < teams) append_team<T, E4M3, true, PASSES>(a, team, threadIdx.x & 31, 32, red, stash);
     } else {
-      append_team<T, E4M3, false>(a, before, threadIdx.x, blockDim.x, red, stash);
+      append_team<T, E4M3, false, PASSES>(a, before, threadIdx.x, blockDim.x, red, stash);
     }
     return;
   }
@@ -611,9 +610,13 @@ template <typename T, bool E4M3>
 cudaError_t launch_append(AppendArgs& a, cudaStream_t stream) {
   const int64_t teams = (int64_t)a.B * a.pages_per_seq * a.Hkv * 2;
   const int rows = std::min(a.T, a.ps);
-  // A team is a warp when the rows that one page can take fit its registers, else a block.
-  const bool warp = rows * a.units <= 32 * kAppendPasses;
-  const int nt = warp ? 128 : std::max(64, a.ps * a.units / kAppendPasses);
+  // Two passes where 256 threads then hold a page's rows, else four: with two, 64 registers a thread let a
+  // third more threads share an SM (pages of 64 rows of 128: 62 against 68 us, 16 rows: 62 against 73; but
+  // 512 threads in two passes for 64 rows of 256: 130 against 126).  A team is a warp when the rows that one
+  // page can take fit its registers, else a block.
+  const int passes = a.ps * a.units <= 512 ? 2 : 4;
+  const bool warp = rows * a.units <= 64;
+  const int nt = warp ? 128 : std::max(64, a.ps * a.units / passes);
   a.kv_blocks = (int)(warp ? (teams + 3) / 4 : teams);
   int qb = 0;
   if (a.H > 0) {
@@ -624,11 +627,13 @@ cudaError_t launch_append(AppendArgs& a, cudaStream_t stream) {
   }
   const unsigned grid = (unsigned)(a.kv_blocks + qb);
   if (warp) {
-    append_kernel<T, E4M3, true, 128><<<grid, nt, 0, stream>>>(a);
+    append_kernel<T, E4M3, true, 2, 128><<<grid, nt, 0, stream>>>(a);
     return cudaGetLastError();
   }
-  const auto kernel = nt <= 256 ? append_kernel<T, E4M3, false, 256> : append_kernel<T, E4M3, false, 512>;
-  const size_t smem = E4M3 && a.r.rotary_dim ? (size_t)nt * kAppendPasses * 4 * sizeof(float4) : 0;  // up to 128 KB
+  const auto kernel = passes == 2 ? append_kernel<T, E4M3, false, 2, 256>
+                      : nt <= 256 ? append_kernel<T, E4M3, false, 4, 256>
+                                  : append_kernel<T, E4M3, false, 4, 512>;
+  const size_t smem = E4M3 && a.r.rotary_dim ? (size_t)nt * passes * 4 * sizeof(float4) : 0;  // up to 128 KB
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
