@@ -189,7 +189,7 @@ __device__ __forceinline__ void turn16(float (&g0)[8], float (&g1)[8], const flo
 
 // ------------------------------------------------------------------ fa_rotary
 struct RotaryArgs {
-  int B, H, Hkv, T, D, units, heads_per_thread;
+  int B, H, Hkv, T, D, units, heads_per_thread, q_chunks;
   FaTensor q, k, q_out, k_out;
   const int32_t* positions;
   int64_t pos_stride_b;
@@ -206,25 +206,33 @@ __device__ __forceinline__ T* head_row(const FaTensor& q, const FaTensor& k, int
          (int64_t)t * x.stride_t;
 }
 
-// Heads [h0, h1) of one unit of one token.  Two heads (one of fp32) are in work and the next two on
-// their way, as they lie in memory: few registers, so that many warps share an SM.
 template <typename T>
-__device__ __forceinline__ void rotate_heads(const FaTensor& q, const FaTensor& k, const FaTensor& qo,
-                                             const FaTensor& ko, const FaRotarySpec& r, int H, int h0, int h1, int b,
-                                             int t, int u, int pos, float sign) {
+__device__ __forceinline__ T* row_of(const FaTensor& x, int b, int h, int t) {
+  return reinterpret_cast<T*>(x.ptr) + (int64_t)b * x.stride_b + (int64_t)h * x.stride_h + (int64_t)t * x.stride_t;
+}
+
+// Heads [h0, h1) of one unit of one token of one tensor.  Two heads (one of fp32) are in work and the
+// next two on their way, as they lie in memory: few registers, so that many warps share an SM.
+template <typename T>
+__device__ __forceinline__ void rotate_heads(const FaTensor& in, const FaTensor& out, const FaRotarySpec& r, int h0,
+                                             int h1, int b, int t, int u, int pos, float sign) {
   int e0, e1;
   const bool rot = unit_span(r, u, &e0, &e1);
   const bool inter = r.layout == FA_ROTARY_INTERLEAVED;
+  const int apart = e1 - e0;
   constexpr int UN = sizeof(T) == 4 ? 1 : 2;
   typename Io<T>::Raw raw[UN][2];
+  const T* x = row_of<const T>(in, b, h0, t) + e0;
+  T* y = row_of<T>(out, b, h0, t) + e0;
   auto fetch = [&](int h) {
 #pragma unroll
-    for (int i = 0; i < UN; ++i)
+    for (int i = 0; i < UN; ++i) {
       if (h + i < h1) {
-        const T* x = head_row<const T>(q, k, H, h + i, b, t);
-        raw[i][0] = Io<T>::fetch(x + e0);
-        raw[i][1] = Io<T>::fetch(x + e1);
+        raw[i][0] = Io<T>::fetch(x);
+        raw[i][1] = Io<T>::fetch(x + apart);
       }
+      x += in.stride_h;
+    }
   };
   fetch(h0);
   float c[8], s[8];
@@ -244,19 +252,21 @@ __device__ __forceinline__ void rotate_heads(const FaTensor& q, const FaTensor& 
     }
     fetch(h + UN);
 #pragma unroll
-    for (int i = 0; i < UN; ++i)
+    for (int i = 0; i < UN; ++i) {
       if (h + i < h1) {
         float g0[8], g1[8];
         Io<T>::floats(now[i][0], g0);
         Io<T>::floats(now[i][1], g1);
         if (rot) turn16(g0, g1, c, s, inter);
-        T* y = head_row<T>(qo, ko, H, h + i, b, t);
-        Io<T>::store8(y + e0, g0);
-        Io<T>::store8(y + e1, g1);
+        Io<T>::store8(y, g0);
+        Io<T>::store8(y + apart, g1);
       }
+      y += out.stride_h;
+    }
   }
 }
 
+// blockIdx.y: chunks of q's heads, then of k's.
 template <typename T>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   const unsigned idx = blockIdx.x * 256u + threadIdx.x;
@@ -264,8 +274,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   const unsigned tok = idx / a.units, b = tok / a.T;
   const int u = idx % a.units, t = tok % a.T;
   const int pos = a.positions ? __ldg(a.positions + (int64_t)b * a.pos_stride_b + t) : a.pos_offset + t;
-  const int h0 = blockIdx.y * a.heads_per_thread, h1 = min(h0 + a.heads_per_thread, a.H + a.Hkv);
-  rotate_heads<T>(a.q, a.k, a.q_out, a.k_out, a.r, a.H, h0, h1, b, t, u, pos, a.sign);
+  const bool of_k = (int)blockIdx.y >= a.q_chunks;
+  const int h0 = ((int)blockIdx.y - (of_k ? a.q_chunks : 0)) * a.heads_per_thread;
+  const int h1 = min(h0 + a.heads_per_thread, of_k ? a.Hkv : a.H);
+  rotate_heads<T>(of_k ? a.k : a.q, of_k ? a.k_out : a.q_out, a.r, h0, h1, b, t, u, pos, a.sign);
 }
 
 // Any even rotary_dim, head dim, stride and alignment: a thread owns one pair, or two copied
@@ -529,7 +541,7 @@ __global__ void __launch_bounds__(NT, (NT == 512 || sizeof(T) == 4 ? 512 : PASSE
   int start, len;
   const bool ok = new_span(a, b, &start, &len);
   if (ok && start + t < len && a.vec) {
-    rotate_heads<T>(a.q, a.q, a.q_out, a.q_out, a.r, a.H, h0, h1, b, t, u, start + t, 1.f);
+    rotate_heads<T>(a.q, a.q_out, a.r, h0, h1, b, t, u, start + t, 1.f);
     return;
   }
   int e0, e1;
@@ -542,7 +554,7 @@ __global__ void __launch_bounds__(NT, (NT == 512 || sizeof(T) == 4 ? 512 : PASSE
   for (int h = h0; h < h1; ++h) {  // padding rows, and tensors that 16-byte accesses do not fit
     float g0[8] = {0.f}, g1[8] = {0.f};
     if (ok && start + t < len) {
-      const T* x = head_row<const T>(a.q, a.q, a.H, h, b, t);
+      const T* x = row_of<const T>(a.q, b, h, t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         g0[j] = Io<T>::get(x + e0 + j);
@@ -550,7 +562,7 @@ __global__ void __launch_bounds__(NT, (NT == 512 || sizeof(T) == 4 ? 512 : PASSE
       }
       if (rot) turn16(g0, g1, c, s, a.r.layout == FA_ROTARY_INTERLEAVED);
     }
-    T* y = head_row<T>(a.q_out, a.q_out, a.H, h, b, t);
+    T* y = row_of<T>(a.q_out, b, h, t);
     if (a.vec) {
       Io<T>::store8(y + e0, g0);
       Io<T>::store8(y + e1, g1);
@@ -600,9 +612,11 @@ cudaError_t launch_rotary(RotaryArgs& a, bool vec, cudaStream_t stream) {
   a.units = vec ? a.D / 16 : (a.D + 1) / 2;
   const int64_t n = (int64_t)a.B * a.T * a.units;
   a.heads_per_thread = heads_per_thread(n, heads);
-  const dim3 grid((unsigned)((n + 255) / 256), (unsigned)((heads + a.heads_per_thread - 1) / a.heads_per_thread));
-  if (vec) rotary_kernel<T><<<grid, 256, 0, stream>>>(a);
-  else rotary_pair_kernel<T><<<grid, 256, 0, stream>>>(a);
+  const unsigned x = (unsigned)((n + 255) / 256);
+  const int hpt = a.heads_per_thread;
+  a.q_chunks = (a.H + hpt - 1) / hpt;
+  if (vec) rotary_kernel<T><<<dim3(x, a.q_chunks + (a.Hkv + hpt - 1) / hpt), 256, 0, stream>>>(a);
+  else rotary_pair_kernel<T><<<dim3(x, (heads + hpt - 1) / hpt), 256, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
