@@ -7,11 +7,11 @@
 // point in turns, so p * f_i mod 2^64 is the exact phase of any 32-bit position (a product in
 // fp32 is off by 0.06 rad at position 2^20), and its top 32 bits become the reduced angle.
 //
-// Measured (bf16, D 128, 32 + 8 heads): rotation of 2 x 8192 tokens with its gradient 117 us,
-// 5.7 TB/s; one token each of 64 sequences 2.3 us, the launch.  Append of eight prompts of up to
-// 2048 tokens to 8-bit pages with q's rotation 62 us (3.5 TB/s, the zeros of q's padding rows left out;
-// 36 us with 8 + 8 heads): a team's chain of lengths, rows, largest magnitude and stores takes some 4 us.
-// One token each of 64 sequences 4.0 us.
+// Measured (bf16, D 128, 32 + 8 heads): rotation of 2 x 8192 tokens with its gradient 112 us,
+// 6.0 TB/s; one token each of 64 sequences 2.5 us, the launch.  Append of eight prompts of up to
+// 2048 tokens to 8-bit pages with q's rotation 59 us (3.6 TB/s; 34 us with 8 + 8 heads): two thirds of the
+// issue slots, and a team's chain of lengths, rows, largest magnitude and stores.  One token each of 64
+// sequences 4.0 us.
 //
 // A thread owns a unit of 16 elements of a row: 8 + 8 elements rotary_dim / 2 apart for the half
 // layout, 16 neighbours for interleaved pairs and for the copied tail.  It computes the 8 cosines
@@ -127,8 +127,8 @@ __device__ __forceinline__ uint64_t both(float x) { return pack2(x, x); }
 // where the special-function unit's error puts more of them on the wrong side of a border (68 of 16 M
 // codes against 15; cosines and sines rounded from 64 bits: 12).  The angle is reduced to the nearest
 // quarter turn, exactly; then the Taylor series of |y| <= pi / 4, whose first terms left out are
-// y^11 / 11! = 2^-29 and y^10 / 10! = 2^-25.  It cost 3 us in 70 for eight prompts of 2048 tokens, 11
-// without the packed instructions.
+// y^11 / 11! = 2^-29 and y^10 / 10! = 2^-25.  It costs eight prompts of 2048 tokens 3 us (11
+// without the packed instructions).
 __device__ __forceinline__ void pair_turns(const FaRotarySpec& r, int i, uint32_t pos, float* c, float* s) {
   uint32_t w[2];  // phase + 1/8: its two upper bits are the quarter, the others the angle from its middle
   float yf[2], snf[2], csf[2];
@@ -211,16 +211,15 @@ __device__ __forceinline__ T* row_of(const FaTensor& x, int b, int h, int t) {
   return reinterpret_cast<T*>(x.ptr) + (int64_t)b * x.stride_b + (int64_t)h * x.stride_h + (int64_t)t * x.stride_t;
 }
 
-// Heads [h0, h1) of one unit of one token of one tensor.  Two heads (one of fp32) are in work and the
-// next two on their way, as they lie in memory: few registers, so that many warps share an SM.
-template <typename T>
+// Heads [h0, h1) of one unit of one token of one tensor.  UN heads are in work and the next UN on their
+// way, as they lie in memory: few registers, so that many warps share an SM.
+template <typename T, int UN>
 __device__ __forceinline__ void rotate_heads(const FaTensor& in, const FaTensor& out, const FaRotarySpec& r, int h0,
                                              int h1, int b, int t, int u, int pos, float sign) {
   int e0, e1;
   const bool rot = unit_span(r, u, &e0, &e1);
   const bool inter = r.layout == FA_ROTARY_INTERLEAVED;
   const int apart = e1 - e0;
-  constexpr int UN = sizeof(T) == 4 ? 1 : 2;
   typename Io<T>::Raw raw[UN][2];
   const T* x = row_of<const T>(in, b, h0, t) + e0;
   T* y = row_of<T>(out, b, h0, t) + e0;
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   const bool of_k = (int)blockIdx.y >= a.q_chunks;
   const int h0 = ((int)blockIdx.y - (of_k ? a.q_chunks : 0)) * a.heads_per_thread;
   const int h1 = min(h0 + a.heads_per_thread, of_k ? a.Hkv : a.H);
-  rotate_heads<T>(of_k ? a.k : a.q, of_k ? a.k_out : a.q_out, a.r, h0, h1, b, t, u, pos, a.sign);
+  rotate_heads<T, sizeof(T) == 4 ? 1 : 2>(of_k ? a.k : a.q, of_k ? a.k_out : a.q_out, a.r, h0, h1, b, t, u, pos, a.sign);
 }
 
 // Any even rotary_dim, head dim, stride and alignment: a thread owns one pair, or two copied
@@ -353,7 +352,7 @@ __device__ __forceinline__ float page_scale(float top) {
 // magnitude and the store, so they are read once; teams share nothing, and no atomic decides a value.
 // A key's turned values, fp32, wait in shared memory, where each thread reads what it wrote itself (in
 // registers, half as many teams would share an SM; turned twice, eight prompts with as many heads of q as
-// of K took 45 us, now 37; a warp's team, of few rows, turns them twice).  The page's number and its
+// of K took 45 us, then 37; a warp's team, of few rows, turns them twice).  The page's number and its
 // scale are fetched behind the rows' loads.
 // PASSES: row groups that a team holds, 16 values a thread each.
 template <typename T, bool E4M3, bool WARP, int PASSES>
@@ -541,7 +540,7 @@ __global__ void __launch_bounds__(NT, (NT == 512 || sizeof(T) == 4 ? 512 : PASSE
   int start, len;
   const bool ok = new_span(a, b, &start, &len);
   if (ok && start + t < len && a.vec) {
-    rotate_heads<T>(a.q, a.q_out, a.r, h0, h1, b, t, u, start + t, 1.f);
+    rotate_heads<T, sizeof(T) == 4 || PASSES == 2 ? 1 : 2>(a.q, a.q_out, a.r, h0, h1, b, t, u, start + t, 1.f);
     return;
   }
   int e0, e1;
@@ -624,12 +623,13 @@ template <typename T, bool E4M3>
 cudaError_t launch_append(AppendArgs& a, cudaStream_t stream) {
   const int64_t teams = (int64_t)a.B * a.pages_per_seq * a.Hkv * 2;
   const int rows = std::min(a.T, a.ps);
-  // Two passes where 256 threads then hold a page's rows, else four: with two, 64 registers a thread let a
-  // third more threads share an SM (pages of 64 rows of 128: 62 against 68 us, 16 rows: 62 against 73; but
-  // 512 threads in two passes for 64 rows of 256: 130 against 126).  A team is a warp when the rows that one
-  // page can take fit its registers, else a block.
-  const int passes = a.ps * a.units <= 512 ? 2 : 4;
   const bool warp = rows * a.units <= 64;
+  // A team is a warp when the rows that one page can take fit its registers, else a block.  Two passes for
+  // 8-bit pages whose rows 256 threads then hold: with 64 registers a thread, and one of q's heads in work,
+  // a third more threads share an SM (pages of 64 rows of 128: 59 us, with four passes and two heads 66; of
+  // 128 rows, which would take 512 threads: 66 against 59).  bf16 pages, which need no second pass over the
+  // values: 57 with two, 54 with four.
+  const int passes = warp || (E4M3 && a.ps * a.units <= 512) ? 2 : 4;
   const int nt = warp ? 128 : std::max(64, a.ps * a.units / passes);
   a.kv_blocks = (int)(warp ? (teams + 3) / 4 : teams);
   int qb = 0;
@@ -644,7 +644,7 @@ cudaError_t launch_append(AppendArgs& a, cudaStream_t stream) {
     append_kernel<T, E4M3, true, 2, 128><<<grid, nt, 0, stream>>>(a);
     return cudaGetLastError();
   }
-  const auto kernel = passes == 2 ? append_kernel<T, E4M3, false, 2, 256>
+  const auto kernel = passes == 2 ? append_kernel<T, E4M3, false, E4M3 ? 2 : 4, 256>  // (8-bit only)
                       : nt <= 256 ? append_kernel<T, E4M3, false, 4, 256>
                                   : append_kernel<T, E4M3, false, 4, 512>;
   const size_t smem = E4M3 && a.r.rotary_dim ? (size_t)nt * passes * 4 * sizeof(float4) : 0;  // up to 128 KB
