@@ -329,7 +329,9 @@ FA_API int fa_rotary(const FaRotaryParams* p, fa_stream_t stream);
  * j of sequence b is row j % page_size of page block_table[b][j / page_size].  An e4m3 cache
  * holds codes with one scale per page and K/V head: value = code * scale.  fa_paged_append
  * makes the scales powers of two, so that rescaling a page only loses what falls below the
- * 8-bit type's smallest step. */
+ * 8-bit type's smallest step.  A value scale of 2^-100 (the least that an append gives) or less
+ * counts as zero.  Attention's sum keeps every weight that counts while the value scales that a row
+ * sees lie between 2^-100 and 2^64. */
 typedef struct {
   int32_t dtype;             /* FA_DTYPE_BF16 or FA_DTYPE_E4M3 */
   int32_t num_pages, H_kv, page_size, D; /* page_size in {16, 32, 64, 128}; D in {64, 128, 256} */

@@ -78,6 +78,14 @@ constexpr int kScaleRing = 16;     // tiles whose scales may be live at once (> 
 __host__ __device__ constexpr float slack_of(int ES) { return ES == 1 ? 1.75f : 60.f; }
 __host__ __device__ constexpr float head_of(int ES) { return ES == 1 ? 2.f : 0.f; }
 __host__ __device__ constexpr float lift_of(int ES) { return ES == 1 ? 7.f - 8.f : 0.f; }
+// Value scales.  The append's least one, 2^-100, and less count as zero: the page's codes are cleared, and
+// since its place in the exponent is free then, it is one that keeps sums in range and does not push the
+// reference up.  In tiles with such a page, or one of a scale far from 1, P / vs is not formed from P, which
+// may have underflowed (next to a page of 2^30, P of one of 2^-90 is 2^-120 at the same logit), but from the
+// logit.  (A choice in the common loop instead of a loop before it took 247 instead of 235 us for the prompt
+// chunk below.)
+constexpr float kNoScale = 0x1p-100f, kNoScaleLog2 = -80.f, kFarLog2 = 40.f;
+constexpr int kCleared = 1, kFar = 2;  // a tile with a hidden page or one without a scale; with one far from 1
 constexpr float kUnset = -1e30f;   // reference of a row that has seen nothing yet
 
 struct PagedArgs {
@@ -260,7 +268,7 @@ template <int R> struct Smem {
   RowState rs[R <= 16 ? 2 : 4];
   Posted post[2][R <= 16 ? 2 : 4];  // by unit parity and group
   float2 scales[kScaleRing][8];  // (ks, vs) of a tile's pages; ks = -inf hides the page
-  int odd[kScaleRing];           // the tile has a hidden page, or one of a scale below 2^-100
+  int odd[kScaleRing];           // kCleared, kFar: what the tile's pages ask for beside the common path
   uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], posted[2], done[2], fin_bar[2];
   int scan[24];
   Start start;
@@ -655,7 +663,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       const int page = hidden ? a.num_pages : x.page;  // reads as zeros: the map's bounds check
       const int n = min(batch, my_tiles - j0);
       const unsigned pages = (1u << ppt) - 1u;
-      unsigned small = 0;
+      unsigned none = 0, far = 0;  // pages without a value scale, with one far from 1
       for (int k = 0; k < n; ++k) {
         const uint32_t bytes = ((uint32_t)__popc((act >> (k << ppt_log)) & pages) << a.ps_log) * S::ROWB;
 #pragma unroll
@@ -674,9 +682,14 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
             // The scales are there before the slot's barrier can complete.  Their place in the ring is
             // free: the tile that used it lies further back than the ring of slots reaches.
             const int ring = (j0 + k) % kScaleRing;
-            if (ES == 1 && k == 0) small = __ballot_sync(0xffffffffu, x.active && !(x.vs >= 0x1p-100f));
+            if (ES == 1 && k == 0) {
+              none = __ballot_sync(0xffffffffu, x.active && !(x.vs > kNoScale));
+              far = __ballot_sync(0xffffffffu, x.active && x.vs > kNoScale && !(fabsf(lg2_approx(x.vs)) <= kFarLog2));
+            }
             if (sub == k) sm.scales[ring][pg] = make_float2(x.ks, x.vs);
-            if (lane == 0) sm.odd[ring] = (((hid | small) >> (k << ppt_log)) & pages) != 0;
+            if (lane == 0)
+              sm.odd[ring] = ((((hid | none) >> (k << ppt_log)) & pages) ? kCleared : 0) |
+                             (((far >> (k << ppt_log)) & pages) ? kFar : 0);
             __syncwarp();
           }
           if (lane == 0) mbar_arrive(sm.full + slot);
@@ -886,10 +899,9 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         const int odd = sm.odd[j % kScaleRing];
         const bool shown = sc.x != -INFINITY;
         const float ks = ES == 1 ? (shown ? sc.x : 0.f) : 1.f;
-        // a value scale below 2^-100 counts as zero: its codes are cleared below
-        const float lv = ES == 1 ? fmaxf(lg2_approx(sc.y), -100.f) : 0.f;
-        const float inv_vs = ES == 1 ? ex2_approx(-lv) : 1.f;
-        const bool inside = p0 >= sg.in_lo && p0 + kTile - 1 <= sg.in_hi && !odd;
+        const float lv = ES != 1 ? 0.f : sc.y > kNoScale ? lg2_approx(sc.y) : kNoScaleLog2;
+        const float inv_vs = ES == 1 && !odd ? ex2_approx(-lv) : 0.f;
+        const bool inside = p0 >= sg.in_lo && p0 + kTile - 1 <= sg.in_hi && !(odd & kCleared);
         tmem_ld_wait();
         reg_pin(r);
         float z[C], top = -INFINITY;
@@ -982,6 +994,10 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           }
         }
         filled = true;
+        if (ES == 1 && odd) {
+#pragma unroll
+          for (int n = 0; n < C; ++n) l[n] += ex2_approx(z[n] - lv + (KEEP ? bias[n] : rs.bias[n]));
+        }
         // P(j - 2), which lies where P(j) goes, has been read
         if (j >= 2 && !wait_for(sm.o_full + (j & 1), (uint32_t)(((j >> 1) - 1) & 1), abort_flag)) *abort_flag = 1;
         // ---- probabilities: the sum in fp32, P into shared memory as the B operand
@@ -1016,14 +1032,14 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           if constexpr (ES == 1) *reinterpret_cast<uint4*>(pw + S::PPART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           else *reinterpret_cast<uint4*>(pw + 2048) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
         }
-        if (p0 < sg.lo || p0 + kTile - 1 > sg.hi || odd) {
+        if (p0 < sg.lo || p0 + kTile - 1 > sg.hi || (odd & kCleared)) {
           // Positions that no row sees may hold anything (a zero probability times NaN is NaN), and
           // value scales of zero make no contribution: these rows of V become zero when the tile
           // has landed.
           const int ld = 2 * j + 1, slot = ld % NS;
           if (!wait_for(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
           const bool clears = half == 0;  // one group does
-          if (clears && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sc.y >= 0x1p-100f)))) {
+          if (clears && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sc.y > kNoScale)))) {
             unsigned char* v = base + (size_t)slot * S::SLOT + t * SW;
 #pragma unroll 1
             for (int p = 0; p < S::ROWB / SW; ++p)
