@@ -23,11 +23,17 @@
 // the largest below that.
 //
 // Scales.  ks multiplies the thread's logits.  vs goes into the exponent: with z = x + log2 vs and
-// a reference m >= max z - 1.75 per row, P = 2^(z - m + 7) weighs the codes, and the softmax sum
-// adds P / vs; o = sum P code / sum (P / vs).  So a row whose weight sits on pages of small values
-// keeps its precision.  The reference moves only when a tile exceeds it by more than 1.75: one
-// barrier vote per tile.  A unit's tiles are taken from its end to its start: under ALiBi, and mostly
-// without it, the largest logits come first and the references hardly move.
+// a reference m per row, P = 2^(z - m + 7) weighs the codes, and the softmax sum adds P / vs;
+// o = sum P code / sum (P / vs).  So a row whose weight sits on pages of small values keeps its
+// precision.  A reference moves up when a tile exceeds it by more than 1.75: one barrier vote per
+// tile.  A unit's tiles are taken from its end to its start: under ALiBi, and mostly without it, the
+// largest logits come first and the references hardly move.
+// An 8-bit reference moves down again, too, by up to 20 below its highest: the smallest step of the
+// parts is 2^-9, and a tile far below the reference would keep its place in the sum and lose it in O (a key
+// 11 nats above a rest of 32768 positions: o off by 5 to 10 %, now 0.2 at most).  When a row's largest P was below
+// 1/2 in two tiles, the third one's becomes 32, and O and the sum are scaled up.  (After one such tile there
+// would be twice as many moves where neighbouring tiles differ in size.  For the prompt chunk below, whose
+// pages' scales differ by up to 8, references that move down cost 27 us of 262, for decode 1 of 75.)
 //
 // Work.  The tiles of all (sequence, row group, K/V head) units, in that order, are cut into equal
 // contiguous ranges, one per CTA (one CTA per SM): ragged batches balance themselves, and nothing
@@ -47,9 +53,9 @@
 // sums are double-buffered for that).  64 rows leave threads for one set only.
 //
 // Measured on the device (8-bit pages, H 32, H_kv 8, D 128, ragged lengths): 64 users of up to 4096
-// positions, one token each: 74 us, 5.4 TB/s, 0.83 of the measured copy rate; eight of up to 32768: 72 us,
-// 5.6 TB/s; one of 1000: 9.4 us, the launch, one tile's chain and the join.  Chunks of 512 tokens of four
-// users on up to 4096 positions: 228 us, bound by the chain of one set of softmax groups at 64 rows.
+// positions, one token each: 74 us, 5.4 TB/s, 0.83 of the measured copy rate; eight of up to 32768: 73 us,
+// 5.5 TB/s; one of 1000: 9.4 us, the launch, one tile's chain and the join.  Chunks of 512 tokens of four
+// users on up to 4096 positions: 260 us, bound by the chain of one set of softmax groups at 64 rows.
 // bf16, H 16, D 64, window 1024, ALiBi, 32 users: 45 us.
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -87,6 +93,7 @@ __host__ __device__ constexpr float lift_of(int ES) { return ES == 1 ? 7.f - 8.f
 constexpr float kNoScale = 0x1p-100f, kNoScaleLog2 = -80.f, kFarLog2 = 40.f;
 constexpr int kCleared = 1, kFar = 2;  // a tile with a hidden page or one without a scale; with one far from 1
 constexpr float kUnset = -1e30f;   // reference of a row that has seen nothing yet
+constexpr float kDrop = 20.f;      // 8-bit: how far a reference goes below the highest one it had
 
 struct PagedArgs {
   int B, H, Hkv, Tq, G, M;         // M = G * Tq query rows per sequence and K/V head
@@ -159,6 +166,10 @@ template <int R> struct RowConst {
 struct RowState {
   float m[16], bias[16];  // reference; lift - reference
   float move[16];         // factor of the last move
+  float high[16];         // the highest reference so far (8-bit)
+  uint4 seen[2];          // rows with a probability of 1/2 or more in the last two tiles (row_bit), by warp; in turn
+  uint32_t watch;         // rows whose reference may go down
+  int far;                // a value scale far from 1 was met: none may, so that sums stay in range
   float4 red[16];         // a value of each warp
   float fin[2][16];       // factors of the O (of both groups) at the end
 };
@@ -349,6 +360,12 @@ __device__ __forceinline__ uint32_t split_e4m3x4(const float (&p)[4], uint32_t* 
   *lo4 = (la >> 7) | (lb << 1);
   return (ha >> 7) | (hb << 1);
 }
+
+__device__ __forceinline__ float value_log2(float vs) { return vs > kNoScale ? lg2_approx(vs) : kNoScaleLog2; }
+
+// Row n's bit in a mask of 16 rows, as split_e4m3x4's codes give it: byte n % 4 of word n / 4, whose
+// upper bits lie side by side.
+__host__ __device__ constexpr uint32_t row_bit(int n) { return 0x80u << (8 * (n & 3)) >> (n >> 2); }
 
 // Byte offset of 16-byte chunk c of row r in a panel of rows of SW bytes, swizzled over SW.
 template <int SW>
@@ -869,6 +886,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         rs.bias[t] = LIFT - kUnset;
         rs.move[t] = 1.f;
       }
+      if (t == 0) rs.watch = 0u, rs.far = 0;
       // Inside a unit no wait leaves the loops: after a time-out every later wait returns at once and
       // nothing is written at the end.
       // The threads of a group agree on whether the unit is known, so that they leave together.
@@ -887,6 +905,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         bias[n] = LIFT - kUnset;
       }
       bool filled = false;  // this group's O holds something of this unit
+      uint32_t seen = 0xffffffffu;  // the last tile's RowState::seen of this warp alone
       const uint32_t t_o = t_lane + S::TM_O + (TURNS ? ((seg & 1) * 2 + set) * S::ON : 0) + c0;
       for (int it = 0; it < sg.nt; ++it, ++j) {
         if (TURNS && (j & 1) != set) continue;
@@ -899,7 +918,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         const int odd = sm.odd[j % kScaleRing];
         const bool shown = sc.x != -INFINITY;
         const float ks = ES == 1 ? (shown ? sc.x : 0.f) : 1.f;
-        const float lv = ES != 1 ? 0.f : sc.y > kNoScale ? lg2_approx(sc.y) : kNoScaleLog2;
+        const float lv = ES == 1 ? value_log2(sc.y) : 0.f;
         const float inv_vs = ES == 1 && !odd ? ex2_approx(-lv) : 0.f;
         const bool inside = p0 >= sg.in_lo && p0 + kTile - 1 <= sg.in_hi && !(odd & kCleared);
         tmem_ld_wait();
@@ -946,7 +965,16 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           }
           top = fmax3f(top, fmax3f(z[c] + bias[c], z[c + 1] + bias[c + 1], z[c + 2] + bias[c + 2]), z[c + 3] + bias[c + 3]);
         }
-        if (vote_or(bar, 128, top > LIFT + SLACK)) {
+        bool moves = vote_or(bar, 128, top > LIFT + SLACK);
+        uint32_t low = 0;  // rows whose largest probability in both of the group's last two tiles was below 1/2
+        if constexpr (ES == 1) {
+          if (filled) {
+            const uint4 s = rs.seen[((j >> TURNS) & 1) ^ 1];
+            low = rs.watch & ~(s.x | s.y | s.z | s.w);
+            moves |= low != 0;
+          }
+        }
+        if (moves) {
           // ---- a reference has to move to the tile's largest z of its row
 #pragma unroll
           for (int c = 0; c < C; c += CH) {
@@ -958,14 +986,25 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
             }
           }
           named_bar_sync(bar, 128);
+          uint32_t may = 0;
           if (t < (SKIP ? (rr + CH - 1) & -CH : C)) {  // (rows worked on, real or not: an unset one would ask to move again)
             const float old = rs.m[t];
             const float4 w = rs.red[t];
             const float nm = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
-            const float m = nm > old + SLACK ? nm + HEAD : old;
+            float m = nm > old + SLACK ? nm + HEAD : old;
+            if constexpr (ES == 1) {
+              float high = old == kUnset ? kUnset : rs.high[t];
+              if (m == old && (low & row_bit(t))) m = fmaxf(fminf(old, nm + HEAD), high - kDrop);
+              rs.high[t] = high = fmaxf(high, m);
+              if (t < rr && rc.lo[c0 + t] <= rc.hi[c0 + t] && m > fmaxf(high - kDrop, kUnset)) may = row_bit(t);
+            }
             rs.move[t] = m != old ? ex2_approx(old - m) : 1.f;
             rs.m[t] = m;
             rs.bias[t] = LIFT - m;
+          }
+          if (ES == 1 && (warp & 3) == 0) {
+            may = __reduce_or_sync(0xffffffffu, may);
+            if (lane == 0) rs.watch = rs.far ? 0u : may;
           }
           named_bar_sync(bar, 128);
 #pragma unroll
@@ -995,8 +1034,10 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         }
         filled = true;
         if (ES == 1 && odd) {
+          const float lv = value_log2(sm.scales[j % kScaleRing][my_page].y);  // (read again: registers)
 #pragma unroll
           for (int n = 0; n < C; ++n) l[n] += ex2_approx(z[n] - lv + (KEEP ? bias[n] : rs.bias[n]));
+          if (t == 0 && (odd & kFar)) rs.far = 1, rs.watch = 0u;  // (the next vote shows it)
         }
         // P(j - 2), which lies where P(j) goes, has been read
         if (j >= 2 && !wait_for(sm.o_full + (j & 1), (uint32_t)(((j >> 1) - 1) & 1), abort_flag)) *abort_flag = 1;
@@ -1025,6 +1066,15 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
             hi[c / 4] = split_e4m3x4(p, &lo[c / 4]);
           }
         }
+        if constexpr (ES == 1) {
+          // a code of 1/2 is 0x30; the next tile's vote shows it to the other warps
+          uint32_t now = 0;
+#pragma unroll
+          for (int i = 0; i < C / 4; ++i) now |= ((hi[i] + 0x50505050u) & 0x80808080u) >> i;
+          now = __reduce_or_sync(0xffffffffu, now);
+          if (lane == 0) reinterpret_cast<uint32_t*>(&rs.seen[(j >> TURNS) & 1])[warp & 3] = now | seen;
+          seen = now;
+        }
         if constexpr (S::SIDE) {
           *reinterpret_cast<uint4*>(pw) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
         } else {
@@ -1039,7 +1089,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           const int ld = 2 * j + 1, slot = ld % NS;
           if (!wait_for(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
           const bool clears = half == 0;  // one group does
-          if (clears && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sc.y > kNoScale)))) {
+          if (clears && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sm.scales[j % kScaleRing][my_page].y > kNoScale)))) {
             unsigned char* v = base + (size_t)slot * S::SLOT + t * SW;
 #pragma unroll 1
             for (int p = 0; p < S::ROWB / SW; ++p)
