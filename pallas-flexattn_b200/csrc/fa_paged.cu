@@ -171,7 +171,7 @@ struct RowState {
   uint32_t watch;         // rows whose reference may go down
   int far;                // a value scale far from 1 was met: none may, so that sums stay in range
   float4 red[16];         // a value of each warp
-  float fin[2][16];       // factors of the O (of both groups) at the end
+  float fin[2][16];       // factors of the O (of both groups) at the end; the first negative: no position seen
 };
 struct Posted {  // what a group knows of a unit when it leaves it
   float m[16];
@@ -1147,7 +1147,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           // a NaN stays one; a row that may see nothing took part in the tiles that needed no mask
           const bool some = !(sum == 0.f) && rc.lo[c0 + t] <= rc.hi[c0 + t];
           const float inv = some ? (ES == 1 ? 0x1p-8f : 1.f) / sum : 0.f;  // (8-bit P is 2^8 times what the sum adds)
-          rs.fin[0][t] = f * inv;
+          rs.fin[0][t] = some ? f * inv : -1.f;  // negative: zeros, whatever O holds (0 times a NaN is one)
           rs.fin[1][t] = fo * inv;
           const float lse = some ? (m - LIFT + lg2_approx(sum)) * kLn2 : -INFINITY;
           if (!*abort_flag) {
@@ -1192,6 +1192,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
                 }
                 v *= f[u];
                 if constexpr (TURNS) v = fmaf(o, g[u], v);
+                if (f[u] < 0.f) v = 0.f;
                 if (!whole) a.part_o[((int64_t)part * R + n) * D + d] = v;
                 else if (n0 + u < rr) reinterpret_cast<__nv_bfloat16*>(a.o.ptr)[rc.orow[n] + d] = __float2bfloat16_rn(v);
               }
