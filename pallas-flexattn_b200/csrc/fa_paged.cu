@@ -526,7 +526,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
   unsigned char* sP = sQ + 2 * S::QBUF;
   Smem<R>& sm = *reinterpret_cast<Smem<R>*>(sP + 2 * S::PBUF);
   volatile int* abort_flag = &sm.abort_flag;
-  volatile int* never = &sm.never;  // stays 0: waits on it end by time only
+  volatile int* never = &sm.never;  // stays 0: waits on it end by their polls only
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
 
@@ -729,7 +729,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     const int end = 2 * my_tiles;
     for (int ld = issued - STEP; ld >= 0 && ld >= (ok ? end : issued) - NS; ld -= STEP) {
       if (ok) {
-        wait_for_w(sm.full + ld % NS, (uint32_t)((ld / NS) & 1), never);
+        if (!wait_for_w(sm.full + ld % NS, (uint32_t)((ld / NS) & 1), never) && lane == 0) *abort_flag = 1;
       } else {
         for (int n = 0; n < 1000 && !mbar_try_wait(sm.full + ld % NS, (uint32_t)((ld / NS) & 1)); ++n) __nanosleep(1000);
         __syncwarp();
@@ -776,7 +776,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     }
     if (!ok && lane == 0) *abort_flag = 1;
     tc_commit_w(sm.fin_bar);
-    wait_for_w(sm.fin_bar, 0, never);  // every MMA has retired before TMEM is freed
+    if (!wait_for_w(sm.fin_bar, 0, never) && lane == 0) *abort_flag = 1;  // every MMA has retired before TMEM is freed
   } else if (warp == W_PV) {
     // ---------------------------------------------------------------- P V issue
     // V as the M-major operand: panels of SW bytes of D are LBO apart (a head dim of 64 has one
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     }
     if (!ok && lane == 0) *abort_flag = 1;
     tc_commit_w(sm.fin_bar + 1);
-    wait_for_w(sm.fin_bar + 1, 0, never);
+    if (!wait_for_w(sm.fin_bar + 1, 0, never) && lane == 0) *abort_flag = 1;
   } else if (warp == W_Q) {
     // ---------------------------------------------------------------- Q operand and row constants
     // The softmax warps build the first unit's (they have nothing else to do yet).
@@ -854,6 +854,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.q_full + buf);
     }
+    if (!ok && lane == 0) *abort_flag = 1;
   } else {
     // ---------------------------------------------------------------- softmax (thread = position)
     const int grp = warp >> 2, t = tid & 127, bar = 1 + grp;
@@ -1209,10 +1210,11 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       // The references are set anew when all of their readers are here.
       named_bar_sync(bar, 128);
     }
-    if (tid == 0 && *abort_flag) report_status(a.status, FA_ERR_TIMEOUT);
   }
   tc_fence_before();
   __syncthreads();
+  // every warp's waits are behind: one that gave up shows here, whichever it was
+  if (tid == 0 && *abort_flag) report_status(a.status, FA_ERR_TIMEOUT);
   if (warp == W_S) {
     tc_fence_after();
     tmem_dealloc(tmem, S::TM_COLS);
