@@ -330,7 +330,7 @@ FA_API int fa_rotary(const FaRotaryParams* p, fa_stream_t stream);
  * holds codes with one scale per page and K/V head: value = code * scale.  fa_paged_append
  * makes the scales powers of two, so that rescaling a page only loses what falls below the
  * 8-bit type's smallest step.  A value scale of 2^-100 (the least that an append gives) or less
- * counts as zero.  Attention's sum keeps every weight that counts while the value scales that a row
+ * in magnitude counts as zero, one that is NaN or infinite makes its values NaN.  Attention's sum keeps every weight that counts while the value scales that a row
  * sees lie between 2^-100 and 2^64. */
 typedef struct {
   int32_t dtype;             /* FA_DTYPE_BF16 or FA_DTYPE_E4M3 */

@@ -90,8 +90,10 @@ __host__ __device__ constexpr float lift_of(int ES) { return ES == 1 ? 7.f - 8.f
 // may have underflowed (next to a page of 2^30, P of one of 2^-90 is 2^-120 at the same logit), but from the
 // logit.  (A choice in the common loop instead of a loop before it took 247 instead of 235 us for the prompt
 // chunk below.)
-constexpr float kNoScale = 0x1p-100f, kNoScaleLog2 = -80.f, kFarLog2 = 40.f;
-constexpr int kCleared = 1, kFar = 2;  // a tile with a hidden page or one without a scale; with one far from 1
+constexpr float kNoScale = 0x1p-100f, kScaleless = 0x1p-80f, kFar2 = 0x1p40f;
+constexpr uint32_t kZeros = 1u, kSigns = 0x80808080u, kNaNs = 0x7f7f7f7fu;  // codes that become 0, change sign, or become NaN
+constexpr int kCleared = 1, kFar = 2;  // a tile with a hidden page or one whose scale is not above 2^-100 and
+                                       // finite (negative ones are for the codes' signs); with one far from 1
 constexpr float kUnset = -1e30f;   // reference of a row that has seen nothing yet
 constexpr float kDrop = 20.f;      // 8-bit: how far a reference goes below the highest one it had
 
@@ -278,7 +280,8 @@ template <int R> struct Smem {
   RowConst<R> rc[2];
   RowState rs[R <= 16 ? 2 : 4];
   Posted post[2][R <= 16 ? 2 : 4];  // by unit parity and group
-  float2 scales[kScaleRing][8];  // (ks, vs) of a tile's pages; ks = -inf hides the page
+  float2 scales[kScaleRing][8];  // (ks, |vs|) of a tile's pages; ks = -inf hides the page; vs may be kScaleless
+  uint32_t turned[kScaleRing][8];  // what becomes of a page's V codes: 0 (they stay), kZeros, kSigns, kNaNs
   int odd[kScaleRing];           // kCleared, kFar: what the tile's pages ask for beside the common path
   uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], posted[2], done[2], fin_bar[2];
   int scan[24];
@@ -360,8 +363,6 @@ __device__ __forceinline__ uint32_t split_e4m3x4(const float (&p)[4], uint32_t* 
   *lo4 = (la >> 7) | (lb << 1);
   return (ha >> 7) | (hb << 1);
 }
-
-__device__ __forceinline__ float value_log2(float vs) { return vs > kNoScale ? lg2_approx(vs) : kNoScaleLog2; }
 
 // Row n's bit in a mask of 16 rows, as split_e4m3x4's codes give it: byte n % 4 of word n / 4, whose
 // upper bits lie side by side.
@@ -680,7 +681,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       const int page = hidden ? a.num_pages : x.page;  // reads as zeros: the map's bounds check
       const int n = min(batch, my_tiles - j0);
       const unsigned pages = (1u << ppt) - 1u;
-      unsigned none = 0, far = 0;  // pages without a value scale, with one far from 1
+      unsigned none = 0, far = 0;  // pages without a positive value scale, with one far from 1
+      uint32_t turned = 0;
       for (int k = 0; k < n; ++k) {
         const uint32_t bytes = ((uint32_t)__popc((act >> (k << ppt_log)) & pages) << a.ps_log) * S::ROWB;
 #pragma unroll
@@ -700,10 +702,16 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
             // free: the tile that used it lies further back than the ring of slots reaches.
             const int ring = (j0 + k) % kScaleRing;
             if (ES == 1 && k == 0) {
-              none = __ballot_sync(0xffffffffu, x.active && !(x.vs > kNoScale));
-              far = __ballot_sync(0xffffffffu, x.active && x.vs > kNoScale && !(fabsf(lg2_approx(x.vs)) <= kFarLog2));
+              const bool positive = x.vs > kNoScale && x.vs < INFINITY, some = fabsf(x.vs) > kNoScale && fabsf(x.vs) < INFINITY;
+              none = __ballot_sync(0xffffffffu, x.active && !positive);
+              turned = some ? kSigns : fabsf(x.vs) <= kNoScale ? kZeros : kNaNs;
+              x.vs = some ? fabsf(x.vs) : kScaleless;
+              far = __ballot_sync(0xffffffffu, x.active && some && !(x.vs >= 1.f / kFar2 && x.vs <= kFar2));
             }
-            if (sub == k) sm.scales[ring][pg] = make_float2(x.ks, x.vs);
+            if (sub == k) {
+              sm.scales[ring][pg] = make_float2(x.ks, x.vs);
+              if (ES == 1) sm.turned[ring][pg] = none >> lane & 1u ? turned : 0u;
+            }
             if (lane == 0)
               sm.odd[ring] = ((((hid | none) >> (k << ppt_log)) & pages) ? kCleared : 0) |
                              (((far >> (k << ppt_log)) & pages) ? kFar : 0);
@@ -919,7 +927,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         const int odd = sm.odd[j % kScaleRing];
         const bool shown = sc.x != -INFINITY;
         const float ks = ES == 1 ? (shown ? sc.x : 0.f) : 1.f;
-        const float lv = ES == 1 ? value_log2(sc.y) : 0.f;
+        const float lv = ES == 1 ? lg2_approx(sc.y) : 0.f;
         const float inv_vs = ES == 1 && !odd ? ex2_approx(-lv) : 0.f;
         const bool inside = p0 >= sg.in_lo && p0 + kTile - 1 <= sg.in_hi && !(odd & kCleared);
         tmem_ld_wait();
@@ -1035,7 +1043,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         }
         filled = true;
         if (ES == 1 && odd) {
-          const float lv = value_log2(sm.scales[j % kScaleRing][my_page].y);  // (read again: registers)
+          const float lv = lg2_approx(sm.scales[j % kScaleRing][my_page].y);  // (read again: registers)
 #pragma unroll
           for (int n = 0; n < C; ++n) l[n] += ex2_approx(z[n] - lv + (KEEP ? bias[n] : rs.bias[n]));
           if (t == 0 && (odd & kFar)) rs.far = 1, rs.watch = 0u;  // (the next vote shows it)
@@ -1086,17 +1094,25 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         if (p0 < sg.lo || p0 + kTile - 1 > sg.hi || (odd & kCleared)) {
           // Positions that no row sees may hold anything (a zero probability times NaN is NaN), and
           // value scales of zero make no contribution: these rows of V become zero when the tile
-          // has landed.
+          // has landed.  The sign of a negative scale goes to the codes, and a NaN or an infinity makes
+          // them NaN.
           const int ld = 2 * j + 1, slot = ld % NS;
           if (!wait_for(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
           const bool clears = half == 0;  // one group does
-          if (clears && (pos < sg.lo || pos > sg.hi || (ES == 1 && !(sm.scales[j % kScaleRing][my_page].y > kNoScale)))) {
+          const bool seen_here = pos >= sg.lo && pos <= sg.hi;
+          const uint32_t turn = !seen_here ? kZeros : ES == 1 ? sm.turned[j % kScaleRing][my_page] : 0u;
+          if (clears && turn) {
             unsigned char* v = base + (size_t)slot * S::SLOT + t * SW;
 #pragma unroll 1
             for (int p = 0; p < S::ROWB / SW; ++p)
 #pragma unroll
-              for (int c = 0; c < SW / 16; ++c)
-                *reinterpret_cast<uint4*>(v + p * S::PANEL + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+              for (int c = 0; c < SW / 16; ++c) {
+                uint4* at = reinterpret_cast<uint4*>(v + p * S::PANEL + c * 16);
+                const uint32_t w = turn == kZeros ? 0u : turn;
+                uint4 x = make_uint4(w, w, w, w);
+                if (ES == 1 && turn == kSigns) x.x ^= at->x, x.y ^= at->y, x.z ^= at->z, x.w ^= at->w;
+                *at = x;
+              }
           }
         }
         fence_proxy_async_smem();

@@ -59,3 +59,34 @@ def test_rows_that_see_nothing_are_zero_next_to_nan(name, dtype, special):
     hit[5] = True
     assert not torch.isfinite(o[live][:, hit]).any()
     assert torch.isfinite(o[live][:, ~hit]).all() and torch.isfinite(lse[live]).all()
+
+
+@pytest.mark.parametrize("G,Tq,D", [(4, 1, 128), (12, 1, 64), (8, 3, 128), (8, 8, 256)])
+def test_value_scales_that_are_not_positive_numbers(G, Tq, D):
+    """value = code * scale whatever the scale: negative ones turn the sign, NaN and infinity reach every row that
+    sees the page, and no other head or sequence."""
+    g = torch.Generator().manual_seed(D + G)
+    cache = cache_of(24, 2, 32, D, F8, g)
+    table = torch.randperm(24, generator=g).view(2, 12).to(DEV, torch.int32)
+    q = torch.randn(2, 2 * G, Tq, D, generator=g).to(DEV, BF16)
+    lens = [370, 300]
+    cache.v_scale[table[0, 2:5].long(), 0] = -(2.0 ** -5)
+    cache.v_scale[table[1, 7].long(), 1] = -(2.0 ** -101)  # counts as zero
+    cache.k_scale[table[1, 3].long(), 0] *= -1
+    args = (q, cache, table, lens, pf.causal_mask)
+    o, lse = pf.flash_attention_paged(*args)
+    ro, rl, to, tl = attend64(q, cache, table, lens, [Tq] * 2, "causal", 0, None, 0, 1 / math.sqrt(D))
+    # attend64 bounds the logits' sum with log2 vs, of a positive vs: the same for its magnitude
+    signed = cache.v_scale.clone()
+    cache.v_scale.abs_()
+    _, _, to, tl = attend64(q, cache, table, lens, [Tq] * 2, "causal", 0, None, 0, 1 / math.sqrt(D))
+    cache.v_scale.copy_(signed)
+    assert_within("lse", lse, rl, tl)
+    assert_within("o", o, ro, to)
+    for bad in (math.nan, math.inf, -math.inf):
+        cache.v_scale[table[0, 4].long(), 0] = bad
+        o2, lse2 = pf.flash_attention_paged(*args)
+        check_device_status(DEV)
+        assert torch.isnan(o2[0, :G]).all()
+        assert torch.equal(o2[0, G:], o[0, G:]) and torch.equal(o2[1], o[1])
+        assert_within("lse", lse2, rl, tl)
