@@ -66,11 +66,25 @@ def device_status(device) -> torch.Tensor:
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     k = str(device)
-    if k not in _STATUS:
-        _STATUS[k] = torch.zeros(1, dtype=torch.int32, device=device)
-    return _STATUS[k]
+    st = _STATUS.get(k)
+    if st is None:
+        st = torch.zeros(1, dtype=torch.int32, device=device)
+        if device.type == "cuda" and _capturing(device):
+            # Memory of the graph, zeroed by each of its replays: a word for this graph alone.
+            _GRAPH_STATUS.setdefault(k, []).append(st)
+        else:
+            if device.type == "cuda":
+                torch.cuda.current_stream(device).synchronize()  # no kernel of another stream reports before the zero
+            _STATUS[k] = st
+    return st
 
 
+def _capturing(device: torch.device) -> bool:
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+_GRAPH_STATUS: dict = {}  # words of graphs whose capture held the first call on a device
 _STATUS_PTR: dict = {}
 
 
@@ -78,20 +92,27 @@ def status_ptr(index: int) -> int:
     """Address of device_status of CUDA device `index`."""
     p = _STATUS_PTR.get(index)
     if p is None:
-        p = _STATUS_PTR[index] = device_status(torch.device("cuda", index)).data_ptr()
+        dev = torch.device("cuda", index)
+        if str(dev) not in _STATUS and _capturing(dev):
+            raise RuntimeError("the status word of this device does not exist yet and cannot be made inside a stream "
+                               "capture: call check_device_status() before it")
+        p = _STATUS_PTR[index] = device_status(dev).data_ptr()
     return p
 
 
 def check_device_status(device=None) -> None:
     """Synchronise and raise if any kernel on `device` reported a timeout or an invalid length or page."""
     device = torch.device(device if device is not None else "cuda")
-    st = device_status(device)
-    v = int(st.item())
-    if v:
-        st.zero_()
-        if v == L.FA_ERR_INVALID:
-            raise L.FlexAttnError(v, "a length or page number read on the device was out of range (it was skipped)")
-        raise L.FlexAttnError(v, "a device-side wait timed out (kernel aborted its tile)")
+    words = [device_status(device)]
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    for st in words + _GRAPH_STATUS.get(str(device), []):
+        v = int(st.item())
+        if v:
+            st.zero_()
+            if v == L.FA_ERR_INVALID:
+                raise L.FlexAttnError(v, "a length or page number read on the device was out of range (it was skipped)")
+            raise L.FlexAttnError(v, "a device-side wait timed out (kernel aborted its tile)")
 
 
 def clear_table_cache() -> None:

@@ -78,6 +78,7 @@ class PagedKVCache:
                         *v.stride()[:3], *((k_scale.data_ptr(), v_scale.data_ptr()) if k_scale is not None else (0, 0)))
         self._shape, self._device = (n, hkv, ps, d), k.device
         self._plans: dict = {}  # by the shape of a call: see _plan
+        status_ptr(k.device.index)  # made here, so that a call's capture finds it
 
     @classmethod
     def empty(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,

@@ -90,3 +90,58 @@ def test_value_scales_that_are_not_positive_numbers(G, Tq, D):
         assert torch.isnan(o2[0, :G]).all()
         assert torch.equal(o2[0, G:], o[0, G:]) and torch.equal(o2[1], o[1])
         assert_within("lse", lse2, rl, tl)
+
+
+CAPTURE_FIRST = """
+import torch, pallas_flexattn as pf
+from pallas_flexattn import _lib as L
+dev = torch.device("cuda", 0)
+make = lambda: pf.PagedKVCache(*[torch.randn(4, 1, 16, 64, device=dev).to(torch.bfloat16) for _ in range(2)])
+cache = None if {late} else make()
+table = torch.tensor([[0, 1]], device=dev, dtype=torch.int32)
+lens = torch.tensor([20], device=dev, dtype=torch.int32)
+q = torch.randn(1, 2, 1, 64, device=dev).to(torch.bfloat16)
+torch.cuda.synchronize()
+stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+if {late}:
+    pools = [torch.randn(4, 1, 16, 64, device=dev).to(torch.bfloat16) for _ in range(2)]
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            pf.PagedKVCache(*pools)
+    except RuntimeError as e:
+        assert "check_device_status" in str(e), e
+    else:
+        raise SystemExit("made a status word inside a capture")
+    torch.cuda.synchronize()
+    pf.check_device_status()
+    cache, graph = make(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=stream):
+    out = pf.flash_attention_paged(q, cache, table, lens, pf.causal_mask)
+pf.check_device_status()           # nothing has run: nothing is reported
+table[0, 1] = 9
+graph.replay()                     # a page out of range
+table[0, 1] = 1
+graph.replay()                     # and one that is fine: the report of the first stays
+try:
+    pf.check_device_status()
+except L.FlexAttnError as e:
+    assert "out of range" in str(e)
+else:
+    raise SystemExit("the report of a replay was lost")
+pf.check_device_status()
+want = pf.flash_attention_paged(q, cache, table, lens, pf.causal_mask)
+assert all(torch.equal(a, b) for a, b in zip(out, want))
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("late", [False, True])
+def test_a_capture_holds_the_first_call_on_a_device(late):
+    """In a fresh process: reports of replays are neither invented nor lost."""
+    import subprocess
+    import sys
+
+    path = ["pallas-flexattn_b200" if p == "" else p for p in sys.path]
+    r = subprocess.run([sys.executable, "-c", f"import sys; sys.path[:0] = {path!r}" + CAPTURE_FIRST.format(late=late)],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr

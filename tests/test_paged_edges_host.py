@@ -2,6 +2,12 @@
 import re
 from pathlib import Path
 
+import pytest
+import torch
+
+from pallas_flexattn import _lib as L
+from pallas_flexattn import flash_attn as F
+
 CSRC = Path(__file__).resolve().parent.parent / "pallas-flexattn_b200" / "csrc"
 
 
@@ -18,3 +24,29 @@ def test_a_wait_that_gave_up_is_reported_whichever_warp_it_was():
         start = max(kernel.rindex(c, 0, at) for c in ";{}") + 1
         used = kernel[start:at].strip()
         assert used, f"a wait whose result is dropped: {kernel[at:at + 80]}"
+
+
+def test_a_status_word_of_a_capture_is_not_the_devices(monkeypatch):
+    """A word made inside a stream capture is memory of that graph: it is never cached as the device's."""
+    on = {"capturing": True}
+    zeros = torch.zeros
+    monkeypatch.setattr(F, "_STATUS", {})
+    monkeypatch.setattr(F, "_STATUS_PTR", {})
+    monkeypatch.setattr(F, "_GRAPH_STATUS", {})
+    monkeypatch.setattr(F, "_capturing", lambda dev: on["capturing"])
+    monkeypatch.setattr(torch, "zeros", lambda *a, device=None, **kw: zeros(*a, **kw))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev: type("S", (), {"synchronize": lambda self: None})())
+    with pytest.raises(RuntimeError, match="check_device_status"):
+        F.status_ptr(0)
+    graph = F.device_status("cuda:0")
+    on["capturing"] = False
+    word = F.device_status("cuda:0")
+    assert word is not graph and F.device_status("cuda:0") is word and F.status_ptr(0) == word.data_ptr()
+    on["capturing"] = True
+    assert F.device_status("cuda:0") is word and F.status_ptr(0) == word.data_ptr()
+    for w in (word, graph):
+        w.fill_(L.FA_ERR_INVALID)
+        with pytest.raises(L.FlexAttnError, match="out of range"):
+            F.check_device_status("cuda:0")
+        assert int(w) == 0
+        F.check_device_status("cuda:0")
