@@ -40,6 +40,7 @@ from collections import OrderedDict
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as fwad
 
 from . import _lib as L
 from .block_mask import BlockMask, BlockTables, build_tables_from_spec
@@ -154,6 +155,12 @@ class on_device:
     def __exit__(self, *exc):
         if self.back != self.index:
             torch._C._cuda_setDevice(self.back)
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors (or None) carries a tangent of forward-mode differentiation."""
+    return getattr(fwad, "_current_level", 0) >= 0 and any(  # (a level is open: rarely, and unpacking costs 1 us)
+        t is not None and fwad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _DTYPES = {torch.bfloat16: L.FA_DTYPE_BF16, torch.float32: L.FA_DTYPE_F32}

@@ -27,7 +27,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib as L
-from .flash_attn import _DTYPES, on_device, status_ptr
+from .flash_attn import _DTYPES, has_tangent, on_device, status_ptr
 from .mask_mod import MaskMod
 from .mask_mod import spec_of as mask_spec_of
 from .rotary import RotarySpec
@@ -187,6 +187,8 @@ def paged_kv_append(cache: PagedKVCache, block_table: torch.Tensor, kv_lens: Len
         raise ValueError(f"head dim {D}, but the rotary_spec is for {rotary.head_dim}")
     if (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)) and torch.is_grad_enabled():
         raise ValueError("paged_kv_append has no gradient: call it under torch.no_grad()")
+    if has_tangent(k, v, q):
+        raise ValueError("paged_kv_append has no gradient: its inputs cannot carry tangents")
     out, heads, fq, fo = None, 0, _NONE, _NONE
     if q is not None:
         out = _out_like(q)
@@ -260,6 +262,8 @@ def flash_attention_paged(q: torch.Tensor, cache: PagedKVCache, block_table: tor
         raise ValueError(f"H={H} must be a multiple of the K/V heads {hkv}")
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("flash_attention_paged has no gradient: call it under torch.no_grad()")
+    if has_tangent(q):
+        raise ValueError("flash_attention_paged has no gradient: q cannot carry a tangent")
     mspec = mask_spec_of(mask_mod)
     if mspec is None or mspec.flags & ~(L.FA_MASK_CAUSAL | L.FA_MASK_WINDOW):
         raise NotImplementedError("paged attention takes None, causal_mask, sliding_window_mask or their and_masks")

@@ -8,7 +8,8 @@ the angle ``p * f[i]`` radians and scaled by a magnitude ``m``::
 The pairs are ``(x[i], x[i + rotary_dim / 2])`` (half layout) or ``(x[2 i], x[2 i + 1])``
 (interleaved); elements from ``rotary_dim`` on are copied.  The frequencies are ``f[i] =
 base ** (-2 i / rotary_dim)``, stretched for long contexts by one of the scalings below.  The
-gradient is the transposed rotation, run by the same kernel with the angle negated.
+gradient is the transposed rotation, run by the same kernel with the angle negated, and tangents of
+forward-mode differentiation turn like their primals.
 
 The kernel holds each ``f[i]`` as a 64-bit fixed-point fraction of a turn and reduces the angle
 with integer arithmetic, so it is as exact at position 2^30 as at position 1.  bf16 and fp32
@@ -25,7 +26,7 @@ from typing import Callable, List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib as L
-from .flash_attn import _DTYPES, on_device
+from .flash_attn import _DTYPES, has_tangent, on_device
 
 _PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
 
@@ -201,6 +202,7 @@ class _Rotary(torch.autograd.Function):
         tensor = isinstance(positions, torch.Tensor)
         if tensor:  # saved, so that a change in place before the backward pass is an error
             ctx.save_for_backward(positions)
+            ctx.save_for_forward(positions)
         ctx.args = (spec, None if tensor else positions, inverse)
         return _launch(q, k, spec, positions, inverse)
 
@@ -212,9 +214,26 @@ class _Rotary(torch.autograd.Function):
         if dq is None and dk is None:
             return None, None, None, None, None
         # linear, so its own gradient is the same operator turned back
-        turn = _Rotary.apply if torch.is_grad_enabled() else _launch
-        gq, gk = turn(dq, dk, spec, positions, not inverse)
+        gq, gk = _turn(dq, dk, spec, positions, not inverse)
         return gq, gk, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        spec, positions, inverse = ctx.args
+        if ctx.saved_tensors:
+            positions, = ctx.saved_tensors
+        return _turn(tq, tk, spec, positions, inverse)  # linear: a tangent turns like its primal
+
+
+def _turn(q, k, spec: RotarySpec, positions: Positions, inverse: bool):
+    """_launch, differentiable where something asks for it."""
+    tangent = has_tangent(q, k)
+    if tangent and q is not None and k is not None and not (has_tangent(q) and has_tangent(k)):
+        # a call of its own each: either all outputs of a call have tangents or none
+        return _Rotary.apply(q, None, spec, positions, inverse)[0], _Rotary.apply(None, k, spec, positions, inverse)[1]
+    if tangent or (torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k))):
+        return _Rotary.apply(q, k, spec, positions, inverse)
+    return _launch(q, k, spec, positions, inverse)
 
 
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], rotary: RotarySpec,
@@ -237,6 +256,4 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], rotary: RotaryS
             positions = positions.to(device=q.device, dtype=torch.int32).contiguous()
     elif positions is not None and not -(1 << 31) <= int(positions) <= (1 << 31) - 1 - q.shape[2]:
         raise ValueError("positions must fit 32 bits")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, rotary, positions, False)
-    return _launch(q, k, rotary, positions, False)
+    return _turn(q, k, rotary, positions, False)

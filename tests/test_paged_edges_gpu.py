@@ -8,7 +8,7 @@ import torch
 import pallas_flexattn as pf
 from pallas_flexattn import _lib as L
 from pallas_flexattn.flash_attn import check_device_status
-from paged_reference import assert_within, attend64
+from paged_reference import assert_within, attend64, rotate64, unit
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0) if torch.cuda.is_available() else None
@@ -145,3 +145,35 @@ def test_a_capture_holds_the_first_call_on_a_device(late):
     r = subprocess.run([sys.executable, "-c", f"import sys; sys.path[:0] = {path!r}" + CAPTURE_FIRST.format(late=late)],
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("which", ["q", "k", "both"])
+def test_tangents_of_the_rotation(which, dtype):
+    """Forward-mode tangents are the rotated tangents, also through a gradient taken backwards."""
+    fw = torch.autograd.forward_ad
+    g = torch.Generator().manual_seed(1)
+    spec = pf.rotary_spec(64, rotary_dim=32, scaling=pf.by_parts_scaling(4.0, 64))
+    q, tq, w, tw = (torch.randn(2, 4, 9, 64, generator=g).to(DEV, dtype) for _ in range(4))
+    k, tk = (torch.randn(2, 2, 9, 64, generator=g).to(DEV, dtype) for _ in range(2))
+    pos = torch.randint(0, 10 ** 6, (9,), generator=g).to(DEV, torch.int32)
+
+    def check(got, x, inverse=False):
+        want, err = rotate64(x, spec, pos, inverse)
+        assert_within("tangent", got, want, err + unit(dtype) * want.abs())
+
+    q.requires_grad_(True)
+    with fw.dual_level():
+        dq = fw.make_dual(q, tq) if which != "k" else q
+        dk = fw.make_dual(k, tk) if which != "q" else k
+        oq, ok = pf.rotary_embedding(dq, dk, spec, pos)
+        check(fw.unpack_dual(oq).primal, q.detach())
+        check(fw.unpack_dual(ok).primal, k)
+        for o, t, has in ((oq, tq, which != "k"), (ok, tk, which != "q")):
+            if has:
+                check(fw.unpack_dual(o).tangent.detach(), t)
+            else:
+                assert fw.unpack_dual(o).tangent is None
+        gq, = torch.autograd.grad(oq, q, fw.make_dual(w, tw))
+        check(fw.unpack_dual(gq).primal, w, True)
+        check(fw.unpack_dual(gq).tangent, tw, True)

@@ -5,8 +5,12 @@ from pathlib import Path
 import pytest
 import torch
 
+import pallas_flexattn as pf
+from paged_reference import rotate64
 from pallas_flexattn import _lib as L
 from pallas_flexattn import flash_attn as F
+from pallas_flexattn import paged as P
+from pallas_flexattn import rotary as R
 
 CSRC = Path(__file__).resolve().parent.parent / "pallas-flexattn_b200" / "csrc"
 
@@ -50,3 +54,54 @@ def test_a_status_word_of_a_capture_is_not_the_devices(monkeypatch):
             F.check_device_status("cuda:0")
         assert int(w) == 0
         F.check_device_status("cuda:0")
+
+
+def _plain_launch(q, k, spec, positions, inverse):
+    pos = positions if positions is not None else torch.arange((q if q is not None else k).shape[2])
+    plain = [None if x is None else torch.from_numpy(torch.autograd.forward_ad.unpack_dual(x).primal.detach().numpy().copy())
+             for x in (q, k)]  # as opaque to differentiation as a kernel
+    return tuple(None if x is None else rotate64(x, spec, pos, inverse)[0].to(x.dtype) for x in plain)
+
+
+@pytest.mark.parametrize("case", ["q", "k", "both", "no_grad", "requires_grad", "given"])
+def test_tangents_of_the_rotation(monkeypatch, case):
+    """Forward-mode tangents turn like their primals (the launch is replaced by the formula)."""
+    fw = torch.autograd.forward_ad
+    monkeypatch.setattr(R, "_launch", _plain_launch)
+    monkeypatch.setattr(R, "_check_qk", lambda q, k, spec: None)
+    spec = pf.rotary_spec(16, rotary_dim=8, interleaved=True, scaling=pf.by_parts_scaling(4.0, 64))
+    g = torch.Generator().manual_seed(0)
+    q, k, tq, tk = (torch.randn(1, 2, 5, 16, generator=g, dtype=torch.float64) for _ in range(4))
+    pos = torch.tensor([4, 0, 9, 100, 7], dtype=torch.int32) if case == "given" else None
+    q.requires_grad_(case == "requires_grad")
+    with fw.dual_level(), torch.set_grad_enabled(case != "no_grad"):
+        dq = fw.make_dual(q, tq) if case != "k" else q
+        dk = fw.make_dual(k, tk) if case != "q" else k
+        oq, ok = R.rotary_embedding(dq, dk, spec, pos)
+        want = _plain_launch(tq, tk, spec, pos, False)
+        for o, d, w in ((oq, dq, want[0]), (ok, dk, want[1])):
+            t = fw.unpack_dual(o).tangent
+            if fw.unpack_dual(d).tangent is None:
+                assert t is None
+            else:
+                assert torch.allclose(t, w, atol=1e-12)
+    if case == "requires_grad":
+        gq, = torch.autograd.grad(oq, q, tq)
+        assert torch.allclose(gq, _plain_launch(tq, None, spec, pos, True)[0], atol=1e-12)
+
+
+def test_tangents_are_refused_where_there_is_no_gradient():
+    """Appends and paged attention have no gradient, so neither a tangent."""
+    fw = torch.autograd.forward_ad
+    x = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)
+    cache = P.PagedKVCache.__new__(P.PagedKVCache)
+    cache._shape, cache._device, cache._plans = (1, 1, 16, 64), torch.device("cpu"), {}
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), [1]
+    with fw.dual_level(), torch.no_grad():
+        d = fw.make_dual(x, x)
+        for call in (lambda: P.flash_attention_paged(d, cache, table, lens),
+                     lambda: P.paged_kv_append(cache, table, lens, d, x),
+                     lambda: P.paged_kv_append(cache, table, lens, x, d),
+                     lambda: P.paged_kv_append(cache, table, lens, x, x, q=d)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
