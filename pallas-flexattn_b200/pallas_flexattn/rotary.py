@@ -19,6 +19,7 @@ dimension (rows that 16-byte accesses do not fit take a slower kernel).  There i
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass, field
 from fractions import Fraction
 from typing import Callable, List, Optional, Sequence, Tuple, Union
@@ -254,6 +255,11 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], rotary: RotaryS
             positions = positions[0]
         if positions.device != q.device or positions.dtype != torch.int32 or positions.stride(-1) != 1:
             positions = positions.to(device=q.device, dtype=torch.int32).contiguous()
-    elif positions is not None and not -(1 << 31) <= int(positions) <= (1 << 31) - 1 - q.shape[2]:
-        raise ValueError("positions must fit 32 bits")
+    elif positions is not None:
+        try:
+            positions = operator.index(positions)
+        except TypeError:
+            raise ValueError(f"positions must be a tensor, an int or None, got {type(positions).__name__}") from None
+        if not -(1 << 31) <= positions <= (1 << 31) - q.shape[2]:
+            raise ValueError("positions must fit 32 bits")
     return _turn(q, k, rotary, positions, False)

@@ -2,6 +2,7 @@
 import re
 from pathlib import Path
 
+import numpy as np
 import pytest
 import torch
 
@@ -105,3 +106,14 @@ def test_tangents_are_refused_where_there_is_no_gradient():
                      lambda: P.paged_kv_append(cache, table, lens, x, x, q=d)):
             with pytest.raises(ValueError, match="tangent"):
                 call()
+
+
+def test_positions_that_are_no_integers_are_refused(monkeypatch):
+    monkeypatch.setattr(R, "_launch", lambda q, k, spec, positions, inverse: positions)
+    monkeypatch.setattr(R, "_check_qk", lambda q, k, spec: None)
+    spec, q = pf.rotary_spec(16), torch.zeros(1, 1, 3, 16)
+    for bad in (2.5, "4", [1, 2, 3], 1e20, object(), (1 << 31) - 2, -(1 << 31) - 1):
+        with pytest.raises(ValueError, match="positions"):
+            R.rotary_embedding(q, None, spec, bad)
+    for good in (0, 7, -5, (1 << 31) - 3, -(1 << 31), np.int64(12)):
+        assert R.rotary_embedding(q, None, spec, good) == good
