@@ -93,19 +93,30 @@ class RotarySpec:
 
     def turns(self, device: torch.device) -> torch.Tensor:
         """Fractions of a turn per position, in units of 2^-64 turns, on `device` (cached)."""
-        t = self._dev.get(device)
-        if t is None:
-            t = self._dev[device] = self._dev["host"].to(device)
-        return t
+        return self._on(device)[0]
+
+    def _on(self, device: torch.device) -> tuple:
+        """(turns on `device`, their address, streams that read them)."""
+        on = self._dev.get(device)
+        if on is None:
+            t = self._dev["host"].to(device)
+            on = self._dev[device] = (t, t.data_ptr(), set())
+        return on
 
     def __post_init__(self):
         bits = [round(Fraction(f) / (2 * _PI) * (1 << 64)) % (1 << 64) for f in self.frequencies]
         self._dev["host"] = torch.tensor([b - (1 << 64) if b >> 63 else b for b in bits], dtype=torch.int64)
 
     def packed(self, device: torch.device) -> tuple:
-        """The fields of an FaRotarySpec on `device`."""
-        return (self.rotary_dim, int(self.interleaved), self.turns(device).data_ptr() if self.rotary_dim else 0,
-                self.magnitude)
+        """The fields of an FaRotarySpec on `device`, for a call on its current stream."""
+        if not self.rotary_dim:
+            return (0, int(self.interleaved), 0, self.magnitude)
+        t, ptr, streams = self._dev.get(device) or self._on(device)
+        stream = torch._C._cuda_getCurrentRawStream(device.index)
+        if stream not in streams:  # memory that a dropped spec gives back waits for every stream that read it
+            t.record_stream(torch.cuda.current_stream(device))
+            streams.add(stream)
+        return (self.rotary_dim, int(self.interleaved), ptr, self.magnitude)
 
 
 def rotary_spec(head_dim: int, *, rotary_dim: Optional[int] = None, base: float = 10000.0, interleaved: bool = False,
@@ -262,4 +273,6 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], rotary: RotaryS
             raise ValueError(f"positions must be a tensor, an int or None, got {type(positions).__name__}") from None
         if not -(1 << 31) <= positions <= (1 << 31) - q.shape[2]:
             raise ValueError("positions must fit 32 bits")
-    return _turn(q, k, rotary, positions, False)
+    if has_tangent(q, k) or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+        return _turn(q, k, rotary, positions, False)
+    return _launch(q, k, rotary, positions, False)

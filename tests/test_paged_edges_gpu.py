@@ -177,3 +177,27 @@ def test_tangents_of_the_rotation(which, dtype):
         gq, = torch.autograd.grad(oq, q, fw.make_dual(w, tw))
         check(fw.unpack_dual(gq).primal, w, True)
         check(fw.unpack_dual(gq).tangent, tw, True)
+
+
+def test_a_spec_may_be_dropped_while_another_stream_still_reads_it():
+    """The table of a rotary_spec, made by its first call, is not handed out again before calls on other
+    streams have read it."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(1, 2, 16, 128, generator=g).to(DEV, BF16)
+    want, _ = pf.rotary_embedding(x, None, pf.rotary_spec(128))
+    other = torch.cuda.Stream()
+    spec = pf.rotary_spec(128)
+    pf.rotary_embedding(x, None, spec)
+    torch.empty(64, dtype=torch.int64, device=DEV).fill_(1)  # (a kernel's first launch waits for the device)
+    torch.cuda.synchronize()
+    at = spec.turns(DEV).data_ptr()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(200_000_000)  # some 100 ms
+        got, _ = pf.rotary_embedding(x, None, spec)
+    del spec
+    new = [torch.empty(64, dtype=torch.int64, device=DEV) for _ in range(2000)]  # on the first stream
+    for n in new:
+        if n.data_ptr() == at:
+            n.fill_(1 << 60)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
