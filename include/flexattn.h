@@ -358,7 +358,7 @@ typedef struct {
   int32_t B, H, T;          /* H may be 0 (no q) */
   FaTensor q, k, v, q_out;  /* [B, H, T, D], [B, H_kv, T, D] */
   const int32_t* kv_lens;   /* [B] device */
-  const int32_t* new_lens;  /* [B] device, or NULL: T */
+  const int32_t* new_lens;  /* [B] device, or NULL: T, and 0 where kv_lens[b] is 0 (an empty slot) */
   FaRotarySpec rotary;      /* rotary_dim a multiple of 16 */
   FaPagedCache cache;
   int32_t* status;

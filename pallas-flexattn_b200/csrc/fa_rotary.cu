@@ -314,10 +314,10 @@ struct AppendArgs {
   int* status;
 };
 
-// The span of new positions [*start, *len) of sequence b; false (and a status) when its lengths
-// are out of range.
+// The span of new positions [*start, *len) of sequence b, none where the batch has an empty slot; false (and a
+// status) when its lengths are out of range.
 __device__ __forceinline__ bool new_span(const AppendArgs& a, int b, int* start, int* len) {
-  const int n = __ldg(a.kv_lens + b), t = a.new_lens ? __ldg(a.new_lens + b) : a.T;
+  const int n = __ldg(a.kv_lens + b), t = a.new_lens ? __ldg(a.new_lens + b) : n == 0 ? 0 : a.T;
   *start = n - t;
   *len = n;
   const bool ok = t >= 0 && t <= a.T && n >= t && n <= a.cols * a.ps;

@@ -15,8 +15,9 @@ A step of a server is two calls::
 of a padded batch (None: all T), so row ``i`` of sequence ``b`` sits at position ``kv_lens[b] -
 new[b] + i``.  Both calls read the lengths on the device and never wait for it, so one captured
 CUDA graph serves every length up to the table's.  A sequence with ``kv_lens`` 0 is an empty
-slot of the batch.  Page numbers and lengths out of range are skipped on the device and
-reported by ``check_device_status``.  There is no CPU path.
+slot of the batch (without ``new`` too).  Page numbers and lengths out of range are reported by
+``check_device_status``: an append writes nothing for them, attention hides such a page and cuts such
+a length to what there is.  There is no CPU path.
 """
 from __future__ import annotations
 

@@ -201,3 +201,28 @@ def test_a_spec_may_be_dropped_while_another_stream_still_reads_it():
             n.fill_(1 << 60)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("T", [1, 3, 70])
+def test_empty_slots_without_new_lens(T, dtype):
+    """kv_lens 0 is an empty slot in both calls of a step, whether or not new_lens says so."""
+    g = torch.Generator().manual_seed(T)
+    B, lens, spec = 4, [0, T + 5, 0, T], pf.rotary_spec(64)
+    q, k, v = (torch.randn(B, h, T, 64, generator=g).to(DEV, BF16) for h in (4, 2, 2))
+    table = torch.arange(B * 6, device=DEV, dtype=torch.int32).view(B, 6)
+    results = []
+    for new in (None, [0, T, 0, T]):
+        cache = cache_of(B * 6, 2, 16, 64, dtype, torch.Generator().manual_seed(7))
+        before = cache.k.clone()
+        rq = pf.paged_kv_append(cache, table, lens, k, v, new_lens=new, rotary=spec, q=q)
+        o, lse = pf.flash_attention_paged(rq, cache, table, lens, pf.causal_mask, q_lens=new)
+        check_device_status(DEV)
+        for b in (0, 2):
+            assert torch.all(rq[b] == 0) and torch.all(o[b] == 0) and torch.all(lse[b] == -math.inf)
+            assert torch.equal(cache.k[table[b].long()].float(), before[table[b].long()].float())
+        results.append((rq, o, lse, cache.k.float(), cache.v.float()))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    pf.paged_kv_append(cache, table, lens, k, v, new_lens=[T] * B)  # tokens for a sequence without a length
+    with pytest.raises(L.FlexAttnError, match="out of range"):
+        check_device_status(DEV)
