@@ -350,7 +350,7 @@ typedef struct {
  * holds rows of the sequence) and the least power of two >= (largest finite new magnitude) / 448;
  * when it grows, the rows held are requantised.  Magnitudes above 448 * scale (infinities) are
  * stored as +-448, NaN as NaN.  Rows behind the new tokens are left as they were.
- * A page that is written must belong to one sequence of the call only.
+ * A page that is written must be listed once in the tables of the call.
  * Lengths or page numbers out of range write nothing (that sequence, that page) and set
  * *status to FA_ERR_INVALID. */
 typedef struct {

@@ -134,12 +134,19 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(3) == 1 else t.contiguous()
 
 
+def _int32(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """x as int32 on `dev`; what does not fit becomes the nearest int32, which is out of range as well."""
+    if x.element_size() > 4 or x.dtype is torch.uint32:
+        x = x.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
+    return x.to(device=dev, dtype=torch.int32).contiguous()
+
+
 def _lengths(name: str, x: Lengths, B: int, dev: torch.device) -> torch.Tensor:
     if not (isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.device == dev and x.is_contiguous()):
         x = torch.as_tensor(x)
         if x.is_floating_point() or x.dtype == torch.bool:
             raise ValueError(f"{name} must be integers")
-        x = x.to(device=dev, dtype=torch.int32).contiguous()
+        x = _int32(x, dev)
     if x.shape != (B,):
         raise ValueError(f"{name} must have shape ({B},), got {tuple(x.shape)}")
     return x
@@ -151,7 +158,7 @@ def _table(t: torch.Tensor, B: int, dev: torch.device) -> torch.Tensor:
     if t.dtype is not torch.int32 and (t.is_floating_point() or t.dtype == torch.bool):
         raise ValueError("block_table must be integers")
     if t.dtype is not torch.int32 or t.device != dev or t.stride(1) != 1:
-        t = t.to(device=dev, dtype=torch.int32).contiguous()
+        t = _int32(t, dev)
     return t
 
 
@@ -169,7 +176,7 @@ def paged_kv_append(cache: PagedKVCache, block_table: torch.Tensor, kv_lens: Len
     the sequence) and the least power of two that fits the largest new magnitude; when it grows,
     the positions held are requantised.  Values beyond the 8-bit range (infinities) are stored as
     the largest one.  Positions behind the new tokens are left as they were.  Each written page
-    must belong to one sequence of the batch.
+    must be listed once in the tables of the batch.
     """
     if k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"k and v must be (B, H_kv, T, D), got {tuple(k.shape)} and {tuple(v.shape)}")

@@ -117,3 +117,20 @@ def test_positions_that_are_no_integers_are_refused(monkeypatch):
             R.rotary_embedding(q, None, spec, bad)
     for good in (0, 7, -5, (1 << 31) - 3, -(1 << 31), np.int64(12)):
         assert R.rotary_embedding(q, None, spec, good) == good
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint32, torch.int32, torch.int16])
+def test_numbers_beyond_32_bits_stay_out_of_range(dtype):
+    """Lengths and page numbers are handed to the kernels as 32 bits: one that does not fit must not wrap into range."""
+    cpu = torch.device("cpu")
+    values = [0, 5, 300]
+    if dtype == torch.int64:
+        values += [(1 << 32) + 5, -(1 << 32), 1 << 62, -(1 << 62), (1 << 31) - 1, -1]
+    if dtype == torch.uint32:
+        values += [(1 << 32) - 2]
+    x = torch.tensor(values, dtype=dtype)
+    lo, hi = -(1 << 31), (1 << 31) - 1
+    want = [min(max(v, lo), hi) for v in values]
+    for got in (P._lengths("kv_lens", x, len(values), cpu), P._table(x[:, None], len(values), cpu)[:, 0]):
+        assert got.dtype == torch.int32 and got.tolist() == want
+    assert P._lengths("kv_lens", values, len(values), cpu).tolist() == want
