@@ -305,20 +305,29 @@ size_t paged_smem_bytes(int slots) {
 // legitimate wait of this kind is that of a tile or a unit's Q operand, microseconds.  Only the warp
 // that builds Q waits for whole units, with mbar_wait's bound on time.  No clock here: two dozen waits
 // in line fill the instruction cache, and the shorter one took 10 % off the windowed case.
+// A warp's lanes may leave the polls one by one, and what follows a wait is for whole warps (tcgen05.ld and
+// bar.sync are .aligned): so they meet again here.  Called by whole warps only.
 constexpr uint32_t kSpins = 1u << 20;
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  bool there = false;
 #pragma unroll 1
   for (uint32_t n = 0; n < kSpins; ++n) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
+    there = mbar_try_wait(bar, parity);
+    if (there || *abort_flag) break;
   }
-  return false;
+  __syncwarp();
+  return there;
 }
 __device__ __forceinline__ bool wait_for_w(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   const int ok = wait_for(bar, parity, abort_flag) ? 1 : 0;
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// A named barrier for whole warps, whose lanes may come from a branch.
+__device__ __forceinline__ void bar_sync_w(int id, int nthreads) {
+  __syncwarp();
+  named_bar_sync(id, nthreads);
+}
 __device__ __forceinline__ bool vote_or(int id, int nthreads, bool pred) {
   uint32_t r;
   asm volatile(
@@ -852,7 +861,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       if (!ok) break;
       if (lane == 0) sm.rc[buf].sg = sg;
       if (seg == 0) {
-        named_bar_sync(6, NSM + 32);
+        bar_sync_w(6, NSM + 32);
       } else {
         build_rows<R>(a, wk.e, sg.hk, sm.rc[buf], lane, 32);
         __syncwarp();
@@ -880,10 +889,10 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     constexpr int CH = 4;        // rows worked on together; the ones behind the last real row are left out
     if (my_tiles > 0) {
       build_rows<R>(a, sm.start.e, sm.start.hk, sm.rc[0], tid, NSM);
-      named_bar_sync(5, NSM);
+      bar_sync_w(5, NSM);
       build_q<D, ES, R, NSM>(a, sQ, sm.rc[0], tid);
       fence_proxy_async_smem();
-      named_bar_sync(6, NSM + 32);
+      bar_sync_w(6, NSM + 32);
     }
     int j = 0;
     uint32_t posts = 0;  // parity of the next phase of the `posted` barriers, one bit each
@@ -994,7 +1003,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
               if (lane == n) reinterpret_cast<float*>(&rs.red[n])[warp & 3] = m;
             }
           }
-          named_bar_sync(bar, 128);
+          bar_sync_w(bar, 128);
           uint32_t may = 0;
           if (t < (SKIP ? (rr + CH - 1) & -CH : C)) {  // (rows worked on, real or not: an unset one would ask to move again)
             const float old = rs.m[t];
@@ -1015,7 +1024,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
             may = __reduce_or_sync(0xffffffffu, may);
             if (lane == 0) rs.watch = rs.far ? 0u : may;
           }
-          named_bar_sync(bar, 128);
+          bar_sync_w(bar, 128);
 #pragma unroll
           for (int c = 0; c < C; c += CH) {
             if (SKIP && c >= rr) continue;
@@ -1138,7 +1147,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         }
       }
       if (writer) {
-        named_bar_sync(bar, 128);
+        bar_sync_w(bar, 128);
         if (both && !wait_for(sm.posted + (seg & 1), (posts >> (seg & 1)) & 1u, abort_flag)) *abort_flag = 1;
         const bool whole = sg.first && sg.last;
         const int part = 2 * cta + (seg == 0 ? 0 : 1);
@@ -1175,8 +1184,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         // The last P V, and so all before it (one thread's MMAs end in order).
         if (!wait_for(sm.o_full + ((j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag)) *abort_flag = 1;
         tc_fence_after();
-        named_bar_sync(bar, 128);
-        const bool good = !*abort_flag;
+        bar_sync_w(bar, 128);
+        const bool good = !__any_sync(0xffffffffu, *abort_flag);
         if (D >= 128 || (warp & 3) < 2) {
           const uint32_t t_other = t_lane + S::TM_O + ((seg & 1) * 2 + (set ^ 1)) * S::ON + c0;
 #pragma unroll 1
@@ -1224,7 +1233,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         mbar_arrive(sm.q_empty + (seg & 1));
       }
       // The references are set anew when all of their readers are here.
-      named_bar_sync(bar, 128);
+      bar_sync_w(bar, 128);
     }
   }
   tc_fence_before();
@@ -1232,6 +1241,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
   // every warp's waits are behind: one that gave up shows here, whichever it was
   if (tid == 0 && *abort_flag) report_status(a.status, FA_ERR_TIMEOUT);
   if (warp == W_S) {
+    __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, S::TM_COLS);
   }
