@@ -283,7 +283,10 @@ template <int R> struct Smem {
   float2 scales[kScaleRing][8];  // (ks, |vs|) of a tile's pages; ks = -inf hides the page; vs may be kScaleless
   uint32_t turned[kScaleRing][8];  // what becomes of a page's V codes: 0 (they stay), kZeros, kSigns, kNaNs
   int odd[kScaleRing];           // kCleared, kFar: what the tile's pages ask for beside the common path
-  uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], posted[2], done[2], fin_bar[2];
+  // A slot's loads of K and of V complete on a barrier each: where the ring has an odd number of slots, a slot
+  // holds K and V in turn, and a reader that waits for K by the parity of a common barrier would pass while
+  // the slot's V before it has not landed (its own readers may be behind).
+  uint64_t full_k[kMaxSlots], full_v[kMaxSlots], empty[kMaxSlots], s_full[2], p_full[2], o_full[2], q_full[2], q_empty[2], posted[2], done[2], fin_bar[2];
   int scan[24];
   Start start;
   // the unit whose first part this CTA holds: how many parts it has (0: no such unit), the first one's
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
   extern __shared__ unsigned char dsm_raw[];
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
-  const int NS = a.slots;
+  const int NS = a.slots, turn = NS & 1 ? NS : NS / 2;  // tiles until K (or V) comes to the same slot again
   unsigned char* sQ = base + (size_t)NS * S::SLOT;
   unsigned char* sP = sQ + 2 * S::QBUF;
   Smem<R>& sm = *reinterpret_cast<Smem<R>*>(sP + 2 * S::PBUF);
@@ -543,7 +546,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
   // ---------------------------------------------------------------- setup: barriers, TMEM, range
   if (tid == NT - 1) {  // (the first warps have entries to count)
     for (int i = 0; i < NS; ++i) {
-      mbar_init(sm.full + i, 1);
+      mbar_init(sm.full_k + i, 1);
+      mbar_init(sm.full_v + i, 1);
       mbar_init(sm.empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -698,13 +702,14 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         for (int kv = kv0; kv < 2; kv += STEP) {
           ok = wait_for_w(sm.empty + slot, phase, abort_flag);
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(sm.full + slot, bytes);
+          uint64_t* const full = (kv ? sm.full_v : sm.full_k) + slot;
+          if (lane == 0) mbar_expect_tx(full, bytes);
           __syncwarp();
           if (sub == k && x.active) {
             unsigned char* dst = base + (size_t)slot * S::SLOT + (size_t)(pg << a.ps_log) * SW;
 #pragma unroll
             for (int p = 0; p < S::ROWB / SW; ++p)
-              tma_load_4d(dst + p * S::PANEL, kv ? &tv : &tk, sm.full + slot, p * (SW / ES), 0, x.hk, page);
+              tma_load_4d(dst + p * S::PANEL, kv ? &tv : &tk, full, p * (SW / ES), 0, x.hk, page);
           }
           if (kv == 0) {
             // The scales are there before the slot's barrier can complete.  Their place in the ring is
@@ -726,7 +731,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
                              (((far >> (k << ppt_log)) & pages) ? kFar : 0);
             __syncwarp();
           }
-          if (lane == 0) mbar_arrive(sm.full + slot);
+          if (lane == 0) mbar_arrive(full);
           issued += STEP;
           slot += STEP;
           if (slot >= NS) {
@@ -745,10 +750,12 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
     // differ, and a load that another one followed is not to be waited for: a few polls each instead.
     const int end = 2 * my_tiles;
     for (int ld = issued - STEP; ld >= 0 && ld >= (ok ? end : issued) - NS; ld -= STEP) {
+      uint64_t* const full = (ld & 1 ? sm.full_v : sm.full_k) + ld % NS;
+      const uint32_t parity = (uint32_t)(((ld >> 1) / turn) & 1);
       if (ok) {
-        if (!wait_for_w(sm.full + ld % NS, (uint32_t)((ld / NS) & 1), never) && lane == 0) *abort_flag = 1;
+        if (!wait_for_w(full, parity, never) && lane == 0) *abort_flag = 1;
       } else {
-        for (int n = 0; n < 1000 && !mbar_try_wait(sm.full + ld % NS, (uint32_t)((ld / NS) & 1)); ++n) __nanosleep(1000);
+        for (int n = 0; n < 1000 && !mbar_try_wait(full, parity); ++n) __nanosleep(1000);
         __syncwarp();
       }
     }
@@ -767,7 +774,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       const uint32_t qb = q_lo + (uint32_t)(((seg & 1) * S::QBUF) >> 4);
       for (int it = 0; ok && it < nt; ++it, ++j) {
         if (j >= 2) ok = wait_for_w(sm.p_full + (j & 1), (uint32_t)(((j >> 1) - 1) & 1), abort_flag);
-        ok = ok && wait_for_w(sm.full + slot, phase, abort_flag);
+        ok = ok && wait_for_w(sm.full_k + slot, phase, abort_flag);
         if (!ok) break;
         tc_fence_after();
         const uint32_t ka = slot_k + (uint32_t)((slot * S::SLOT) >> 4);
@@ -784,10 +791,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         tc_commit_w(sm.s_full + (j & 1));
         tc_commit_w(sm.empty + slot);
         slot += 2;
-        if (slot >= NS) {
-          slot -= NS;
-          phase ^= 1u;
-        }
+        if (slot >= NS) slot -= NS;
+        if (slot == 0) phase ^= 1u;
       }
       tc_commit_w(sm.q_empty + (seg & 1));
     }
@@ -816,7 +821,7 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
       // the unit before last, which used the same O, has been written
       if (TURNS && seg >= 2) ok = ok && wait_for_w(sm.done + (seg & 1), (uint32_t)(((seg >> 1) - 1) & 1), abort_flag);
       for (int it = 0; ok && it < nt; ++it, ++j) {
-        ok = wait_for_w(sm.full + slot, phase, abort_flag) &&
+        ok = wait_for_w(sm.full_v + slot, phase, abort_flag) &&
              wait_for_w(sm.p_full + (j & 1), (uint32_t)((j >> 1) & 1), abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -839,10 +844,8 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
         tc_commit_w(sm.o_full + (j & 1));
         tc_commit_w(sm.empty + slot);
         slot += 2;
-        if (slot >= NS) {
-          slot -= NS;
-          phase ^= 1u;
-        }
+        if (slot >= NS) slot -= NS;
+        if (slot == 1 % NS) phase ^= 1u;
       }
     }
     if (!ok && lane == 0) *abort_flag = 1;
@@ -1106,20 +1109,20 @@ __global__ void __launch_bounds__((Shape<D, ES, R>::NT), 1)
           // has landed.  The sign of a negative scale goes to the codes, and a NaN or an infinity makes
           // them NaN.
           const int ld = 2 * j + 1, slot = ld % NS;
-          if (!wait_for(sm.full + slot, (uint32_t)((ld / NS) & 1), abort_flag)) *abort_flag = 1;
+          if (!wait_for(sm.full_v + slot, (uint32_t)((j / turn) & 1), abort_flag)) *abort_flag = 1;
           const bool clears = half == 0;  // one group does
           const bool seen_here = pos >= sg.lo && pos <= sg.hi;
-          const uint32_t turn = !seen_here ? kZeros : ES == 1 ? sm.turned[j % kScaleRing][my_page] : 0u;
-          if (clears && turn) {
+          const uint32_t change = !seen_here ? kZeros : ES == 1 ? sm.turned[j % kScaleRing][my_page] : 0u;
+          if (clears && change) {
             unsigned char* v = base + (size_t)slot * S::SLOT + t * SW;
 #pragma unroll 1
             for (int p = 0; p < S::ROWB / SW; ++p)
 #pragma unroll
               for (int c = 0; c < SW / 16; ++c) {
                 uint4* at = reinterpret_cast<uint4*>(v + p * S::PANEL + c * 16);
-                const uint32_t w = turn == kZeros ? 0u : turn;
+                const uint32_t w = change == kZeros ? 0u : change;
                 uint4 x = make_uint4(w, w, w, w);
-                if (ES == 1 && turn == kSigns) x.x ^= at->x, x.y ^= at->y, x.z ^= at->z, x.w ^= at->w;
+                if (ES == 1 && change == kSigns) x.x ^= at->x, x.y ^= at->y, x.z ^= at->z, x.w ^= at->w;
                 *at = x;
               }
           }
@@ -1378,6 +1381,7 @@ template <int D, int ES, int R, bool MODS>
 cudaError_t launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedArgs& a, const PagedPlan& pl,
                          cudaStream_t stream) {
   const size_t fixed = paged_smem_bytes<D, ES, R>(0), limit = 232448;
+  // (two loaders: 6, 13 or 24; an odd ring below 9 would let one take a slot by the parity of its last use but one)
   a.slots = (int)std::min<size_t>(kMaxSlots, (limit - fixed) / Shape<D, ES, R>::SLOT);
   const size_t smem = paged_smem_bytes<D, ES, R>(a.slots);
   cudaError_t e =

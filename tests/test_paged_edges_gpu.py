@@ -226,3 +226,35 @@ def test_empty_slots_without_new_lens(T, dtype):
     pf.paged_kv_append(cache, table, lens, k, v, new_lens=[T] * B)  # tokens for a sequence without a length
     with pytest.raises(L.FlexAttnError, match="out of range"):
         check_device_status(DEV)
+
+
+# B, H, Hkv, Tq, D, dtype, positions: rings of 5, 3, 5, 3 and 2 slots
+FEW_SLOTS = {
+    "f8_d256_r32": (8, 64, 2, 1, 256, F8, 16384),
+    "f8_d256_r64": (8, 64, 2, 4, 256, F8, 16384),
+    "bf16_d128_r32": (8, 64, 2, 1, 128, BF16, 16384),
+    "bf16_d256_r16": (8, 16, 2, 1, 256, BF16, 16384),
+    "bf16_d256_r32": (8, 64, 2, 1, 256, BF16, 8192),
+}
+
+
+@pytest.mark.parametrize("name", list(FEW_SLOTS))
+def test_long_walks_through_rings_of_few_slots(name):
+    """Dozens of tiles a CTA where shared memory holds two or three of them, many times: the formula and the same bits."""
+    B, H, hkv, Tq, D, dtype, n = FEW_SLOTS[name]
+    g = torch.Generator().manual_seed(len(name))
+    cols = n // 64
+    cache = cache_of(2 * cols, hkv, 64, D, dtype, g)
+    table = torch.randperm(2 * cols, generator=g)[:cols].to(DEV, torch.int32).expand(B, -1).contiguous()
+    q = torch.randn(1, H, Tq, D, generator=g).to(DEV, BF16)
+    qb = q.expand(B, -1, -1, -1).contiguous()
+    lens = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    o, lse = pf.flash_attention_paged(qb, cache, table, lens, pf.causal_mask)
+    ro, rl, to, tl = attend64(q, cache, table[:1], [n], [Tq], "causal", 0, None, 0, 1 / math.sqrt(D))
+    for b in range(B):
+        assert_within("lse", lse[b:b + 1], rl, tl)
+        assert_within("o", o[b:b + 1], ro, to)
+    for _ in range(60):
+        again = pf.flash_attention_paged(qb, cache, table, lens, pf.causal_mask)
+        assert torch.equal(again[0], o) and torch.equal(again[1], lse)
+    check_device_status(DEV)

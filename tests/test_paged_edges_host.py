@@ -1,4 +1,5 @@
 """Paged caches and rotary positions at the edges of what their calls document, without a GPU."""
+import random
 import re
 from pathlib import Path
 
@@ -134,3 +135,84 @@ def test_numbers_beyond_32_bits_stay_out_of_range(dtype):
     for got in (P._lengths("kv_lens", x, len(values), cpu), P._table(x[:, None], len(values), cpu)[:, 0]):
         assert got.dtype == torch.int32 and got.tolist() == want
     assert P._lengths("kv_lens", values, len(values), cpu).tolist() == want
+
+
+class _Barrier:
+    """An mbarrier: waits see the parity of its completed phases only."""
+
+    def __init__(self):
+        self.done = 0
+
+    def passes(self, use):
+        return (self.done & 1) == ((use + 1) & 1)
+
+
+def _walk_the_ring(slots, tiles, sets, apart, rng, loaders=1):
+    """Paged attention's ring of K and V tiles with every role at a random pace: the loader (in order, into a slot
+    whose last reader has released it; or one for K and one for V), loads that land in any order, the warp that issues S, `sets` of softmax
+    groups that take the tiles in turn, the warp that issues P V.  `apart`: a slot's loads of K and of V complete
+    on a barrier each.  Returns what went wrong, or None."""
+    turn = slots if slots & 1 else slots // 2
+    full = [[_Barrier() for _ in range(slots)] for _ in range(2)]
+    empty = [_Barrier() for _ in range(slots)]
+    holds, landed, flying = [None] * slots, set(), []
+    s_done = pv_done = 0
+    issued = list(range(loaders))  # the next load of each
+    at, ready = list(range(sets)), set()
+
+    def wait(ld):
+        return (full[ld & 1][ld % slots], (ld >> 1) // turn) if apart else (full[0][ld % slots], ld // slots)
+
+    def passes(ld):
+        bar, use = wait(ld)
+        return bar.passes(use)
+
+    while pv_done < tiles:
+        steps = [("load", k) for k, ld in enumerate(issued)
+                 if ld < 2 * tiles and (ld < slots or empty[ld % slots].passes(ld // slots - 1))]
+        steps += ["land"] * bool(flying)
+        if s_done < tiles and (s_done < 2 or s_done - 2 in ready) and passes(2 * s_done):
+            steps.append("S")
+        steps += [k for k in range(sets) if at[k] < s_done and (at[k] < 2 or pv_done > at[k] - 2)]
+        if pv_done in ready and passes(2 * pv_done + 1):
+            steps.append("PV")
+        if not steps:
+            return "deadlock"
+        step = rng.choice(steps)
+        if isinstance(step, tuple):
+            ld = issued[step[1]]
+            if empty[ld % slots].done < ld // slots:
+                return f"load {ld} into a slot in use"
+            holds[ld % slots] = ld
+            flying.append(ld)
+            issued[step[1]] += loaders
+        elif step == "land":
+            ld = flying.pop(rng.randrange(len(flying)))
+            landed.add(ld)
+            wait(ld)[0].done += 1
+        elif step in ("S", "PV"):
+            ld = 2 * s_done if step == "S" else 2 * pv_done + 1
+            if ld not in landed or holds[ld % slots] != ld:
+                return f"{step} of tile {ld >> 1} before its load has landed"
+            empty[ld % slots].done += 1
+            s_done, pv_done = s_done + (step == "S"), pv_done + (step == "PV")
+        else:
+            ready.add(at[step])
+            at[step] += sets
+    return None
+
+
+@pytest.mark.parametrize("sets", [1, 2])
+def test_the_ring_of_tiles_at_every_depth_and_any_pace(sets):
+    """With one barrier a slot, rings of 3 and 5 slots let S start on a tile that has not landed (head dim 256, and
+    bf16 of head dim 128 at 32 rows); with one for K and one for V no ring does."""
+    def faults(slots, apart, n):
+        return sum(_walk_the_ring(slots, 30, sets, apart, random.Random(seed)) is not None for seed in range(n))
+
+    for slots in range(2, 25):
+        assert faults(slots, True, 60) == 0
+        assert (faults(slots, False, 60) > 0) == (slots in (3, 5))
+    for slots in (6, 13, 24):  # two loaders: 8 rows of head dim 256, 128, 64 (odd rings below 9 would not do)
+        assert sum(_walk_the_ring(slots, 40, 2, True, random.Random(seed), 2) is not None for seed in range(60)) == 0
+    src = (CSRC / "fa_paged.cu").read_text()
+    assert "full_k[kMaxSlots], full_v[kMaxSlots]" in src
