@@ -368,7 +368,8 @@ FA_API int fa_paged_append(const FaPagedAppendParams* p, fa_stream_t stream);
 
 /* Attention of Tq query rows per sequence against the cache.  Row i < q_lens[b] sits at position
  * kv_lens[b] - q_lens[b] + i; rows from q_lens[b] on are padding and get o = 0, lse = -inf, as
- * do rows that see no key.  Any Tq (a decode step, drafted tokens, a chunk of a prompt).
+ * do rows that see no key, whatever the cache holds.  Rows before position 0 (q_lens above kv_lens) see what
+ * the mask lets them see.  Any Tq (a decode step, drafted tokens, a chunk of a prompt).
  * bf16 q and o; mask flags CAUSAL / WINDOW; score flags ALIBI / SOFTCAP.  The cached positions
  * of all sequences are dealt out evenly over the SMs, whatever their lengths; parts of one
  * sequence on several SMs meet in the workspace and are joined after a grid barrier (a

@@ -53,10 +53,10 @@
 // sums are double-buffered for that).  64 rows leave threads for one set only.
 //
 // Measured on the device (8-bit pages, H 32, H_kv 8, D 128, ragged lengths): 64 users of up to 4096
-// positions, one token each: 74 us, 5.4 TB/s, 0.83 of the measured copy rate; eight of up to 32768: 73 us,
-// 5.5 TB/s; one of 1000: 9.4 us, the launch, one tile's chain and the join.  Chunks of 512 tokens of four
-// users on up to 4096 positions: 260 us, bound by the chain of one set of softmax groups at 64 rows.
-// bf16, H 16, D 64, window 1024, ALiBi, 32 users: 45 us.
+// positions, one token each: 75 us, 5.3 TB/s, 0.82 of the measured copy rate; eight of up to 32768: 74 us,
+// 5.4 TB/s; one of 1000: 10 us, the launch, one tile's chain and the join.  Chunks of 512 tokens of four
+// users on up to 4096 positions: 265 us, bound by the chain of one set of softmax groups at 64 rows.
+// bf16, H 16, D 64, window 1024, ALiBi, 32 users: 46 us.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -1332,10 +1332,11 @@ struct PagedPlan {
 
 // Rows per group: the smallest operand width that holds every query row of a K/V head, or 64 with as
 // many groups as it takes, each reading the cache again.  32 instead of 64 where bf16 pages of head dim
-// 256 leave no room for more, and where the table's whole width makes at most eight tiles per SM: there
-// the latency of a unit counts, not the cache's bytes (40 rows at head dim 256, five users of 2777
-// positions: 27 against 34 us; 32 users of 8192: 93 against 78; a prompt chunk of 141 tiles per SM: 316
-// against 228).
+// 256 leave no room for more, and where the table's whole width makes at most eight tiles of 64 rows an SM:
+// there the latency of a unit counts, not the cache's bytes.  Measured with 32 against 64 rows (8-bit, D 128,
+// 64 query rows a K/V head, four users; us by tiles an SM): 0.9: 15 / 17, 1.7: 18 / 19, 3.5: 25 / 22, 6.9: 30 / 35,
+// 13.8: 42 / 44, 28: 69 / 62, 55: 119 / 93; bf16 and head dims 64 and 256 cross between 7 and 28 as well.  The
+// lengths are on the device, so short sequences in a wide table get the 64 rows.
 PagedPlan plan_paged(const FaPagedAttnParams* p) {
   PagedPlan pl;
   const bool f8 = p->cache.dtype == FA_DTYPE_E4M3;

@@ -7,11 +7,11 @@
 // point in turns, so p * f_i mod 2^64 is the exact phase of any 32-bit position (a product in
 // fp32 is off by 0.06 rad at position 2^20), and its top 32 bits become the reduced angle.
 //
-// Measured (bf16, D 128, 32 + 8 heads): rotation of 2 x 8192 tokens with its gradient 112 us,
-// 6.0 TB/s; one token each of 64 sequences 2.5 us, the launch.  Append of eight prompts of up to
+// Measured (bf16, D 128, 32 + 8 heads): rotation of 2 x 8192 tokens with its gradient 111 us,
+// 6.1 TB/s; one token each of 64 sequences 2.3 us, the launch.  Append of eight prompts of up to
 // 2048 tokens to 8-bit pages with q's rotation 59 us (3.6 TB/s; 34 us with 8 + 8 heads): two thirds of the
 // issue slots, and a team's chain of lengths, rows, largest magnitude and stores.  One token each of 64
-// sequences 4.0 us.
+// sequences 3.9 us.
 //
 // A thread owns a unit of 16 elements of a row: 8 + 8 elements rotary_dim / 2 apart for the half
 // layout, 16 neighbours for interleaved pairs and for the copied tail.  It computes the 8 cosines

@@ -249,7 +249,8 @@ def flash_attention_paged(q: torch.Tensor, cache: PagedKVCache, block_table: tor
     their ``and_masks``; ``score_mod`` ALiBi, softcap or both.  Any Tq: one token of a decode step,
     drafted tokens, a chunk of a prompt.  Returns ``(o, lse)``, ``o`` like ``q`` and ``lse``
     (B, H, Tq) fp32 (natural log); padding rows and rows that see no position give ``o = 0`` and
-    ``lse = -inf``.
+    ``lse = -inf``, whatever the cache holds.  Rows before position 0 (``q_lens`` above ``kv_lens``) see
+    what the mask lets them see, nothing under ``causal_mask``.
 
     Keys are hidden from a row by its mask alone: a NaN or infinity in a cached value that some row
     of the same sequence and K/V head sees reaches only what it would reach by the formula as long
