@@ -31,6 +31,7 @@ class ScoreSpec:
         return (self.flags, self.softcap, id(self.alibi_slopes), id(self.rel_bias))
 
     def device_tensors(self, device: torch.device) -> dict:
+        """The spec's tensors on `device`, for a call on its current stream."""
         k = str(device)
         if k not in self._dev:
             d = {}
@@ -38,8 +39,15 @@ class ScoreSpec:
                 d["slopes"] = self.alibi_slopes.to(device=device, dtype=torch.float32).contiguous()
             if self.rel_bias is not None:
                 d["bias"] = self.rel_bias.to(device=device, dtype=torch.float32).contiguous()
-            self._dev[k] = d
-        return self._dev[k]
+            self._dev[k] = d, set()
+        d, streams = self._dev[k]
+        if device.type == "cuda" and d:
+            stream = torch.cuda.current_stream(device)
+            if stream.cuda_stream not in streams:  # memory that a dropped spec gives back waits for every reader
+                for t in d.values():
+                    t.record_stream(stream)
+                streams.add(stream.cuda_stream)
+        return d
 
     def to_c(self, device: torch.device, H: int, Tq: int, Tkv: int) -> L.FaScoreSpec:
         s = L.FaScoreSpec()

@@ -258,3 +258,31 @@ def test_long_walks_through_rings_of_few_slots(name):
         again = pf.flash_attention_paged(qb, cache, table, lens, pf.causal_mask)
         assert torch.equal(again[0], o) and torch.equal(again[1], lse)
     check_device_status(DEV)
+
+
+def test_a_score_mod_may_be_dropped_while_another_stream_still_reads_it():
+    """The same for the slopes of an ALiBi score mod."""
+    g = torch.Generator().manual_seed(4)
+    H = 128
+    cache = cache_of(8, H, 16, 64, BF16, g)
+    table = torch.arange(8, device=DEV, dtype=torch.int32)[None]
+    q = torch.randn(1, H, 1, 64, generator=g).to(DEV, BF16)
+    lens = torch.tensor([128], device=DEV, dtype=torch.int32)
+    attend = lambda mod: pf.flash_attention_paged(q, cache, table, lens, pf.causal_mask, score_mod=mod)  # noqa: E731
+    want = attend(pf.alibi_score_mod(H))
+    mod = pf.alibi_score_mod(H)
+    attend(mod)
+    torch.empty(H, device=DEV).fill_(1)
+    torch.cuda.synchronize()
+    at = mod.__fa_spec__.device_tensors(DEV)["slopes"].data_ptr()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(200_000_000)
+        got = attend(mod)
+    del mod
+    new = [torch.empty(H, device=DEV) for _ in range(2000)]
+    for n in new:
+        if n.data_ptr() == at:
+            n.fill_(100.0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
