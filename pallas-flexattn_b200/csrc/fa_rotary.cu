@@ -700,6 +700,8 @@ int fa_rotary(const FaRotaryParams* p, fa_stream_t stream) {
   if (rc) return rc;
   if ((int64_t)p->B * p->T * ((p->D + 1) / 2) >= (int64_t)1 << 31)
     return set_last_error(FA_ERR_UNSUPPORTED, "fa_rotary: B * T * D / 2 must stay below 2^31");
+  if (!p->positions && (int64_t)p->pos_offset + p->T > (int64_t)1 << 31)
+    return set_last_error(FA_ERR_INVALID, "fa_rotary: positions from pos_offset on do not fit 32 bits");
   if ((int64_t)p->H + p->H_kv > 65535) return set_last_error(FA_ERR_UNSUPPORTED, "fa_rotary: more than 65535 heads");
   const int es = p->dtype == FA_DTYPE_F32 ? 4 : 2;
   bool vec = p->D % 16 == 0 && p->rotary.rotary_dim % 16 == 0;

@@ -1,4 +1,5 @@
 """Paged caches and rotary positions at the edges of what their calls document, without a GPU."""
+import ctypes as C
 import random
 import re
 from pathlib import Path
@@ -216,3 +217,13 @@ def test_the_ring_of_tiles_at_every_depth_and_any_pace(sets):
         assert sum(_walk_the_ring(slots, 40, 2, True, random.Random(seed), 2) is not None for seed in range(60)) == 0
     src = (CSRC / "fa_paged.cu").read_text()
     assert "full_k[kMaxSlots], full_v[kMaxSlots]" in src
+
+
+def test_rotary_offsets_that_leave_32_bits_are_refused():
+    """Token t sits at pos_offset + t, a 32-bit sum on the device."""
+    p = L.FaRotaryParams()
+    p.dtype, p.B, p.H, p.T, p.D = L.FA_DTYPE_BF16, 1, 1, 4, 64
+    p.q = p.q_out = L.FaTensor(4096, 256, 256, 64)  # never dereferenced: validation fails first
+    p.rotary = L.FaRotarySpec(64, L.FA_ROTARY_HALF, 4096, 1.0)
+    p.pos_offset = (1 << 31) - 3
+    assert L.lib().fa_rotary(C.byref(p), None) == L.FA_ERR_INVALID and b"32 bits" in L.lib().fa_last_error()
